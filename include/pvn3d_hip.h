@@ -633,6 +633,50 @@ int pvn3d_mt_bn_bwd_finalize(int P, int ld, int C, double count, const float* p1
 int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y, const float* a, const float* b,
                           const float* k1, const float* k0, void* dY, void* stream);
 
+/* ---- Layer norm over the channels of every point (csrc/layer_norm*.hip; no reference counterpart) -------------
+ * Beside the BatchNorm passes above: mean, var over a point's own channels, rstd = 1 / sqrt(var + eps),
+ * xh = (x - mean) rstd, z = weight xh + bias, y = z or (relu != 0) max(z, 0).  dtype 0 fp32, 1 bf16, 2 fp16 (x, y, dy,
+ * dx); weight, bias (either may be NULL: ones, zeros), statistics and parameter gradients fp32.  1 <= C <= 8192.
+ * pvn3d_layer_norm: rows [rows][C] of stride xs (elements, any alignment) -> y [rows] of stride ys; columns C .. y_cols - 1
+ *   (y_cols <= C + 15) are written as zeros.  codes != NULL: x also goes to codes / scales in the 8-bit form of
+ *   pvn3d_act8_pack, and mask (may be NULL) gets bit c & 7 of byte [row][c / 8], row length ceil(C / 8), = z > 0.
+ * pvn3d_layer_norm_grad: dx (NULL: not wanted; columns up to dx_cols written, zeros from C on), dweight and dbias (both or
+ *   neither).  The normalised input comes from x, or, if codes != NULL, from codes / scales (relu != 0: and the ReLU from
+ *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
+ *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C, dx_cols) names (dx NULL: C), 4-byte aligned, needed for dweight
+ *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
+ * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors; mean, rstd (B, M). */
+int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
+                     float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
+                     long long pitch, void* scales, void* mask, void* stream);
+size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C, int dx_cols);
+int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
+                          const void* codes, long long pitch, const void* scales, const void* mask, const float* weight,
+                          const float* bias, const float* mean, const float* rstd, int relu, void* dx, long long dxs,
+                          int dx_cols, float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream);
+int pvn3d_layer_norm_chan(int dtype, int B, int C, int M, const void* x, const float* weight, const float* bias, float eps,
+                          int relu, void* y, float* mean, float* rstd, void* stream);
+size_t pvn3d_layer_norm_chan_grad_workspace_bytes(int dtype, int B, int C, int M);
+int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const void* dy, const void* x, const float* weight,
+                               const float* bias, const float* mean, const float* rstd, int relu, void* dx, float* dweight,
+                               float* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Activations in 8 bits for the backward pass (csrc/act8.hip; no reference counterpart) --------------------
+ * 32 consecutive channels of a row (the last group may be shorter) share 2^e: code = rint(x 2^-e) (int8), e >= -126 the
+ * smallest with rint(absmax 2^-e) <= 127 (121 at most: codes stop at +-127 there); scales[row][c / 32] = e + 127.  A group with an infinity or a NaN: scale 255,
+ * codes 0, read back as NaN.  codes [rows] of pitch `pitch` (a multiple of 16, base 16-byte aligned; the last row ends
+ * with a whole 16-byte chunk too), scales [rows][ceil(C / 32)].  Codes behind C are not read as values.
+ * pvn3d_act8_unpack writes the held values (exact in fp32 and bf16), zeros in columns C .. y_cols - 1.
+ * pvn3d_act8_wgrad: dW [M][N] fp32 = dY^T X, dY bf16 [rows] of stride dys (M columns), X = the held values [rows][N], on
+ * v_mfma_f32_32x32x16_bf16; fixed order of the sums.  No rows: zeros. */
+int pvn3d_act8_pack(int dtype, long long rows, int C, const void* x, long long xs, void* codes, long long pitch, void* scales,
+                    void* stream);
+int pvn3d_act8_unpack(int dtype, long long rows, int C, const void* codes, long long pitch, const void* scales, void* y,
+                      long long ys, int y_cols, void* stream);
+size_t pvn3d_act8_wgrad_workspace_bytes(long long rows, int M, int N);
+int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, long long dys, const void* codes, long long pitch,
+                     const void* scales, float* dW, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -107,6 +107,19 @@ SIGNATURES = {
     "pvn3d_mt_bn_bwd_apply_pooled": (_i, [_ll, _i, _i, _i, _p, _ll, _p, _p, _p, _p, _p, _p, _p, _p]),
     "pvn3d_mt_bn_bwd_finalize": (_i, [_i, _i, _i, _d, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "pvn3d_mt_bn_bwd_apply": (_i, [_ll, _i, _p, _p, _p, _p, _p, _p, _p, _p]),
+    # layer norm over the channels (csrc/layer_norm*.hip)
+    "pvn3d_layer_norm": (_i, [_i, _ll, _i, _p, _ll, _p, _p, _f, _i, _p, _ll, _i, _p, _p, _p, _ll, _p, _p, _p]),
+    "pvn3d_layer_norm_grad_workspace_bytes": (_sz, [_i, _ll, _i, _i]),
+    "pvn3d_layer_norm_grad": (_i, [_i, _ll, _i, _p, _ll, _p, _ll, _p, _ll, _p, _p, _p, _p, _p, _p, _i, _p, _ll, _i, _p, _p,
+                                   _p, _sz, _p]),
+    "pvn3d_layer_norm_chan": (_i, [_i, _i, _i, _i, _p, _p, _p, _f, _i, _p, _p, _p, _p]),
+    "pvn3d_layer_norm_chan_grad_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "pvn3d_layer_norm_chan_grad": (_i, [_i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _sz, _p]),
+    # activations in 8 bits for the backward pass (csrc/act8.hip)
+    "pvn3d_act8_pack": (_i, [_i, _ll, _i, _p, _ll, _p, _ll, _p, _p]),
+    "pvn3d_act8_unpack": (_i, [_i, _ll, _i, _p, _ll, _p, _p, _ll, _i, _p]),
+    "pvn3d_act8_wgrad_workspace_bytes": (_sz, [_ll, _i, _i]),
+    "pvn3d_act8_wgrad": (_i, [_ll, _i, _i, _p, _ll, _p, _ll, _p, _p, _p, _sz, _p]),
 }
 
 if not os.path.exists(LIB_PATH):

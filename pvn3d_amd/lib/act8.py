@@ -1,0 +1,206 @@
+"""Activations kept in 8 bits between the forward and the backward pass, and a layer's weight gradient taken from them.
+
+``act8_pack`` / ``act8_unpack``, ``linear8_weight_grad`` and the autograd layer ``linear8`` (the 1x1 convolution of a
+SharedMLP layer, ``Conv2d`` of pvn3d/lib/utils/etw_pytorch_utils/pytorch_utils.py:80-134, on point-major rows).  One HIP
+launch each, plus one that joins the row splits of a weight gradient (csrc/act8.hip).
+
+The 8-bit form: 32 consecutive channels of a row (the last group of a row may be shorter) share a power of two 2^e and a
+value x is held as the int8 code rint(x 2^-e); e >= -126 is the smallest exponent at which the group's largest magnitude
+rounds to 127 at most, held as e + 127 in a byte (e <= 121: magnitudes from 127.5 2^121 on are held as 127 2^121).  A value is off by at most half a step, 1/128 of its group's largest
+magnitude; every held value is exact in bfloat16.  A group that holds an infinity or a NaN comes back as NaN.
+
+Everything runs on the current stream of the tensors' device and reads only its arguments; calls may be captured."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .._lib import lib, check, on_device
+
+GROUP = 32
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _need(ok, what):
+    if not ok:
+        raise RuntimeError(what)
+
+
+def _rows(t, name):
+    """(..., C) -> (2-D view or copy whose channels are contiguous, its row stride)."""
+    C = t.size(-1)
+    m = t if t.dim() == 2 else t.reshape(-1, C) if C else t.reshape(0, 0)
+    if m.stride(1) != 1 and C > 1:
+        m = m.contiguous()
+    return m, (m.stride(0) if m.size(0) > 1 else C)
+
+
+class Act8(object):
+    """A tensor (..., C) in the 8-bit form: `codes` int8 (rows, C), rows 16-byte aligned (pitch a multiple of 16, whole
+    16-byte chunks in its storage), `scales` uint8 (rows, ceil(C / 32)) contiguous, `shape` of the tensor."""
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales, shape=None):
+        _need(codes.dim() == 2 and codes.dtype == torch.int8, "codes must be an int8 matrix")
+        rows, C = codes.shape
+        _need(C > 0, "codes must have at least one channel")
+        _need(scales.dtype == torch.uint8 and tuple(scales.shape) == (rows, (C + GROUP - 1) // GROUP)
+              and scales.is_contiguous(), "scales must be a contiguous uint8 (rows, ceil(channels / 32)) matrix")
+        _need(codes.is_cuda and scales.is_cuda, "CPU not supported")
+        _need(scales.device == codes.device, "scales must be on the codes' device")
+        if rows > 0:
+            _need((codes.stride(1) == 1 or C == 1) and codes.data_ptr() % 16 == 0, "codes must have 16-byte aligned rows")
+            if rows > 1:
+                _need(codes.stride(0) % 16 == 0 and codes.stride(0) >= C, "codes must have 16-byte aligned rows")
+            last = codes.storage_offset() + (rows - 1) * codes.stride(0) + (C + 15) // 16 * 16
+            _need(codes.untyped_storage().nbytes() >= last, "codes must end with a whole 16-byte chunk")
+        if shape is not None:
+            n = 1
+            for v in shape[:-1]:
+                n *= v
+            _need(len(shape) > 0 and shape[-1] == C and n == rows, "shape does not fit the codes")
+        self.codes, self.scales = codes, scales
+        self.shape = torch.Size(shape) if shape is not None else codes.shape
+
+    @property
+    def pitch(self):
+        return self.codes.stride(0) if self.codes.size(0) > 1 else (self.codes.size(1) + 15) // 16 * 16
+
+    @property
+    def nbytes(self):
+        return self.codes.size(0) * self.pitch + self.scales.numel()
+
+    def unpack(self, dtype=torch.bfloat16):
+        return act8_unpack(self, dtype)
+
+
+def _empty_act8(rows, C, shape, dev):
+    codes = torch.empty((rows, (C + 15) // 16 * 16), dtype=torch.int8, device=dev)[:, :C]
+    scales = torch.empty((rows, (C + GROUP - 1) // GROUP), dtype=torch.uint8, device=dev)
+    return Act8(codes, scales, shape)
+
+
+def act8_pack(x):
+    """x (..., C) float32 / bfloat16 / float16 -> Act8."""
+    _need(x.is_cuda, "CPU not supported")
+    _need(x.dtype in DTYPES, "x must be a float32, bfloat16 or float16 tensor")
+    _need(x.dim() >= 1 and x.size(-1) > 0, "x must have at least one channel")
+    with on_device(x.device):
+        m, xs = _rows(x, "x")
+        act = _empty_act8(m.size(0), m.size(1), x.shape, x.device)
+        check(lib.pvn3d_act8_pack(DTYPES[x.dtype], m.size(0), m.size(1), m.data_ptr(), xs, act.codes.data_ptr(), act.pitch,
+                                  act.scales.data_ptr(), _stream(x)), "act8_pack")
+    return act
+
+
+def act8_unpack(act, dtype=torch.bfloat16):
+    """Act8 -> the held values, a contiguous tensor of its shape.  bfloat16 and float32 hold every value exactly; float16
+    does if the tensor was a float16 one (otherwise values are rounded, and overflow to infinity)."""
+    _need(isinstance(act, Act8), "act must be an Act8")
+    _need(dtype in DTYPES, "dtype must be float32, bfloat16 or float16")
+    rows, C = act.codes.shape
+    dev = act.codes.device
+    with on_device(dev):
+        out = torch.empty(act.shape, dtype=dtype, device=dev)
+        check(lib.pvn3d_act8_unpack(DTYPES[dtype], rows, C, act.codes.data_ptr(), act.pitch, act.scales.data_ptr(),
+                                    out.data_ptr(), C, C, _stream(act.codes)), "act8_unpack")
+    return out
+
+
+def linear8_weight_grad(dy, act):
+    """dW (M, N) float32 = dy^T X: dy (..., M) bfloat16, X the rows of `act` (..., N).  Exact operands, fp32 sums in a fixed
+    order (the same bits on every call); no rows: zeros."""
+    _need(dy.is_cuda, "CPU not supported")
+    _need(dy.dtype == torch.bfloat16, "dy must be a bfloat16 tensor")
+    _need(isinstance(act, Act8), "act must be an Act8")
+    _need(act.codes.device == dy.device, "act must be on dy's device")
+    _need(dy.dim() >= 1 and dy.size(-1) > 0, "dy must have at least one channel")
+    rows, N = act.codes.shape
+    M = dy.size(-1)
+    _need(dy.numel() == rows * M, "dy and act must have the same number of rows")
+    with on_device(dy.device):
+        m, ds = _rows(dy, "dy")
+        dw = torch.empty((M, N), dtype=torch.float32, device=dy.device)
+        wsb = lib.pvn3d_act8_wgrad_workspace_bytes(rows, M, N)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
+        check(lib.pvn3d_act8_wgrad(rows, M, N, m.data_ptr(), ds, act.codes.data_ptr(), act.pitch, act.scales.data_ptr(),
+                                   dw.data_ptr(), ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_wgrad")
+    return dw
+
+
+def _ld(c):
+    return (int(c) + 15) // 16 * 16
+
+
+def _padded(m, C):
+    """(rows, C) bfloat16 -> (matrix whose rows hold a multiple of 16 channels, zeros behind C, 16-byte aligned; its row
+    stride): what the matrix kernel reads."""
+    if C % 16 == 0 and m.data_ptr() % 16 == 0 and (m.size(0) <= 1 or m.stride(0) % 8 == 0):
+        return m, (m.stride(0) if m.size(0) > 1 else C)
+    out = torch.zeros((m.size(0), _ld(C)), dtype=torch.bfloat16, device=m.device)
+    out[:, :C] = m
+    return out, _ld(C)
+
+
+def _product(m, C, weight, transpose):
+    """rows x weight^T (transpose = False: weight (N, C)) or rows x weight (weight (C, N)), bfloat16 (rows, N), the rows
+    padded to a multiple of 16 channels in memory."""
+    N = weight.size(1) if transpose else weight.size(0)
+    dev, st = m.device, _stream(m)
+    out = torch.empty((m.size(0), _ld(N)), dtype=torch.bfloat16, device=dev)
+    if m.size(0):
+        a, lda = _padded(m, C)
+        ldw = _ld(C)
+        wb = torch.empty((N, ldw), dtype=torch.bfloat16, device=dev)
+        check(lib.pvn3d_mt_pack_weight(weight.size(0), weight.size(1), weight.data_ptr(), weight.size(1),
+                                       1 if transpose else 0, wb.data_ptr(), N, ldw, st), "mt_pack_weight")
+        check(lib.pvn3d_mt_gemm_nt(m.size(0), N, ldw, a.data_ptr(), lda, wb.data_ptr(), ldw, out.data_ptr(), _ld(N),
+                                   None, None, 0, st), "mt_gemm_nt")
+    return out[:, :N]
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        N, C = weight.shape
+        with on_device(x.device):
+            m, _ = _rows(x, "x")
+            w = weight.detach().contiguous()
+            y = _product(m, C, w, False)
+            ctx.act = None
+            if ctx.needs_input_grad[1]:
+                ctx.act = act8_pack(x.detach())
+        ctx.save_for_backward(weight)
+        ctx.lead = x.shape[:-1]
+        return y.view(x.shape[:-1] + (N,)) if x.dim() != 2 else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, = ctx.saved_tensors
+        N, C = weight.shape
+        dx = dw = None
+        dy = dy.to(torch.bfloat16)
+        with on_device(dy.device):
+            m, _ = _rows(dy, "dy")
+            if ctx.needs_input_grad[0]:
+                dx = _product(m, N, weight.detach().contiguous(), True).reshape(ctx.lead + (C,))
+            if ctx.needs_input_grad[1]:
+                dw = linear8_weight_grad(m, ctx.act)
+        return dx, dw
+
+
+def linear8(x, weight):
+    """y (..., N) = x (..., C) weight^T on the bfloat16 matrix kernels, x bfloat16, weight (N, C) float32 (rounded to
+    bfloat16 for the product, like the fused training chain does).  x is kept for the backward pass in 8 bits; the
+    input's gradient does not depend on it, the weight's is taken from it.  y's rows may be padded in memory (N not a
+    multiple of 16)."""
+    _need(x.is_cuda, "CPU not supported")
+    _need(x.dtype == torch.bfloat16, "x must be a bfloat16 tensor")
+    _need(weight.device == x.device, "weight must be on x's device")
+    _need(weight.dim() == 2 and weight.dtype == torch.float32, "weight must be a float32 matrix")
+    _need(x.dim() >= 1 and x.size(-1) == weight.size(1) and weight.numel() > 0, "x and weight must have the same channels")
+    _need(x.numel() // x.size(-1) < 2 ** 31, "too many rows")
+    return _Linear8.apply(x, weight)

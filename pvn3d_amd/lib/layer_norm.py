@@ -1,0 +1,251 @@
+"""Layer norm over the channels of every point, forward and backward (csrc/layer_norm*.hip), beside the BatchNorm that the
+SharedMLP layers of the reference use (pvn3d/lib/utils/etw_pytorch_utils/pytorch_utils.py:53-77): the statistics are a
+point's own, so a rank that trains on one frame computes what one that trains on 24 does.
+
+    mean = sum_c x / C    var = sum_c (x - mean)^2 / C    rstd = 1 / sqrt(var + eps)    xh = (x - mean) rstd
+    y = weight xh + bias, with relu: max(y, 0)
+
+x is float32, bfloat16 or float16; statistics, sums and gradients of the parameters are float32 in a fixed order (the same
+bits on every call).  ``channel_dim`` -1: channels last, (..., C), rows of any stride; ``channel_dim`` 1: (B, C, ...), a
+contiguous tensor or a transposed view of a point-major one (read in place).  1 <= C <= 8192.
+
+``layer_norm`` is the differentiable call and ``LayerNorm`` the module; ``layer_norm_forward`` / ``layer_norm_backward`` are
+the two launches for callers with a backward pass of their own, ``layer_norm_forward8`` / ``layer_norm_backward8`` the same
+with the input kept in 8 bits (act8.py) and one bit per value for the ReLU.  Everything runs on the current stream of x's
+device and may be captured."""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .._lib import lib, check, on_device
+from .act8 import Act8, DTYPES, _empty_act8, _need, _rows, _stream
+
+MAX_CHANNELS = 8192
+
+
+def _param(p, C, x, name):
+    if p is None:
+        return None
+    _need(p.dtype == torch.float32 and tuple(p.shape) == (C,), "%s must be a float32 tensor of the channels' length" % name)
+    _need(p.device == x.device, "%s must be on x's device" % name)
+    return p.contiguous()
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _check_x(x, name="x"):
+    _need(x.is_cuda, "CPU not supported")
+    _need(x.dtype in DTYPES, "%s must be a float32, bfloat16 or float16 tensor" % name)
+
+
+def _by_rows(x, channel_dim):
+    """-> (True, x with the channels last) or (False, contiguous (B, C, ...)); refuses what is neither."""
+    _need(x.dim() >= 1, "x must have a channel dimension")
+    d = channel_dim + x.dim() if channel_dim < 0 else channel_dim
+    if d == x.dim() - 1:
+        rows, C = True, x.size(-1)
+    else:
+        _need(d == 1, "channel_dim must be 1 or the last dimension")
+        C = x.size(1)
+        rows = x.movedim(1, -1).is_contiguous() and not x.is_contiguous()
+        x = x.movedim(1, -1) if rows else x.contiguous()
+    _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
+    return rows, x
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False):
+    """-> (y like x, mean, rstd): the statistics are float32, one value per point in the points' order."""
+    _check_x(x)
+    rows, v = _by_rows(x, channel_dim)
+    C = v.size(-1) if rows else v.size(1)
+    w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
+    dev = x.device
+    with on_device(dev):
+        n = v.numel() // C
+        y = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        stat = torch.empty((2, n), dtype=torch.float32, device=dev)
+        mean, rstd = stat[0], stat[1]
+        if rows:
+            m, xs = _rows(v, "x")
+            check(lib.pvn3d_layer_norm(DTYPES[v.dtype], n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), float(eps),
+                                       1 if relu else 0, y.data_ptr(), C, C, mean.data_ptr(), rstd.data_ptr(), None, 0,
+                                       None, None, _stream(x)), "layer_norm")
+            if v is not x:
+                y = y.movedim(-1, 1)
+        else:
+            check(lib.pvn3d_layer_norm_chan(DTYPES[v.dtype], v.size(0), C, n // max(v.size(0), 1), v.data_ptr(), _ptr(w),
+                                            _ptr(b), float(eps), 1 if relu else 0, y.data_ptr(), mean.data_ptr(),
+                                            rstd.data_ptr(), _stream(x)), "layer_norm_chan")
+    return y, mean, rstd
+
+
+def _workspace(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _check_stats(mean, rstd, n, x):
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous() and t.device == x.device,
+              "%s must be a contiguous float32 tensor with one value per point" % name)
+
+
+def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=False, need_dx=True, need_dparams=True):
+    """-> (dx like x or None, dweight (C,), dbias (C,) float32 or None, None).  mean, rstd: the forward's; relu: the
+    derivative is taken where weight xh + bias > 0."""
+    _check_x(x)
+    _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device, "dy must be like x")
+    _need(need_dx or need_dparams, "nothing to compute")
+    rows, v = _by_rows(x, channel_dim)
+    C = v.size(-1) if rows else v.size(1)
+    w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
+    n = v.numel() // C
+    _check_stats(mean, rstd, n, x)
+    dev, t = x.device, DTYPES[v.dtype]
+    with on_device(dev):
+        st = _stream(x)
+        dx = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_dx else None
+        dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
+        pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
+        if rows:
+            d = dy if v is x else dy.movedim(1, -1)
+            (m, xs), (g, gs) = _rows(v, "x"), _rows(d, "dy")
+            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C, C) if need_dparams else 0
+            ws = _workspace(wsb, dev)
+            check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, m.data_ptr(), xs, None, 0, None, None, _ptr(w),
+                                            _ptr(b), mean.data_ptr(), rstd.data_ptr(), 1 if relu else 0, _ptr(dx), C, C,
+                                            pw, pb, _ptr(ws), wsb, st), "layer_norm_grad")
+            if need_dx and v is not x:
+                dx = dx.movedim(-1, 1)
+        else:
+            g = dy.contiguous()
+            B = v.size(0)
+            wsb = lib.pvn3d_layer_norm_chan_grad_workspace_bytes(t, B, C, n // max(B, 1)) if need_dparams else 0
+            ws = _workspace(wsb, dev)
+            check(lib.pvn3d_layer_norm_chan_grad(t, B, C, n // max(B, 1), g.data_ptr(), v.data_ptr(), _ptr(w), _ptr(b),
+                                                 mean.data_ptr(), rstd.data_ptr(), 1 if relu else 0, _ptr(dx), pw, pb,
+                                                 _ptr(ws), wsb, st), "layer_norm_chan_grad")
+    return (dx, dp[0], dp[1]) if need_dparams else (dx, None, None)
+
+
+class Saved8(object):
+    """What layer_norm_forward8 keeps for the backward pass: x in 8 bits, the statistics, and with a ReLU one bit per
+    value (mask (rows, ceil(C / 8)) uint8, bit i of byte j: channel 8 j + i is on)."""
+    __slots__ = ("act", "mask", "mean", "rstd", "dtype")
+
+    def __init__(self, act, mask, mean, rstd, dtype):
+        rows, C = act.codes.shape
+        if mask is not None:
+            _need(mask.dtype == torch.uint8 and tuple(mask.shape) == (rows, (C + 7) // 8) and mask.is_contiguous()
+                  and mask.device == act.codes.device, "mask must be a contiguous uint8 (rows, ceil(channels / 8)) matrix")
+        _check_stats(mean, rstd, rows, act.codes)
+        self.act, self.mask, self.mean, self.rstd, self.dtype = act, mask, mean, rstd, dtype
+
+    @property
+    def nbytes(self):
+        return self.act.nbytes + (self.mask.numel() if self.mask is not None else 0) + 8 * self.mean.numel()
+
+
+def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
+    """x (..., C) -> (y like x, Saved8).  y is layer_norm_forward's, bit for bit."""
+    _check_x(x)
+    _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
+    C = x.size(-1)
+    w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
+    dev = x.device
+    with on_device(dev):
+        m, xs = _rows(x, "x")
+        n = m.size(0)
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stat = torch.empty((2, n), dtype=torch.float32, device=dev)
+        act = _empty_act8(n, C, x.shape, dev)
+        mask = torch.empty((n, (C + 7) // 8), dtype=torch.uint8, device=dev) if relu else None
+        check(lib.pvn3d_layer_norm(DTYPES[x.dtype], n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), float(eps), 1 if relu else 0,
+                                   y.data_ptr(), C, C, stat[0].data_ptr(), stat[1].data_ptr(), act.codes.data_ptr(),
+                                   act.pitch, act.scales.data_ptr(), _ptr(mask), _stream(x)), "layer_norm")
+        saved = Saved8(act, mask, stat[0], stat[1], x.dtype)
+    return y, saved
+
+
+def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True):
+    """layer_norm_backward with xh = (held x - mean) rstd from the 8-bit form and the ReLU from its bits."""
+    _need(isinstance(saved, Saved8), "saved must be what layer_norm_forward8 returned")
+    _check_x(dy, "dy")
+    act = saved.act
+    _need(dy.shape == act.shape and dy.dtype == saved.dtype and dy.device == act.codes.device, "dy must be like x")
+    _need(need_dx or need_dparams, "nothing to compute")
+    n, C = act.codes.shape
+    w = _param(weight, C, dy, "weight")
+    dev, t = dy.device, DTYPES[dy.dtype]
+    with on_device(dev):
+        g, gs = _rows(dy, "dy")
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev) if need_dx else None
+        dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
+        wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C, C) if need_dparams else 0
+        ws = _workspace(wsb, dev)
+        pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
+        check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, None, 0, act.codes.data_ptr(), act.pitch,
+                                        act.scales.data_ptr(), _ptr(saved.mask), _ptr(w), None, saved.mean.data_ptr(),
+                                        saved.rstd.data_ptr(), 1 if saved.mask is not None else 0, _ptr(dx), C, C, pw, pb,
+                                        _ptr(ws), wsb, _stream(dy)), "layer_norm_grad")
+    return (dx, dp[0], dp[1]) if need_dparams else (dx, None, None)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, channel_dim, relu, ckpt8):
+        ctx.meta = (channel_dim, relu)
+        ctx.saved8 = None
+        if ckpt8:
+            rows, v = _by_rows(x, channel_dim)
+            _need(rows, "ckpt8 takes channels-last tensors (or a transposed view of one)")
+            ctx.moved = v is not x
+            y, ctx.saved8 = layer_norm_forward8(v, weight, bias, eps, relu)
+            ctx.save_for_backward(weight)
+            return y.movedim(-1, 1) if ctx.moved else y
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, channel_dim, relu)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        channel_dim, relu = ctx.meta
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if not (need_x or need_w or need_b):
+            return (None,) * 7
+        if ctx.saved8 is not None:
+            weight, = ctx.saved_tensors
+            d = dy.movedim(1, -1) if ctx.moved else dy
+            dx, dw, db = layer_norm_backward8(d, ctx.saved8, weight, need_x, need_w or need_b)
+            if ctx.moved and need_x:
+                dx = dx.movedim(-1, 1)
+        else:
+            x, weight, bias, mean, rstd = ctx.saved_tensors
+            dx, dw, db = layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim, relu, need_x, need_w or need_b)
+        return dx, dw if need_w else None, db if need_b else None, None, None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False, ckpt8=False):
+    """Differentiable layer norm (see the top of this file).  ckpt8: keep x for the backward pass in 8 bits instead of
+    holding on to it (channels last only); the output is the same, the gradients take xh from the 8-bit form."""
+    _check_x(x)
+    return _LayerNorm.apply(x, weight, bias, eps, channel_dim, bool(relu), bool(ckpt8))
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over `channels` channels at `channel_dim` with learned weight (ones) and bias (zeros)."""
+
+    def __init__(self, channels, eps=1e-5, channel_dim=-1, relu=False, ckpt8=False):
+        super(LayerNorm, self).__init__()
+        self.eps, self.channel_dim, self.relu, self.ckpt8 = eps, channel_dim, relu, ckpt8
+        self.weight = nn.Parameter(torch.ones(channels))
+        self.bias = nn.Parameter(torch.zeros(channels))
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps, self.channel_dim, self.relu, self.ckpt8)
+
+    def extra_repr(self):
+        return "%d, eps=%g, channel_dim=%d, relu=%s, ckpt8=%s" % (self.weight.numel(), self.eps, self.channel_dim, self.relu,
+                                                                  self.ckpt8)
