@@ -643,13 +643,13 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  * pvn3d_layer_norm_grad: dx (NULL: not wanted; columns up to dx_cols written, zeros from C on), dweight and dbias (both or
  *   neither).  The normalised input comes from x, or, if codes != NULL, from codes / scales (relu != 0: and the ReLU from
  *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
- *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C, dx_cols) names (dx NULL: C), 4-byte aligned, needed for dweight
+ *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C) names, 4-byte aligned, needed for dweight
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
- * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors; mean, rstd (B, M). */
+ * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, M >= 4 (or 0); mean, rstd (B, M). */
 int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
                      float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
                      long long pitch, void* scales, void* mask, void* stream);
-size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C, int dx_cols);
+size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C);
 int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
                           const void* codes, long long pitch, const void* scales, const void* mask, const float* weight,
                           const float* bias, const float* mean, const float* rstd, int relu, void* dx, long long dxs,

@@ -109,7 +109,7 @@ SIGNATURES = {
     "pvn3d_mt_bn_bwd_apply": (_i, [_ll, _i, _p, _p, _p, _p, _p, _p, _p, _p]),
     # layer norm over the channels (csrc/layer_norm*.hip)
     "pvn3d_layer_norm": (_i, [_i, _ll, _i, _p, _ll, _p, _p, _f, _i, _p, _ll, _i, _p, _p, _p, _ll, _p, _p, _p]),
-    "pvn3d_layer_norm_grad_workspace_bytes": (_sz, [_i, _ll, _i, _i]),
+    "pvn3d_layer_norm_grad_workspace_bytes": (_sz, [_i, _ll, _i]),
     "pvn3d_layer_norm_grad": (_i, [_i, _ll, _i, _p, _ll, _p, _ll, _p, _ll, _p, _p, _p, _p, _p, _p, _i, _p, _ll, _i, _p, _p,
                                    _p, _sz, _p]),
     "pvn3d_layer_norm_chan": (_i, [_i, _i, _i, _i, _p, _p, _p, _f, _i, _p, _p, _p, _p]),

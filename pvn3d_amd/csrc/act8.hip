@@ -16,7 +16,19 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------------------------------------------ pack / unpack
-// 256 / TPR rows per workgroup, TPR threads across a row (a power of two that covers whole groups or the row)
+// tpr threads across a row (a power of two that covers whole groups or the row), 256 / tpr rows per workgroup.  Chunks are
+// windows (rowvec.h); a row shorter than one is read value by value.
+template <typename T>
+__device__ __forceinline__ void load_any(const T* __restrict__ row, int at, int C, float (&v)[traits<T>::VEC]) {
+  constexpr int VEC = traits<T>::VEC;
+  if (C >= VEC) {
+    rv::load_vec<T>(row + at, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(row + i) : 0.f;
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, int tpr, const T* __restrict__ x,
                                                         long long xs, signed char* __restrict__ codes, long long pitch,
@@ -26,10 +38,18 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, i
   const int G = (C + rv::GROUP - 1) / rv::GROUP;
   for (long long row = (long long)blockIdx.x * rpb + rg; row < rows; row += (long long)gridDim.x * rpb) {
     for (int c = t * VEC; c < G * rv::GROUP; c += tpr * VEC) {      // whole groups: every lane of one takes part
+      const int at = C >= VEC ? min(c, C - VEC) : 0, skip = C >= VEC ? min(c - at, VEC) : (c ? VEC : 0);
       float v[VEC];
-      rv::load_chunk<T>(x + row * xs + c, C - c, v);
-      const unsigned sc = rv::lanes_scale<VEC, LPG>(v);
-      if (c < C) rv::store_codes<VEC>(codes + row * pitch + c, v, rv::group_inverse(sc));
+      load_any<T>(x + row * xs, at, C, v);
+      unsigned big = 0, wd[VEC / 4];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {                               // as integers: NaN is the largest
+        const unsigned a = __float_as_uint(v[i]) & 0x7fffffffu;
+        big = max(big, i >= skip ? a : 0u);
+      }
+      const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
+      rv::group_codes<VEC>(v, sc, wd);
+      if (c < C) rv::store_codes(codes + row * pitch, c, skip, wd);
       if ((c & (rv::GROUP - 1)) == 0) scales[row * G + c / rv::GROUP] = (unsigned char)sc;
     }
   }
@@ -43,14 +63,24 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C,
   const int t = threadIdx.x & (tpr - 1), rg = threadIdx.x / tpr, rpb = 256 / tpr;
   const int G = (C + rv::GROUP - 1) / rv::GROUP;
   for (long long row = (long long)blockIdx.x * rpb + rg; row < rows; row += (long long)gridDim.x * rpb) {
-    for (int c = t * VEC; c < ycols; c += tpr * VEC) {
+    for (int c = t * VEC; c < C; c += tpr * VEC) {
+      const int at = C >= VEC ? min(c, C - VEC) : 0, skip = c - at;
+      unsigned wd[VEC / 4];
+      rv::load_codes(codes + row * pitch + at, wd);
+      const float s1 = rv::group_step(scales[row * G + c / rv::GROUP]), s0 = rv::group_step(scales[row * G + at / rv::GROUP]);
       float v[VEC];
-      const bool in = c < C;
-      rv::load_codes<VEC>(codes + row * pitch + (in ? c : 0), rv::group_step(scales[row * G + (in ? c / rv::GROUP : 0)]), v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? v[i] : 0.f;
-      rv::store_chunk<T>(y + row * ys + c, ycols - c, v);
+      for (int i = 0; i < VEC; ++i) v[i] = rv::code_at(wd, i) * (i < skip ? s0 : s1);
+      if (C >= VEC) {
+        rv::store_vec<T>(y + row * ys + at, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i < C) traits<T>::store1(y + row * ys + i, v[i]);
+      }
     }
+    if (ycols > C)
+      for (int c = C + t; c < ycols; c += tpr) traits<T>::store1(y + row * ys + c, 0.f);
   }
 }
 
@@ -61,7 +91,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C,
 // transposed.  Row strides of 64 bytes times an odd number keep the four rows of such a block in different banks.
 // A workgroup owns a (32 MB WM) x (32 NB WN) tile of dW and steps s, s + S, ...: WM WN waves share a step's staging (a
 // barrier per step), or, with WM = WN = 1, each of the four waves stages its own steps.  S partial tiles go to the
-// workspace, summed in a fixed order by act8_wgrad_sum_kernel (S = 1: straight to dW).
+// workspace, summed in a fixed order by rowvec.h's fold (S = 1: straight to dW).
 constexpr int WG_ROWS = 32;
 
 __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride, int lane) {
@@ -158,15 +188,10 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, 
       const int q = i * NT + tid, r = q / (TN / 16), c = (q - r * (TN / 16)) * 16;
       if (WG_ROWS * TN / 16 % NT == 0 || r < WG_ROWS) {
         const float step = rv::group_step(rs[i]);
-        float v[16], f[4];
-        rv::group_values(rb[i].x, step, f);
-        v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
-        rv::group_values(rb[i].y, step, f);
-        v[4] = f[0]; v[5] = f[1]; v[6] = f[2]; v[7] = f[3];
-        rv::group_values(rb[i].z, step, f);
-        v[8] = f[0]; v[9] = f[1]; v[10] = f[2]; v[11] = f[3];
-        rv::group_values(rb[i].w, step, f);
-        v[12] = f[0]; v[13] = f[1]; v[14] = f[2]; v[15] = f[3];
+        const unsigned wd[4] = {rb[i].x, rb[i].y, rb[i].z, rb[i].w};
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = rv::code_at(wd, e) * step;
         typedef traits<bf16> tb16;
         *reinterpret_cast<uint4*>(tb + r * LB + c) =
             make_uint4(tb16::p2(v[0], v[1]), tb16::p2(v[2], v[3]), tb16::p2(v[4], v[5]), tb16::p2(v[6], v[7]));
@@ -249,15 +274,6 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, 
       if (m < M && n < N) dst[(size_t)m * N + n] = fold[e];
     }
   }
-}
-
-__global__ __launch_bounds__(256) void act8_wgrad_sum_kernel(int S, size_t count, const float* __restrict__ part,
-                                                             float* __restrict__ dW) {
-  const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= count) return;
-  float a = 0.f;
-  for (int s = 0; s < S; ++s) a += part[(size_t)s * count + e];
-  dW[e] = a;
 }
 
 // tile and number of row splits of a call
@@ -373,10 +389,5 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
   }
 #undef A8_CALL
   PVN3D_LAUNCH_CHECK();
-  if (p.S > 1) {
-    hipLaunchKernelGGL(act8_wgrad_sum_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, A8_ST, p.S, count,
-                       (const float*)workspace, dW);
-    PVN3D_LAUNCH_CHECK();
-  }
-  return 0;
+  return p.S > 1 ? rv::fold(p.S, count, count, (const float*)workspace, dW, nullptr, A8_ST) : 0;
 }

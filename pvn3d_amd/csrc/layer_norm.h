@@ -14,8 +14,7 @@ constexpr int MAX_PARTS = 1024;      // workgroups of a backward launch, each wi
 // sum over the TPR lanes of a row; TPR = 256: over the workgroup (a barrier: every thread of it calls this)
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o, 64);
+  v = rv::lanes_sum<(TPR < 64 ? TPR : 64)>(v);
   if (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     __syncthreads();
@@ -26,11 +25,58 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
+// The chunks of one row of a thread, in registers: chunk k's window, and which of its values are this lane's own (1 / 0).
+// TPR = 1 is the kernel for C <= VEC: one thread holds the whole row, value by value.
+template <typename T, int TPR, int K>
+struct lane_cols {
+  static constexpr int VEC = traits<T>::VEC;
+  int c[K], at[K], skip[K];
+  float own[K][VEC];
+  __device__ __forceinline__ lane_cols(int t, int C) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      c[k] = (k * TPR + t) * VEC;
+      at[k] = 0;
+      skip[k] = 0;
+      if (TPR > 1) {
+        const rv::window<VEC> w(c[k], C);
+        at[k] = w.at;
+        skip[k] = w.skip;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) own[k][i] = i >= skip[k] && at[k] + i < C ? 1.f : 0.f;
+    }
+  }
+  __device__ __forceinline__ void params(const float* __restrict__ p, float missing, int C, float (&v)[K][VEC]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[k][i] = at[k] + i < C ? (p ? p[at[k] + i] : missing) : 0.f;
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ row, int k, int C, float (&v)[VEC]) const {
+    if (TPR > 1) {
+      rv::load_vec<T>(row + at[k], v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(row + i) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(T* __restrict__ row, int k, int C, const float (&v)[VEC]) const {
+    if (TPR > 1) {
+      if (c[k] < C) rv::store_vec<T>(row + at[k], v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < C) traits<T>::store1(row + i, v[i]);
+    }
+  }
+};
+
 inline int vec_of(int dtype) { return dtype == 0 ? 4 : 8; }
 
 // threads per row: the power of two whose chunks cover it, 64 at most; a workgroup where four chunks a lane do not
-inline int rows_threads(int cover, int vec) {
-  const int chunks = (cover + vec - 1) / vec;
+inline int rows_threads(int C, int vec) {
+  const int chunks = (C + vec - 1) / vec;
   int t = 1;
   while (t < chunks && t < 64) t <<= 1;
   return chunks > 4 * 64 ? 256 : t;
@@ -40,12 +86,12 @@ inline long long rows_blocks(long long rows, int tpr, int r) {
   return (rows + per - 1) / per;
 }
 
-// the (threads per row, chunks, rows in flight) instance that covers `cover` columns
-#define LN_ROWS_PICK(T, CALL)                                             \
+// the (threads per row, chunks, rows in flight) instance for C columns
+#define LN_ROWS_PICK(T, C, CALL)                                          \
   do {                                                                    \
     constexpr int vec__ = rv::traits<T>::VEC;                             \
-    const int tpr__ = ln::rows_threads(cover, vec__);                     \
-    const int k__ = (cover + tpr__ * vec__ - 1) / (tpr__ * vec__);        \
+    const int tpr__ = ln::rows_threads(C, vec__);                         \
+    const int k__ = (C + tpr__ * vec__ - 1) / (tpr__ * vec__);            \
     if (tpr__ == 1) CALL(T, 1, 1, 2);                                     \
     else if (tpr__ == 2) CALL(T, 2, 1, 2);                                \
     else if (tpr__ == 4) CALL(T, 4, 1, 2);                                \
@@ -58,8 +104,5 @@ inline long long rows_blocks(long long rows, int tpr, int r) {
     else if (vec__ == 8 || k__ <= 4) CALL(T, 256, 4, 1);                  \
     else CALL(T, 256, (vec__ == 8 ? 4 : 8), 1);                           \
   } while (0)
-
-// part [parts][2 C] -> dweight, dbias (layer_norm_grad.hip)
-int sum_parts(int parts, int C, const float* part, float* dw, float* db, hipStream_t st);
 
 }  // namespace ln

@@ -22,8 +22,8 @@ using rv::traits;
 using ln::row_sum;
 
 // ------------------------------------------------------------------------------------------------ rows, forward
-// TPR threads share a row, chunk k of thread t = channels (k TPR + t) VEC ..: K chunks cover the row, R rows per thread
-// are in flight at once.
+// TPR threads share a row, chunk k of thread t = the VEC channels from (k TPR + t) VEC on (16 bytes): K chunks cover the
+// row, R rows per thread are in flight at once.
 template <typename T, int TPR, int K, int R, bool SAVE8>
 __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, const T* __restrict__ x, long long xs,
                                                       const float* __restrict__ w, const float* __restrict__ b, float eps,
@@ -36,27 +36,20 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
   constexpr int RPB = 256 / TPR;
   __shared__ float red[4];
   const int t = threadIdx.x % TPR, rg = threadIdx.x / TPR;
+  const int G = (C + rv::GROUP - 1) / rv::GROUP, MB = (C + 7) / 8;
+  const ln::lane_cols<T, TPR, K> col(t, C);
   float g[K][VEC], be[K][VEC];
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int c = (k * TPR + t) * VEC + i;
-      g[k][i] = c < C ? (w ? w[c] : 1.f) : 0.f;
-      be[k][i] = c < C && b ? b[c] : 0.f;
-    }
-  const float rc = 1.f / (float)C;
+  col.params(w, 1.f, C, g);
+  col.params(b, 0.f, C, be);
+  const float rc = 1.f / (float)C, floor = relu ? 0.f : -__builtin_inff();
   for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)gridDim.x * (RPB * R)) {
     float v[R][K][VEC];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = base + r * RPB + rg;
-      const T* p = x + (row < rows ? row : rows - 1) * xs;
+      const T* const p = x + (row < rows ? row : rows - 1) * xs;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * TPR + t) * VEC;
-        rv::load_chunk<T>(p + c, C - c, v[r][k]);
-      }
+      for (int k = 0; k < K; ++k) col.load(p, k, C, v[r][k]);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -66,15 +59,15 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s += v[r][k][i];
+        for (int i = 0; i < VEC; ++i) s = fmaf(v[r][k][i], col.own[k][i], s);
       const float mu = row_sum<TPR>(s, red) * rc;
       float q = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float d = (k * TPR + t) * VEC + i < C ? v[r][k][i] - mu : 0.f;
-          q = fmaf(d, d, q);
+          const float d = v[r][k][i] - mu;
+          q = fmaf(d * col.own[k][i], d, q);
         }
       const float rs = 1.f / sqrtf(row_sum<TPR>(q, red) * rc + eps);
       if (live && t == 0) {
@@ -83,33 +76,41 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * TPR + t) * VEC;
+        const int c = col.c[k];
         float z[VEC];
-        unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          z[i] = fmaf((v[r][k][i] - mu) * rs, g[k][i], be[k][i]);
-          bits |= (z[i] > 0.f ? 1u : 0u) << i;
-          // (a NaN stays one: max(z, 0) would make it 0)
-          if (relu) z[i] = z[i] < 0.f ? 0.f : z[i];
-          if (c + i >= C) z[i] = 0.f;
-        }
-        if (live && c < ycols) rv::store_chunk<T>(y + row * ys + c, ycols - c, z);
+        for (int i = 0; i < VEC; ++i)       // (maximum: a NaN stays one, which max(z, 0) would make 0)
+          z[i] = __builtin_elementwise_maximum(fmaf((v[r][k][i] - mu) * rs, g[k][i], be[k][i]), floor);
+        if (live) col.store(y + row * ys, k, C, z);
         if (SAVE8) {
           constexpr int LPG = rv::GROUP / VEC < TPR ? rv::GROUP / VEC : TPR;       // lanes per group
-          const unsigned sc = rv::lanes_scale<VEC, LPG>(v[r][k]);
-          if (live && c < C) {
-            rv::store_codes<VEC>(codes + row * pitch + c, v[r][k], rv::group_inverse(sc));
-            if ((c & (rv::GROUP - 1)) == 0) scales[row * ((C + rv::GROUP - 1) / rv::GROUP) + c / rv::GROUP] = (unsigned char)sc;
+          unsigned big = 0, wd[VEC / 4];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {                      // as integers: NaN is the largest
+            const unsigned a = __float_as_uint(v[r][k][i]) & 0x7fffffffu;
+            big = max(big, col.own[k][i] != 0.f ? a : 0u);
           }
-          if (mask) {
-            unsigned other = 0;
-            if (VEC == 4) other = (unsigned)__shfl_down((int)bits, 1, 64);          // two lanes share a byte
-            if (live && c < C && (c & 7) == 0)
-              mask[row * ((C + 7) / 8) + c / 8] = (unsigned char)(bits | (VEC == 4 ? (c + 4 < C && TPR > 1 ? other << 4 : 0u) : 0u));
+          const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
+          rv::group_codes<VEC>(v[r][k], sc, wd);
+          if (live && c < C) {
+            rv::store_codes(codes + row * pitch, c, col.skip[k], wd);
+            if ((c & (rv::GROUP - 1)) == 0) scales[row * G + c / rv::GROUP] = (unsigned char)sc;
+          }
+          if (mask) {                                          // y is 0 or positive here: minus its bits, the sign bit
+            unsigned bits = 0;
+#pragma unroll
+            for (int i = VEC - 1; i >= 0; --i) bits = __builtin_amdgcn_alignbit(bits, 0u - __float_as_uint(z[i]), 31);
+            bits >>= col.skip[k];
+            if (VEC == 4 && TPR > 1) {                         // two lanes share a byte
+              const unsigned other = rv::dpp(bits, 1);
+              bits |= c + 4 < C ? other << 4 : 0u;
+            }
+            if (live && c < C && (c & 7) == 0) mask[row * MB + c / 8] = (unsigned char)bits;
           }
         }
       }
+      if (ycols > C && live)
+        for (int c = C + t; c < ycols; c += TPR) traits<T>::store1(y + row * ys + c, 0.f);
     }
   }
 }
@@ -118,7 +119,6 @@ template <typename T>
 int rows_forward(long long rows, int C, const void* x, long long xs, const float* w, const float* b, float eps, int relu,
                  void* y, long long ys, int ycols, float* mean, float* rstd, void* codes, long long pitch, void* scales,
                  void* mask, hipStream_t st) {
-  const int cover = C > ycols ? C : ycols;
 #define LN_CALL(T, TPR, K, R)                                                                                           \
   do {                                                                                                                  \
     const long long nb = ln::rows_blocks(rows, TPR, R);                                                                     \
@@ -131,7 +131,7 @@ int rows_forward(long long rows, int C, const void* x, long long xs, const float
       hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, xs, w, b, \
                          eps, relu, (T*)y, ys, ycols, mean, rstd, nullptr, 0ll, nullptr, nullptr);                      \
   } while (0)
-  LN_ROWS_PICK(T, LN_CALL);
+  LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
   return 0;

@@ -35,35 +35,28 @@ __device__ __forceinline__ raw4<T> shut(const float (&v)[4]) {
 template <>
 __device__ __forceinline__ raw4<float> shut<float>(const float (&v)[4]) { return raw4<float>{traits<float>::pack(v)}; }
 
-// `left`: points from p to the row's end; a partial chunk is read point by point (zeros behind it)
-template <typename T>
-__device__ __forceinline__ raw4<T> get(const T* __restrict__ p, int left) {
-  if (left >= 4) return *reinterpret_cast<const raw4<T>*>(p);
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < left ? traits<T>::load1(p + i) : 0.f;
-  return shut<T>(v);
-}
-template <typename T>
-__device__ __forceinline__ void put(T* __restrict__ p, int left, const float (&v)[4]) {
-  if (left >= 4) {
-    *reinterpret_cast<raw4<T>*>(p) = shut<T>(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) traits<T>::store1(p + i, v[i]);
+// Chunks are whole and unconditional: the last, partial one of a row of points is taken as its last four points, which
+// overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.
+struct tile_at {
+  int b, m0, skip;
+  bool live;
+  __device__ __forceinline__ tile_at(int tile, int NV, int MV, int M) {
+    const int pv = tile * 16 + (threadIdx.x & 15);
+    live = pv < NV;
+    const int at = live ? pv : NV - 1;
+    b = at / MV;
+    const int m = (at - b * MV) * PTS;
+    m0 = min(m, M - PTS);
+    skip = m - m0;
   }
-}
+};
 
 // s[i] -> sum over the workgroup's channel slots of s[i], for the thread's own points
 template <int N>
 __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[16 * N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane & 15, waves = blockDim.x >> 6;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    s[i] += __shfl_xor(s[i], 16, 64);
-    s[i] += __shfl_xor(s[i], 32, 64);
-  }
+  for (int i = 0; i < N; ++i) s[i] = rv::add32(rv::add16(s[i]));
   if (lane < 16) {
 #pragma unroll
     for (int i = 0; i < N; ++i) buf[wave][px * N + i] = s[i];
@@ -83,22 +76,21 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int B, int C, int 
                                                               float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int KR = KC > 0 ? KC : 1;
   __shared__ float buf[2][MAX_THREADS / 64][16 * PTS];
-  const int px = threadIdx.x & 15, cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
+  const int cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
   const int NV = B * MV;
-  const float rc = 1.f / (float)C;
+  const float rc = 1.f / (float)C, floor = relu ? 0.f : -__builtin_inff();
   for (int tile = blockIdx.x; tile < (NV + 15) / 16; tile += gridDim.x) {
-    const int pv = tile * 16 + px;
-    const bool live = pv < NV;
-    const int at = live ? pv : NV - 1, bi = at / MV, m0 = (at - bi * MV) * PTS, nv = M - m0;
-    const T* const p = x + (size_t)bi * C * M + m0;
-    T* const q = y + (size_t)bi * C * M + m0;
+    const tile_at at(tile, NV, MV, M);
+    const size_t off = (size_t)at.b * C * M + at.m0;
+    const T* const p = x + off;
+    T* const q = y + off;
     raw4<T> r[KR];
     float s[PTS] = {0.f, 0.f, 0.f, 0.f}, mu[PTS], rs[PTS];
     if (KC > 0) {
 #pragma unroll
       for (int k = 0; k < KR; ++k) {
         const int c = cy + k * CY;
-        r[k] = get<T>(p + (size_t)(c < C ? c : 0) * M, nv);
+        r[k] = *reinterpret_cast<const raw4<T>*>(p + (size_t)(c < C ? c : 0) * M);
       }
     }
     // f(channel, values) for each of the thread's channels
@@ -114,7 +106,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int B, int C, int 
         }
       } else {
         for (int c = cy; c < C; c += CY) {
-          open<T>(get<T>(p + (size_t)c * M, nv), v);
+          open<T>(*reinterpret_cast<const raw4<T>*>(p + (size_t)c * M), v);
           f(c, v);
         }
       }
@@ -133,23 +125,20 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int B, int C, int 
     slot_sum<PTS>(s, buf[1]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) rs[i] = 1.f / sqrtf(s[i] * rc + eps);
-    if (live && cy == 0) {
+    if (at.live && cy == 0) {
 #pragma unroll
-      for (int i = 0; i < PTS; ++i)
-        if (i < nv) {
-          mean[(size_t)bi * M + m0 + i] = mu[i];
-          rstd[(size_t)bi * M + m0 + i] = rs[i];
-        }
+      for (int i = 0; i < PTS; ++i) {
+        mean[(size_t)at.b * M + at.m0 + i] = mu[i];
+        rstd[(size_t)at.b * M + at.m0 + i] = rs[i];
+      }
     }
     each([&](int c, const float (&v)[PTS]) {
       const float g = w ? w[c] : 1.f, be = b ? b[c] : 0.f;
       float z[PTS];
 #pragma unroll
-      for (int i = 0; i < PTS; ++i) {
-        z[i] = fmaf((v[i] - mu[i]) * rs[i], g, be);
-        if (relu) z[i] = z[i] < 0.f ? 0.f : z[i];        // (a NaN stays one)
-      }
-      if (live) put<T>(q + (size_t)c * M, nv, z);
+      for (int i = 0; i < PTS; ++i)                      // (maximum: a NaN stays one)
+        z[i] = __builtin_elementwise_maximum(fmaf((v[i] - mu[i]) * rs[i], g, be), floor);
+      if (at.live) *reinterpret_cast<raw4<T>*>(q + (size_t)c * M) = shut<T>(z);
     });
   }
 }
@@ -178,15 +167,13 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
   }
   int turn = 0;
   for (int tile = blockIdx.x; tile < (NV + 15) / 16; tile += gridDim.x, turn ^= 1) {
-    const int pv = tile * 16 + px;
-    const bool live = pv < NV;
-    const int at = live ? pv : NV - 1, bi = at / MV, m0 = (at - bi * MV) * PTS, nv = M - m0;
-    const size_t off = (size_t)bi * C * M + m0;
+    const tile_at at(tile, NV, MV, M);
+    const size_t off = (size_t)at.b * C * M + at.m0;
     raw4<T> rx[KR], rd[KR];
     float mu[PTS], rs[PTS], s[2 * PTS];
 #pragma unroll
     for (int i = 0; i < PTS; ++i) {
-      const size_t mi = (size_t)bi * M + m0 + (i < nv ? i : 0);
+      const size_t mi = (size_t)at.b * M + at.m0 + i;
       mu[i] = mean[mi];
       rs[i] = rstd[mi];
       s[i] = 0.f;
@@ -196,12 +183,12 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
 #pragma unroll
       for (int k = 0; k < KR; ++k) {
         const size_t o = off + (size_t)(cy + k * CY < C ? cy + k * CY : 0) * M;
-        rx[k] = get<T>(x + o, nv);
-        rd[k] = get<T>(dy + o, nv);
+        rx[k] = *reinterpret_cast<const raw4<T>*>(x + o);
+        rd[k] = *reinterpret_cast<const raw4<T>*>(dy + o);
       }
     }
-    // f(k, channel, xh, dz, weight) for each of the thread's channels; dz = 0 where the ReLU is off, behind the last
-    // point and in a lane without points
+    // f(k, channel, xh, dz, weight) for each of the thread's channels; dz = 0 where the ReLU is off and in a lane without
+    // points
     auto each = [&](auto f) {
       float v[PTS], d[PTS];
       auto one = [&](int k, int c) {
@@ -209,8 +196,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
 #pragma unroll
         for (int i = 0; i < PTS; ++i) {
           v[i] = (v[i] - mu[i]) * rs[i];
-          const bool on = live && i < nv && (!relu || fmaf(v[i], g, be) > 0.f);
-          d[i] = on ? d[i] : 0.f;
+          const bool off_ = relu && fmaf(v[i], g, be) <= 0.f;      // (a NaN passes, as in the forward)
+          d[i] = at.live && !off_ ? d[i] : 0.f;
         }
         f(k, c, v, d, g);
       };
@@ -225,8 +212,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
         }
       } else {
         for (int c = cy; c < C; c += CY) {
-          open<T>(get<T>(x + off + (size_t)c * M, nv), v);
-          open<T>(get<T>(dy + off + (size_t)c * M, nv), d);
+          open<T>(*reinterpret_cast<const raw4<T>*>(x + off + (size_t)c * M), v);
+          open<T>(*reinterpret_cast<const raw4<T>*>(dy + off + (size_t)c * M), d);
           one(0, c);
         }
       }
@@ -235,8 +222,9 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
       float w1 = 0.f, b1 = 0.f;
 #pragma unroll
       for (int i = 0; i < PTS; ++i) {
-        w1 = fmaf(dz[i], xh[i], w1);
-        b1 += dz[i];
+        const float own = i >= at.skip ? dz[i] : 0.f;
+        w1 = fmaf(own, xh[i], w1);
+        b1 += own;
         s[i] = fmaf(dz[i], g, s[i]);
         s[PTS + i] = fmaf(dz[i] * g, xh[i], s[PTS + i]);
       }
@@ -263,7 +251,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
       float o[PTS];
 #pragma unroll
       for (int i = 0; i < PTS; ++i) o[i] = rs[i] * (dz[i] * g - s[i] - xh[i] * s[PTS + i]);
-      if (live) put<T>(dx + off + (size_t)c * M, nv, o);
+      if (at.live) *reinterpret_cast<raw4<T>*>(dx + off + (size_t)c * M) = shut<T>(o);
     });
   }
   if (!part) return;
@@ -304,7 +292,7 @@ int chan_grad_parts(int B, int M) {
   return (int)(n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
 }
 bool chan_ok(int dtype, int B, int C, int M) {
-  return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && M >= 0 && (long long)B * points4(M) < 0x7fffff00LL;
+  return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || M >= PTS) && (long long)B * points4(M) < 0x7fffff00LL;
 }
 
 template <typename T>
@@ -399,5 +387,5 @@ extern "C" int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const 
     default: rc = chan_backward<fp16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, part, st); break;
   }
   if (rc || !dweight) return rc;
-  return ln::sum_parts(parts, C, part, dweight, dbias, st);
+  return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, st);
 }

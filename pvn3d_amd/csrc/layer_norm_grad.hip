@@ -11,6 +11,7 @@ using ln::row_sum;
 // ------------------------------------------------------------------------------------------------ rows, backward
 // As the forward; a thread's channels are the same for all its rows, so dw and db are summed in its registers over the
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
+// FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
 __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, long long dys,
                                                            const T* __restrict__ x, long long xs,
@@ -28,21 +29,23 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
   __shared__ float fold[TPR > 64 ? 1 : 4 * COLS];
   const int t = threadIdx.x % TPR, rg = threadIdx.x / TPR;
   const int G = (C + rv::GROUP - 1) / rv::GROUP, MB = (C + 7) / 8;
+  const bool ragged = (C & (VEC - 1)) != 0;
+  const ln::lane_cols<T, TPR, K> col(t, C);
   float g[K][VEC], be[K][VEC], aw[K][VEC], ab[K][VEC];
+  col.params(w, 1.f, C, g);
+  col.params(b, 0.f, C, be);
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const int c = (k * TPR + t) * VEC + i;
-      g[k][i] = c < C ? (w ? w[c] : 1.f) : 0.f;
-      be[k][i] = c < C && b ? b[c] : 0.f;
       aw[k][i] = 0.f;
       ab[k][i] = 0.f;
     }
   const float rc = 1.f / (float)C;
   for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)gridDim.x * (RPB * R)) {
     float v[R][K][VEC], d[R][K][VEC], mu[R], rs[R];
-    unsigned bits[R][K];
+    unsigned cw[R][K][VEC / 4], bits[R][K];
+    float step[R][K], step0[R][K];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long at = base + r * RPB + rg, row = at < rows ? at : rows - 1;
@@ -50,15 +53,21 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       rs[r] = rstd[row];
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * TPR + t) * VEC;
-        rv::load_chunk<T>(dy + row * dys + c, C - c, d[r][k]);
+        col.load(dy + row * dys, k, C, d[r][k]);
         if (FROM8) {
-          const bool in = c < C;
-          rv::load_codes<VEC>(codes + row * pitch + (in ? c : 0), rv::group_step(scales[row * G + (in ? c / rv::GROUP : 0)]),
-                              v[r][k]);
-          bits[r][k] = mask ? (unsigned)mask[row * MB + (in ? c / 8 : 0)] >> (c & 7) : 0xffu;
+          // a window that repeats values of its neighbour may start in the group before its own
+          const int c = min(col.c[k], (C - 1) & ~(VEC - 1)), at = col.at[k];
+          rv::load_codes(codes + row * pitch + at, cw[r][k]);
+          step[r][k] = rv::group_step(scales[row * G + c / rv::GROUP]);
+          step0[r][k] = ragged ? rv::group_step(scales[row * G + at / rv::GROUP]) : step[r][k];
+          bits[r][k] = 0xffffffffu;
+          if (mask) {
+            bits[r][k] = mask[row * MB + at / 8];
+            if (ragged) bits[r][k] |= (unsigned)mask[row * MB + min(at / 8 + 1, MB - 1)] << 8;
+            bits[r][k] >>= at & 7;
+          }
         } else {
-          rv::load_chunk<T>(x + row * xs + c, C - c, v[r][k]);
+          col.load(x + row * xs, k, C, v[r][k]);
         }
       }
     }
@@ -68,37 +77,42 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       const bool live = row < rows;
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
+        const float a = FROM8 ? step[r][k] : 0.f, a0 = FROM8 ? step0[r][k] : 0.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const bool in = (k * TPR + t) * VEC + i < C;
-          const float xh = in ? (v[r][k][i] - mu[r]) * rs[r] : 0.f;
-          bool on = in && live;
-          if (FROM8)
-            on = on && ((bits[r][k] >> i) & 1u);
-          else if (relu)
-            on = on && fmaf(xh, g[k][i], be[k][i]) > 0.f;
-          const float dz = on ? d[r][k][i] : 0.f;
+          const float xm = FROM8 ? fmaf(rv::code_at(cw[r][k], i), i < col.skip[k] ? a0 : a, -mu[r]) : v[r][k][i] - mu[r];
+          const float xh = xm * rs[r];
+          float dz;
+          if (FROM8) {
+            // bit i as a mask of the whole word
+            const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)(live ? bits[r][k] : 0u), i, 1);
+            dz = __uint_as_float(__float_as_uint(d[r][k][i]) & on);
+          } else {
+            const bool off_ = relu && fmaf(xh, g[k][i], be[k][i]) <= 0.f;          // (a NaN passes, as in the forward)
+            dz = live && !off_ ? d[r][k][i] : 0.f;
+          }
           aw[k][i] = fmaf(dz, xh, aw[k][i]);
           ab[k][i] += dz;
-          const float u = dz * g[k][i];
-          s1 += u;
-          s2 = fmaf(u, xh, s2);
+          const float u = dz * g[k][i], um = u * col.own[k][i];
+          s1 += um;
+          s2 = fmaf(um, xh, s2);
           d[r][k][i] = u;
           v[r][k][i] = xh;
         }
+      }
       if (dx) {
         s1 = row_sum<TPR>(s1, red) * rc;
         s2 = row_sum<TPR>(s2, red) * rc;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          const int c = (k * TPR + t) * VEC;
           float o[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            o[i] = c + i < C ? rs[r] * (d[r][k][i] - s1 - v[r][k][i] * s2) : 0.f;
-          if (live && c < dxcols) rv::store_chunk<T>(dx + row * dxs + c, dxcols - c, o);
+          for (int i = 0; i < VEC; ++i) o[i] = rs[r] * (d[r][k][i] - s1 - v[r][k][i] * s2);
+          if (live) col.store(dx + row * dxs, k, C, o);
         }
+        if (dxcols > C && live)
+          for (int c = C + t; c < dxcols; c += TPR) traits<T>::store1(dx + row * dxs + c, 0.f);
       }
     }
   }
@@ -108,13 +122,11 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = (k * TPR + t) * VEC + i;
-        if (c < C) {
-          pw[c] = aw[k][i];
-          pw[C + c] = ab[k][i];
+      for (int i = 0; i < VEC; ++i)
+        if (col.own[k][i] != 0.f) {
+          pw[col.at[k] + i] = aw[k][i];
+          pw[C + col.at[k] + i] = ab[k][i];
         }
-      }
     return;
   }
 #pragma unroll
@@ -134,7 +146,8 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) fold[wave * COLS + (k * TPR + t) * VEC + i] = which ? ab[k][i] : aw[k][i];
+        for (int i = 0; i < VEC; ++i)
+          if (col.own[k][i] != 0.f) fold[wave * COLS + col.at[k] + i] = which ? ab[k][i] : aw[k][i];
     }
     __syncthreads();
     for (int c = threadIdx.x; c < C; c += 256)
@@ -142,27 +155,9 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
   }
 }
 
-// part [P][2 C] -> dw, db: 32 columns x 32 slices of P per workgroup, in a fixed order
-__global__ __launch_bounds__(1024) void ln_grad_sum_kernel(int P, int C, const float* __restrict__ part,
-                                                           float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float s[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
-  float a = 0.f;
-  if (col < 2 * C)
-    for (int p = sl; p < P; p += 32) a += part[(size_t)p * 2 * C + col];
-  s[sl][threadIdx.x & 31] = a;
-  __syncthreads();
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    if (sl < o) s[sl][threadIdx.x & 31] += s[sl + o][threadIdx.x & 31];
-    __syncthreads();
-  }
-  if (sl == 0 && col < 2 * C) (col < C ? dw[col] : db[col - C]) = s[0][threadIdx.x & 31];
-}
-
 // workgroups of a rows backward launch = its partial sums
-int rows_grad_parts(int dtype, long long rows, int cover) {
-  const long long n = ln::rows_blocks(rows, ln::rows_threads(cover, ln::vec_of(dtype)), 1);
+int rows_grad_parts(int dtype, long long rows, int C) {
+  const long long n = ln::rows_blocks(rows, ln::rows_threads(C, ln::vec_of(dtype)), 1);
   return (int)(n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
 }
 
@@ -171,7 +166,6 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
                   const void* codes, long long pitch, const void* scales, const void* mask, const float* w, const float* b,
                   const float* mean, const float* rstd, int relu, void* dx, long long dxs, int dxcols, float* part,
                   hipStream_t st) {
-  const int cover = C > dxcols ? C : dxcols;
 #define LN_CALL(T, TPR, K, R)                                                                                            \
   do {                                                                                                                   \
     if (codes)                                                                                                           \
@@ -185,7 +179,7 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
                          (const unsigned char*)nullptr, (const unsigned char*)nullptr, w, b, mean, rstd, relu, (T*)dx,   \
                          dxs, dxcols, part);                                                                             \
   } while (0)
-  LN_ROWS_PICK(T, LN_CALL);
+  LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
   return 0;
@@ -193,15 +187,9 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
 
 }  // namespace
 
-int ln::sum_parts(int parts, int C, const float* part, float* dw, float* db, hipStream_t st) {
-  hipLaunchKernelGGL(ln_grad_sum_kernel, dim3(pvn3d_ceil_div(2 * C, 32)), dim3(1024), 0, st, parts, C, part, dw, db);
-  PVN3D_LAUNCH_CHECK();
-  return 0;
-}
-
-extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C, int cols) {
+extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C) {
   if (rows <= 0 || C <= 0 || C > ln::MAX_C || dtype < 0 || dtype > 2) return 0;
-  return (size_t)rows_grad_parts(dtype, rows, C > cols ? C : cols) * 2 * C * sizeof(float);
+  return (size_t)rows_grad_parts(dtype, rows, C) * 2 * C * sizeof(float);
 }
 extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x,
                                      long long xs, const void* codes, long long pitch, const void* scales,
@@ -221,8 +209,7 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
     return 0;
   }
   if (!dy || (!x && !codes) || !mean || !rstd) return (int)hipErrorInvalidValue;
-  if (!dx) dx_cols = C;
-  const int parts = rows_grad_parts(dtype, rows, dx_cols);
+  const int parts = rows_grad_parts(dtype, rows, C);
   if (dweight && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float))) return (int)hipErrorInvalidValue;
   float* part = dweight ? (float*)workspace : nullptr;
   int rc;
@@ -232,5 +219,5 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
     default: rc = rows_backward<fp16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, part, (hipStream_t)stream); break;
   }
   if (rc || !dweight) return rc;
-  return ln::sum_parts(parts, C, part, dweight, dbias, (hipStream_t)stream);
+  return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, (hipStream_t)stream);
 }

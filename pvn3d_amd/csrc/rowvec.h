@@ -71,37 +71,24 @@ template <> struct traits<fp16> {
   }
 };
 
-// One chunk of a row: `left` = values from p to the row's end (may be <= 0: zeros).  The whole chunk is one 16-byte load;
-// the last, partial chunk of a row is read value by value and never past the end.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* __restrict__ p, int left, float (&v)[traits<T>::VEC]) {
-  constexpr int VEC = traits<T>::VEC;
-  if (left >= VEC) {
-    traits<T>::unpack(*reinterpret_cast<const u4_any*>(p), v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = 0.f;
-    if (left > 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float f = traits<T>::load1(p + (i < left ? i : 0));
-        v[i] = i < left ? f : 0.f;
-      }
-    }
-  }
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[traits<T>::VEC]) {
+  traits<T>::unpack(*reinterpret_cast<const u4_any*>(p), v);
 }
-// `room` = values from p to the end of what may be written
 template <typename T>
-__device__ __forceinline__ void store_chunk(T* __restrict__ p, int room, const float (&v)[traits<T>::VEC]) {
-  constexpr int VEC = traits<T>::VEC;
-  if (room >= VEC) {
-    *reinterpret_cast<u4_any*>(p) = traits<T>::pack(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (i < room) traits<T>::store1(p + i, v[i]);
-  }
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[traits<T>::VEC]) {
+  *reinterpret_cast<u4_any*>(p) = traits<T>::pack(v);
 }
+
+// A lane's chunk of a row of C >= VEC values: whole chunks start at c, a multiple of VEC; the last, partial one is taken as
+// the row's last VEC values instead -- it overlaps its neighbour by `skip` values, which this lane computes a second time
+// (the same bits) and leaves out of every sum.  So all loads and stores are whole and unconditional: a guarded load is a
+// branch, and the loads behind it wait for the ones before.  A lane behind the row's end (c >= C) owns nothing.
+template <int VEC>
+struct window {
+  int c, at, skip;
+  __device__ __forceinline__ window(int c_, int C) : c(c_), at(min(c_, C - VEC)), skip(min(c_ - min(c_, C - VEC), VEC)) {}
+};
 
 // ---------------------------------------------------------------------------------------------- 8-bit group form
 // 32 consecutive channels of a row (the last group of a row may be shorter) share a power of two 2^e; a value is held as
@@ -117,60 +104,130 @@ __device__ __forceinline__ unsigned group_scale(unsigned absmax_bits) {
   const int e = (int)((absmax_bits + 0x10000u) >> 23) - 6;
   return absmax_bits >= 0x7f800000u ? 255u : (unsigned)min(max(e, 1), 248);
 }
-// 2^-e as fp32 (0 for a non-finite group: its codes are set to zero by group_code)
-__device__ __forceinline__ float group_inverse(unsigned scale) {
-  return scale == 255u ? 0.f : __uint_as_float((254u - scale) << 23);
-}
+__device__ __forceinline__ float group_inverse(unsigned scale) { return __uint_as_float((254u - min(scale, 248u)) << 23); }
 __device__ __forceinline__ float group_step(unsigned scale) { return __uint_as_float(scale << 23); }
-__device__ __forceinline__ int group_code(float x, float inverse) {
-  return inverse == 0.f ? 0 : (int)fminf(fmaxf(rintf(x * inverse), -127.f), 127.f);
-}
-// four codes, 2^e -> four values (exact; scale 255: 0 x inf = NaN)
-__device__ __forceinline__ void group_values(unsigned codes, float step, float (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)(signed char)(codes >> (8 * i)) * step;
-}
 
+// VEC codes, four to a word.  x 2^-e is exact and at most 127.5, so adding 1.5 2^23 leaves its integer part, rounded to
+// nearest even, in the low byte of the sum's bit pattern, two's complement.  Only the last scale needs codes held at 127 and
+// only 255 codes set to zero: one branch for a wave that has either.
 template <int VEC>
-__device__ __forceinline__ void load_codes(const signed char* __restrict__ p, float step, float (&v)[VEC]) {
-  if (VEC == 8) {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    float a[4], b[4];
-    group_values(r.x, step, a);
-    group_values(r.y, step, b);
+__device__ __forceinline__ void group_codes(const float (&v)[VEC], unsigned scale, unsigned (&w)[VEC / 4]) {
+  const float inverse = group_inverse(scale);
+  unsigned t[VEC];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[VEC / 2 + i] = b[i]; }
-  } else {
-    float a[4];
-    group_values(*reinterpret_cast<const unsigned*>(p), step, a);
+  for (int i = 0; i < VEC; ++i) t[i] = __float_as_uint(fmaf(v[i], inverse, 12582912.f));
+  if (__any(scale >= 248u)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i];
+    for (int i = 0; i < VEC; ++i)
+      t[i] = scale == 255u ? 0u : __float_as_uint(fminf(fmaxf(v[i] * inverse, -127.f), 127.f) + 12582912.f);
+  }
+#pragma unroll
+  for (int q = 0; q < VEC / 4; ++q)
+    w[q] = __builtin_amdgcn_perm(t[4 * q + 1], t[4 * q], 0x0c0c0400u) | __builtin_amdgcn_perm(t[4 * q + 3], t[4 * q + 2], 0x04000c0cu);
+}
+// a window's codes to their place: the values it skips are a neighbour's
+__device__ __forceinline__ void store_codes(signed char* __restrict__ row, int c, int skip, const unsigned (&w)[2]) {
+  const unsigned long long b = (((unsigned long long)w[1] << 32) | w[0]) >> (8 * (skip & 7));
+  *reinterpret_cast<uint2*>(row + c) = make_uint2((unsigned)b, (unsigned)(b >> 32));
+}
+__device__ __forceinline__ void store_codes(signed char* __restrict__ row, int c, int skip, const unsigned (&w)[1]) {
+  *reinterpret_cast<unsigned*>(row + c) = w[0] >> (8 * (skip & 3));
+}
+// the codes of a window, at any alignment
+struct __attribute__((packed, aligned(1))) u2_byte { unsigned x, y; };
+struct __attribute__((packed, aligned(1))) u1_byte { unsigned x; };
+__device__ __forceinline__ void load_codes(const signed char* __restrict__ p, unsigned (&w)[2]) {
+  const u2_byte r = *reinterpret_cast<const u2_byte*>(p);
+  w[0] = r.x;
+  w[1] = r.y;
+}
+__device__ __forceinline__ void load_codes(const signed char* __restrict__ p, unsigned (&w)[1]) {
+  w[0] = reinterpret_cast<const u1_byte*>(p)->x;
+}
+// code i as fp32; times the group's step: the held value (exact; scale 255: 0 x inf = NaN)
+template <int N>
+__device__ __forceinline__ float code_at(const unsigned (&w)[N], int i) { return (float)(signed char)(w[i >> 2] >> (8 * (i & 3))); }
+
+// ---------------------------------------------------------------------------------------------- across lanes
+// Sums and maxima over 2, 4, .. 64 neighbouring lanes, every lane getting the result: the mirrored permutations equal an
+// exchange with lane ^ 4 / lane ^ 8 once the smaller groups hold one value each.
+__device__ __forceinline__ unsigned dpp(unsigned v, int step) {
+  switch (step) {
+    case 1: return __builtin_amdgcn_update_dpp(0u, v, 0xB1, 0xf, 0xf, true);       // quad_perm 1 0 3 2
+    case 2: return __builtin_amdgcn_update_dpp(0u, v, 0x4E, 0xf, 0xf, true);       // quad_perm 2 3 0 1
+    case 4: return __builtin_amdgcn_update_dpp(0u, v, 0x141, 0xf, 0xf, true);      // row_half_mirror
+    default: return __builtin_amdgcn_update_dpp(0u, v, 0x140, 0xf, 0xf, true);     // row_mirror
   }
 }
-
-// The scale of this lane's group: LANES consecutive lanes (a power of two) hold the group's values, VEC each
-template <int VEC, int LANES>
-__device__ __forceinline__ unsigned lanes_scale(const float (&v)[VEC]) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);   // as integers: NaN is the largest
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-  return group_scale(m);
+__device__ __forceinline__ float add16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-template <int VEC>
-__device__ __forceinline__ void store_codes(signed char* __restrict__ p, const float (&v)[VEC], float inverse) {
-  unsigned w[VEC / 4];
+__device__ __forceinline__ float add32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if (LANES > 1) v += __uint_as_float(dpp(__float_as_uint(v), 1));
+  if (LANES > 2) v += __uint_as_float(dpp(__float_as_uint(v), 2));
+  if (LANES > 4) v += __uint_as_float(dpp(__float_as_uint(v), 4));
+  if (LANES > 8) v += __uint_as_float(dpp(__float_as_uint(v), 8));
+  if (LANES > 16) v = add16(v);
+  if (LANES > 32) v = add32(v);
+  return v;
+}
+template <int LANES>                                      // 8 lanes at most
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+  if (LANES > 1) v = max(v, dpp(v, 1));
+  if (LANES > 2) v = max(v, dpp(v, 2));
+  if (LANES > 4) v = max(v, dpp(v, 4));
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------- partial sums
+// out[e] = sum over p of part[p][count], e < count, in a fixed order: SL slices of p a workgroup, 1024 / SL columns, eight
+// loads in flight per thread.  e < first goes to a, the rest to b.
+template <int SL>
+__global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t first, const float* __restrict__ part,
+                                                    float* __restrict__ a, float* __restrict__ b) {
+  constexpr int COLS = 1024 / SL;
+  __shared__ float s[SL][COLS];
+  const int col = threadIdx.x % COLS, sl = threadIdx.x / COLS;
+  const size_t e = (size_t)blockIdx.x * COLS + col;
+  float v = 0.f;
+  if (e < count) {
+    const float* p = part + e;
+    int i = sl;
+    for (; i + 7 * SL < P; i += 8 * SL) {
+      float f[8];
 #pragma unroll
-  for (int q = 0; q < VEC / 4; ++q) {
-    w[q] = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[q] |= ((unsigned)group_code(v[q * 4 + i], inverse) & 0xffu) << (8 * i);
+      for (int j = 0; j < 8; ++j) f[j] = p[(size_t)(i + j * SL) * count];
+      v += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    }
+    for (; i < P; i += SL) v += p[(size_t)i * count];
   }
-  if (VEC == 8)
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[VEC / 4 - 1]);
-  else
-    *reinterpret_cast<unsigned*>(p) = w[0];
+  s[sl][col] = v;
+  __syncthreads();
+#pragma unroll
+  for (int o = SL / 2; o >= 1; o >>= 1) {
+    if (sl < o) s[sl][col] += s[sl + o][col];
+    __syncthreads();
+  }
+  if (sl == 0 && e < count) (e < first ? a[e] : b[e - first]) = s[0][col];
+}
+static inline int fold(int P, size_t count, size_t first, const float* part, float* a, float* b, hipStream_t st) {
+  // slices: as many as leave a thread about eight partial sums (64 slices of 16 columns still read whole 64-byte lines)
+#define RV_FOLD(SL)                                                                                                   \
+  hipLaunchKernelGGL((fold_kernel<SL>), dim3((unsigned)((count + 1024 / SL - 1) / (1024 / SL))), dim3(1024), 0, st, P, \
+                     count, first, part, a, b)
+  if (P >= 256) RV_FOLD(64);
+  else if (P >= 64) RV_FOLD(32);
+  else if (P >= 16) RV_FOLD(8);
+  else RV_FOLD(2);
+#undef RV_FOLD
+  PVN3D_LAUNCH_CHECK();
+  return 0;
 }
 
 }  // namespace rv

@@ -49,10 +49,17 @@ def _by_rows(x, channel_dim):
     else:
         _need(d == 1, "channel_dim must be 1 or the last dimension")
         C = x.size(1)
-        rows = x.movedim(1, -1).is_contiguous() and not x.is_contiguous()
+        # a point-major view in place; fewer points than a chunk of the channel-major kernel: as rows of a copy
+        few = x.numel() // max(1, x.size(0) * C) < 4
+        rows = few or (x.movedim(1, -1).is_contiguous() and not x.is_contiguous())
         x = x.movedim(1, -1) if rows else x.contiguous()
     _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
     return rows, x
+
+
+def _like(y, x):
+    """A channels-second result in x's layout: channel-major if x is, else the point-major view it is."""
+    return y.contiguous() if x.is_contiguous() else y
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False):
@@ -73,7 +80,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
                                        1 if relu else 0, y.data_ptr(), C, C, mean.data_ptr(), rstd.data_ptr(), None, 0,
                                        None, None, _stream(x)), "layer_norm")
             if v is not x:
-                y = y.movedim(-1, 1)
+                y = _like(y.movedim(-1, 1), x)
         else:
             check(lib.pvn3d_layer_norm_chan(DTYPES[v.dtype], v.size(0), C, n // max(v.size(0), 1), v.data_ptr(), _ptr(w),
                                             _ptr(b), float(eps), 1 if relu else 0, y.data_ptr(), mean.data_ptr(),
@@ -111,13 +118,13 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=Fa
         if rows:
             d = dy if v is x else dy.movedim(1, -1)
             (m, xs), (g, gs) = _rows(v, "x"), _rows(d, "dy")
-            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C, C) if need_dparams else 0
+            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
             ws = _workspace(wsb, dev)
             check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, m.data_ptr(), xs, None, 0, None, None, _ptr(w),
                                             _ptr(b), mean.data_ptr(), rstd.data_ptr(), 1 if relu else 0, _ptr(dx), C, C,
                                             pw, pb, _ptr(ws), wsb, st), "layer_norm_grad")
             if need_dx and v is not x:
-                dx = dx.movedim(-1, 1)
+                dx = _like(dx.movedim(-1, 1), x)
         else:
             g = dy.contiguous()
             B = v.size(0)
@@ -182,7 +189,7 @@ def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True
         g, gs = _rows(dy, "dy")
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev) if need_dx else None
         dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
-        wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C, C) if need_dparams else 0
+        wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
         ws = _workspace(wsb, dev)
         pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
         check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, None, 0, act.codes.data_ptr(), act.pitch,

@@ -44,8 +44,8 @@ def test_layer_norm_entry_points_refuse():
     assert lib.pvn3d_layer_norm_chan_grad(0, 2, 8, 4, P, P, None, None, P, P, 0, P, P, P, None, 0, None) != 0
     assert lib.pvn3d_layer_norm_chan(0, 0, 8, 4, P, None, None, 1e-5, 0, P, P, P, None) == 0
     # the workspace holds a partial dweight and dbias per workgroup
-    assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 10 ** 6, 64, 64) % (2 * 64 * 4) == 0
-    assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 0, 64, 64) == 0
+    assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 10 ** 6, 64) % (2 * 64 * 4) == 0
+    assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 0, 64) == 0
 
 
 def test_act8_entry_points_refuse():
