@@ -636,7 +636,8 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
 /* ---- Layer norm over the channels of every point (csrc/layer_norm*.hip; no reference counterpart) -------------
  * Beside the BatchNorm passes above: mean, var over a point's own channels, rstd = 1 / sqrt(var + eps),
  * xh = (x - mean) rstd, z = weight xh + bias, y = z or (relu != 0) max(z, 0).  dtype 0 fp32, 1 bf16, 2 fp16 (x, y, dy,
- * dx); weight, bias (either may be NULL: ones, zeros), statistics and parameter gradients fp32.  1 <= C <= 8192.
+ * dx); weight, bias (either may be NULL: ones, zeros), statistics and parameter gradients fp32.  1 <= C <= 8192; row
+ * strides (and pitch) of 2^20 elements at most.
  * pvn3d_layer_norm: rows [rows][C] of stride xs (elements, any alignment) -> y [rows] of stride ys; columns C .. y_cols - 1
  *   (y_cols <= C + 15) are written as zeros.  codes != NULL: x also goes to codes / scales in the 8-bit form of
  *   pvn3d_act8_pack, and mask (may be NULL) gets bit c & 7 of byte [row][c / 8], row length ceil(C / 8), = z > 0.
@@ -645,7 +646,7 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
  *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C) names, 4-byte aligned, needed for dweight
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
- * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, M >= 4 (or 0); mean, rstd (B, M). */
+ * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^24 (or 0); mean, rstd (B, M). */
 int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
                      float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
                      long long pitch, void* scales, void* mask, void* stream);

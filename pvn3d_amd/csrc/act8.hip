@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, i
       }
       const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
       rv::group_codes<VEC>(v, sc, wd);
-      if (c < C) rv::store_codes(codes + row * pitch, c, skip, wd);
+      if (c < C) rv::store_codes(codes + row * pitch + c, skip, wd);
       if ((c & (rv::GROUP - 1)) == 0) scales[row * G + c / rv::GROUP] = (unsigned char)sc;
     }
   }

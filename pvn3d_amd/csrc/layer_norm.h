@@ -9,7 +9,12 @@ using rv::fp16;
 using rv::traits;
 
 constexpr int MAX_C = 8192;
-constexpr int MAX_PARTS = 1024;      // workgroups of a backward launch, each with a partial dw and db
+// Workgroups of a backward launch, each with a partial dw and db: what the registers of one chunk a lane let stay on the
+// chip (bf16, 98304 x 1024, two chunks a lane: 111 us from the 8-bit input, 124 with 1024; the others within 2 %).
+constexpr int MAX_PARTS = 2048;
+// Row strides the kernels take: a workgroup addresses its rows (512 at most) as one base and 32-bit byte offsets -- the
+// 64-bit products of a row index cost more than the arithmetic on the row.
+constexpr long long MAX_STRIDE = 1 << 20;
 
 // sum over the TPR lanes of a row; TPR = 256: over the workgroup (a barrier: every thread of it calls this)
 template <int TPR>
@@ -51,23 +56,35 @@ struct lane_cols {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[k][i] = at[k] + i < C ? (p ? p[at[k] + i] : missing) : 0.f;
-  }
-  __device__ __forceinline__ void load(const T* __restrict__ row, int k, int C, float (&v)[VEC]) const {
-    if (TPR > 1) {
-      rv::load_vec<T>(row + at[k], v);
-    } else {
+      for (int i = 0; i < VEC; i += 4) {
+        float f[4] = {missing, missing, missing, missing};
+        if (p && TPR > 1) {
+          traits<float>::unpack(*reinterpret_cast<const rv::u4_any*>(p + at[k] + i), f);
+        } else if (p) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(row + i) : 0.f;
-    }
+          for (int j = 0; j < 4; ++j) f[j] = i + j < C ? p[i + j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][i + j] = f[j];
+      }
   }
-  __device__ __forceinline__ void store(T* __restrict__ row, int k, int C, const float (&v)[VEC]) const {
+  // the chunk as loaded; row: its place behind base, in elements
+  __device__ __forceinline__ rv::u4_any load(const T* __restrict__ base, unsigned row, int k, int C) const {
+    const T* const p = rv::at32(base, (row + at[k]) * (unsigned)sizeof(T));
+    if (TPR > 1) return *reinterpret_cast<const rv::u4_any*>(p);
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(p + i) : 0.f;
+    return traits<T>::pack(v);                         // (exact: the values are of type T)
+  }
+  __device__ __forceinline__ void store(T* __restrict__ base, unsigned row, int k, int C, const float (&v)[VEC]) const {
+    T* const p = rv::at32(base, (row + at[k]) * (unsigned)sizeof(T));
     if (TPR > 1) {
-      if (c[k] < C) rv::store_vec<T>(row + at[k], v);
+      if (c[k] < C) rv::store_vec<T>(p, v);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (i < C) traits<T>::store1(row + i, v[i]);
+        if (i < C) traits<T>::store1(p + i, v[i]);
     }
   }
 };

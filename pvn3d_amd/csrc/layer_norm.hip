@@ -25,11 +25,11 @@ using ln::row_sum;
 // TPR threads share a row, chunk k of thread t = the VEC channels from (k TPR + t) VEC on (16 bytes): K chunks cover the
 // row, R rows per thread are in flight at once.
 template <typename T, int TPR, int K, int R, bool SAVE8>
-__global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, const T* __restrict__ x, long long xs,
+__global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, const T* __restrict__ x, int xs,
                                                       const float* __restrict__ w, const float* __restrict__ b, float eps,
-                                                      int relu, T* __restrict__ y, long long ys, int ycols,
+                                                      int relu, T* __restrict__ y, int ys, int ycols,
                                                       float* __restrict__ mean, float* __restrict__ rstd,
-                                                      signed char* __restrict__ codes, long long pitch,
+                                                      signed char* __restrict__ codes, int pitch,
                                                       unsigned char* __restrict__ scales,
                                                       unsigned char* __restrict__ mask) {
   constexpr int VEC = traits<T>::VEC;
@@ -41,38 +41,48 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
   float g[K][VEC], be[K][VEC];
   col.params(w, 1.f, C, g);
   col.params(b, 0.f, C, be);
-  const float rc = 1.f / (float)C, floor = relu ? 0.f : -__builtin_inff();
+  const float rc = 1.f / (float)C;
+  float low = relu ? 0.f : -__builtin_inff();
+  asm("" : "+v"(low));             // a register, not a choice of two constants at every use
   for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)gridDim.x * (RPB * R)) {
-    float v[R][K][VEC];
+    const int last = (int)(rows - 1 - base < RPB * R - 1 ? rows - 1 - base : RPB * R - 1);
+    const T* const xb = x + base * xs;
+    T* const yb = y + base * ys;
+    signed char* const cb = codes + base * pitch;
+    unsigned char* const sb = scales + base * G;
+    unsigned char* const mb = mask + base * MB;
+    rv::u4_any raw[R][K];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = base + r * RPB + rg;
-      const T* const p = x + (row < rows ? row : rows - 1) * xs;
+      const unsigned row = __umul24(min(rg + r * RPB, last), xs);
 #pragma unroll
-      for (int k = 0; k < K; ++k) col.load(p, k, C, v[r][k]);
+      for (int k = 0; k < K; ++k) raw[r][k] = col.load(xb, row, k, C);
     }
+    __builtin_amdgcn_sched_barrier(0);       // all loads on their way before anything waits for one
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = base + r * RPB + rg;
-      const bool live = row < rows;
-      float s = 0.f;
+      const int rl = rg + r * RPB;
+      const bool live = rl <= last;
+      float v[K][VEC], s = 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
+        traits<T>::unpack(raw[r][k], v[k]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s = fmaf(v[r][k][i], col.own[k][i], s);
+        for (int i = 0; i < VEC; ++i) s = fmaf(v[k][i], col.own[k][i], s);
+      }
       const float mu = row_sum<TPR>(s, red) * rc;
       float q = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float d = v[r][k][i] - mu;
+          const float d = v[k][i] - mu;
           q = fmaf(d * col.own[k][i], d, q);
         }
-      const float rs = 1.f / sqrtf(row_sum<TPR>(q, red) * rc + eps);
+      const float rs = __builtin_amdgcn_rsqf(fmaf(row_sum<TPR>(q, red), rc, eps));      // v_rsq_f32: within one ulp
       if (live && t == 0) {
-        mean[row] = mu;
-        rstd[row] = rs;
+        *rv::at32(mean + base, rl * 4u) = mu;
+        *rv::at32(rstd + base, rl * 4u) = rs;
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -80,21 +90,21 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
         float z[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i)       // (maximum: a NaN stays one, which max(z, 0) would make 0)
-          z[i] = __builtin_elementwise_maximum(fmaf((v[r][k][i] - mu) * rs, g[k][i], be[k][i]), floor);
-        if (live) col.store(y + row * ys, k, C, z);
+          z[i] = __builtin_elementwise_maximum(fmaf((v[k][i] - mu) * rs, g[k][i], be[k][i]), low);
+        if (live) col.store(yb, __umul24(rl, ys), k, C, z);
         if (SAVE8) {
           constexpr int LPG = rv::GROUP / VEC < TPR ? rv::GROUP / VEC : TPR;       // lanes per group
           unsigned big = 0, wd[VEC / 4];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {                      // as integers: NaN is the largest
-            const unsigned a = __float_as_uint(v[r][k][i]) & 0x7fffffffu;
+            const unsigned a = __float_as_uint(v[k][i]) & 0x7fffffffu;
             big = max(big, col.own[k][i] != 0.f ? a : 0u);
           }
           const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
-          rv::group_codes<VEC>(v[r][k], sc, wd);
+          rv::group_codes<VEC>(v[k], sc, wd);
           if (live && c < C) {
-            rv::store_codes(codes + row * pitch, c, col.skip[k], wd);
-            if ((c & (rv::GROUP - 1)) == 0) scales[row * G + c / rv::GROUP] = (unsigned char)sc;
+            rv::store_codes(rv::at32(cb, __umul24(rl, pitch) + c), col.skip[k], wd);
+            if ((c & (rv::GROUP - 1)) == 0) *rv::at32(sb, __umul24(rl, G) + c / rv::GROUP) = (unsigned char)sc;
           }
           if (mask) {                                          // y is 0 or positive here: minus its bits, the sign bit
             unsigned bits = 0;
@@ -105,15 +115,21 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
               const unsigned other = rv::dpp(bits, 1);
               bits |= c + 4 < C ? other << 4 : 0u;
             }
-            if (live && c < C && (c & 7) == 0) mask[row * MB + c / 8] = (unsigned char)bits;
+            if (live && c < C && (c & 7) == 0) *rv::at32(mb, __umul24(rl, MB) + c / 8) = (unsigned char)bits;
           }
         }
       }
       if (ycols > C && live)
-        for (int c = C + t; c < ycols; c += TPR) traits<T>::store1(y + row * ys + c, 0.f);
+#pragma unroll 1
+        for (int c = C + t; c < ycols; c += TPR) traits<T>::store1(rv::at32(yb, (__umul24(rl, ys) + c) * (unsigned)sizeof(T)), 0.f);
     }
   }
 }
+
+// Workgroups of a forward launch: enough to keep every CU at its eight and to end evenly, few enough that loading the
+// parameters is spread over several rows (bf16, 786432 x 128: 75.7 us; 1024 workgroups 77.3, one per 32 rows 74.8 -- and
+// 98304 x 1024 with the input saved: 100 us against 114 with one per four rows).
+constexpr long long MAX_GRID = 8192;
 
 template <typename T>
 int rows_forward(long long rows, int C, const void* x, long long xs, const float* w, const float* b, float eps, int relu,
@@ -122,14 +138,14 @@ int rows_forward(long long rows, int C, const void* x, long long xs, const float
 #define LN_CALL(T, TPR, K, R)                                                                                           \
   do {                                                                                                                  \
     const long long nb = ln::rows_blocks(rows, TPR, R);                                                                     \
-    const dim3 grid((unsigned)(nb < 16384 ? nb : 16384));                                                               \
+    const dim3 grid((unsigned)(nb < MAX_GRID ? nb : MAX_GRID));                                                               \
     if (codes)                                                                                                          \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, xs, w, b, \
-                         eps, relu, (T*)y, ys, ycols, mean, rstd, (signed char*)codes, pitch, (unsigned char*)scales,   \
+      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, b, \
+                         eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch, (unsigned char*)scales,   \
                          (unsigned char*)mask);                                                                         \
     else                                                                                                                \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, xs, w, b, \
-                         eps, relu, (T*)y, ys, ycols, mean, rstd, nullptr, 0ll, nullptr, nullptr);                      \
+      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, b, \
+                         eps, relu, (T*)y, (int)ys, ycols, mean, rstd, nullptr, 0, nullptr, nullptr);                      \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
@@ -144,6 +160,7 @@ extern "C" int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x,
                                 float* rstd, void* codes, long long pitch, void* scales, void* mask, void* stream) {
   if (dtype < 0 || dtype > 2 || C <= 0 || C > ln::MAX_C || y_cols < C || y_cols > C + 15 || ys < y_cols || xs < 0)
     return (int)hipErrorInvalidValue;
+  if (xs > ln::MAX_STRIDE || ys > ln::MAX_STRIDE || pitch > ln::MAX_STRIDE) return (int)hipErrorInvalidValue;
   if (codes && (!scales || (pitch & 15) || pitch < C)) return (int)hipErrorInvalidValue;
   if (rows <= 0) return 0;
   if (!x || !y || !mean || !rstd) return (int)hipErrorInvalidValue;

@@ -1,10 +1,12 @@
 // layer_norm_chan.hip -- layer norm over the channels of (B, C, M) tensors, M contiguous: the layout in which the modules
 // hand features on.  The formulas are those of layer_norm.hip.
 //
-// 16 lanes x 4 consecutive points across, blockDim.x / 16 channel slots down: a thread holds channels cy, cy + CY, ... (KC
-// of them) of its four points in registers, as loaded (unpacked at each use), so memory is read once.  The sums over the
-// channels go through two shuffles and one LDS exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more
-// channels than the registers of 1024 threads hold -- x is read again for every pass.
+// A tile is 64 consecutive points of one cloud: 16 lanes x 4 points across, blockDim.x / 16 channel slots down.  A thread
+// holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
+// is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
+// every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
+// exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more channels than the registers of 1024 threads hold
+// -- x is read again for every pass.
 #include "layer_norm.h"
 
 namespace {
@@ -35,17 +37,32 @@ __device__ __forceinline__ raw4<T> shut(const float (&v)[4]) {
 template <>
 __device__ __forceinline__ raw4<float> shut<float>(const float (&v)[4]) { return raw4<float>{traits<float>::pack(v)}; }
 
+// The compiler forgets what it has derived from a chunk: values unpacked before a barrier are not kept in registers for
+// their second use behind it (they were twice the chunk's size).
+template <typename T>
+__device__ __forceinline__ void forget(raw4<T>& a) {
+  unsigned p = a.r.x, q = a.r.y;
+  asm volatile("" : "+v"(p), "+v"(q));
+  a.r.x = p;
+  a.r.y = q;
+}
+template <>
+__device__ __forceinline__ void forget<float>(raw4<float>& a) {
+  unsigned p = a.r.x, q = a.r.y, s = a.r.z, t = a.r.w;
+  asm volatile("" : "+v"(p), "+v"(q), "+v"(s), "+v"(t));
+  a.r = rv::u4_any{p, q, s, t};
+}
+
 // Chunks are whole and unconditional: the last, partial one of a row of points is taken as its last four points, which
-// overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.
+// overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.  Lanes behind the
+// cloud's last point repeat its last four without a store.
 struct tile_at {
   int b, m0, skip;
   bool live;
-  __device__ __forceinline__ tile_at(int tile, int NV, int MV, int M) {
-    const int pv = tile * 16 + (threadIdx.x & 15);
-    live = pv < NV;
-    const int at = live ? pv : NV - 1;
-    b = at / MV;
-    const int m = (at - b * MV) * PTS;
+  __device__ __forceinline__ tile_at(int tile, int per_cloud, int M) {
+    b = tile / per_cloud;
+    const int m = ((tile - b * per_cloud) * 16 + (threadIdx.x & 15)) * PTS;
+    live = m < M;
     m0 = min(m, M - PTS);
     skip = m - m0;
   }
@@ -70,75 +87,86 @@ __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[16 * N]) {
 }
 
 template <typename T, int KC>
-__global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int B, int C, int M, int MV, const T* __restrict__ x,
+__global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per_cloud, int C, int M, const T* __restrict__ x,
                                                               const float* __restrict__ w, const float* __restrict__ b,
                                                               float eps, int relu, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int KR = KC > 0 ? KC : 1;
   __shared__ float buf[2][MAX_THREADS / 64][16 * PTS];
   const int cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
-  const int NV = B * MV;
-  const float rc = 1.f / (float)C, floor = relu ? 0.f : -__builtin_inff();
-  for (int tile = blockIdx.x; tile < (NV + 15) / 16; tile += gridDim.x) {
-    const tile_at at(tile, NV, MV, M);
-    const size_t off = (size_t)at.b * C * M + at.m0;
-    const T* const p = x + off;
-    T* const q = y + off;
+  const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
+  const float rc = 1.f / (float)C;
+  float low = relu ? 0.f : -__builtin_inff();
+  asm("" : "+v"(low));             // a register, not a choice of two constants at every use
+  float gk[KR], bk[KR];
+  bool has[KR];                    // (only the last of a thread's channels can be missing)
+#pragma unroll
+  for (int k = 0; k < KR; ++k) {
+    const int c = cy + k * CY;
+    has[k] = k < KR - 1 || c < C;
+    gk[k] = KC > 0 && w && has[k] ? w[c] : 1.f;
+    bk[k] = KC > 0 && b && has[k] ? b[c] : 0.f;
+  }
+  const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const tile_at at(tile, per_cloud, M);
+    const T* const p = x + at.b * C * M_;
+    T* const q = y + at.b * C * M_;
+    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> r[KR];
     float s[PTS] = {0.f, 0.f, 0.f, 0.f}, mu[PTS], rs[PTS];
     if (KC > 0) {
 #pragma unroll
-      for (int k = 0; k < KR; ++k) {
-        const int c = cy + k * CY;
-        r[k] = *reinterpret_cast<const raw4<T>*>(p + (size_t)(c < C ? c : 0) * M);
-      }
+      for (int k = 0; k < KR; ++k) r[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(p + k * slots, k < KR - 1 ? o : ol));
+      __builtin_amdgcn_sched_barrier(0);     // all loads on their way before anything waits for one
     }
-    // f(channel, values) for each of the thread's channels
+    // f(k, channel's base, channel, values) for each of the thread's channels
     auto each = [&](auto f) {
       float v[PTS];
       if (KC > 0) {
 #pragma unroll
         for (int k = 0; k < KR; ++k) {
-          if (cy + k * CY < C) {
+          if (has[k]) {
             open<T>(r[k], v);
-            f(cy + k * CY, v);
+            f(k, k * slots, cy + k * CY, v);
           }
         }
       } else {
-        for (int c = cy; c < C; c += CY) {
-          open<T>(*reinterpret_cast<const raw4<T>*>(p + (size_t)c * M), v);
-          f(c, v);
+        size_t at_c = 0;
+        for (int c = cy; c < C; c += CY, at_c += slots) {
+          open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(p + at_c, o)), v);
+          f(0, at_c, c, v);
         }
       }
     };
-    each([&](int, const float (&v)[PTS]) {
+    each([&](int, size_t, int, const float (&v)[PTS]) {
 #pragma unroll
       for (int i = 0; i < PTS; ++i) s[i] += v[i];
     });
     slot_sum<PTS>(s, buf[0]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) { mu[i] = s[i] * rc; s[i] = 0.f; }
-    each([&](int, const float (&v)[PTS]) {
+    each([&](int, size_t, int, const float (&v)[PTS]) {
 #pragma unroll
       for (int i = 0; i < PTS; ++i) s[i] = fmaf(v[i] - mu[i], v[i] - mu[i], s[i]);
     });
     slot_sum<PTS>(s, buf[1]);
 #pragma unroll
-    for (int i = 0; i < PTS; ++i) rs[i] = 1.f / sqrtf(s[i] * rc + eps);
+    for (int i = 0; i < PTS; ++i) rs[i] = __builtin_amdgcn_rsqf(fmaf(s[i], rc, eps));       // v_rsq_f32: within one ulp
     if (at.live && cy == 0) {
 #pragma unroll
       for (int i = 0; i < PTS; ++i) {
-        mean[(size_t)at.b * M + at.m0 + i] = mu[i];
-        rstd[(size_t)at.b * M + at.m0 + i] = rs[i];
+        mean[at.b * M_ + at.m0 + i] = mu[i];
+        rstd[at.b * M_ + at.m0 + i] = rs[i];
       }
     }
-    each([&](int c, const float (&v)[PTS]) {
-      const float g = w ? w[c] : 1.f, be = b ? b[c] : 0.f;
+    each([&](int k, size_t at_c, int c, const float (&v)[PTS]) {
+      const float g = KC > 0 ? gk[k] : w ? w[c] : 1.f, be = KC > 0 ? bk[k] : b ? b[c] : 0.f;
       float z[PTS];
 #pragma unroll
       for (int i = 0; i < PTS; ++i)                      // (maximum: a NaN stays one)
-        z[i] = __builtin_elementwise_maximum(fmaf((v[i] - mu[i]) * rs[i], g, be), floor);
-      if (at.live) *reinterpret_cast<raw4<T>*>(q + (size_t)c * M) = shut<T>(z);
+        z[i] = __builtin_elementwise_maximum(fmaf((v[i] - mu[i]) * rs[i], g, be), low);
+      if (at.live) *reinterpret_cast<raw4<T>*>(rv::at32(q + at_c, o)) = shut<T>(z);
     });
   }
 }
@@ -146,8 +174,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int B, int C, int 
 // dw / db: a thread has the same channels for all its tiles: a register each, summed over the 16 lanes at the end (KC = 0:
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
 template <typename T, int KC>
-__global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C, int M, int MV, const T* __restrict__ dy,
-                                                                   const T* __restrict__ x, const float* __restrict__ w,
+__global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int per_cloud, int C, int M,
+                                                                   const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ w,
                                                                    const float* __restrict__ b,
                                                                    const float* __restrict__ mean,
                                                                    const float* __restrict__ rstd, int relu,
@@ -156,116 +184,147 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
   __shared__ float buf[2][MAX_THREADS / 64][16 * 2 * PTS];
   extern __shared__ float lacc[];
   const int px = threadIdx.x & 15, cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
-  const int NV = B * MV;
+  const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
   const float rc = 1.f / (float)C;
-  float aw[KR], ab[KR];
+  float aw[KR], ab[KR], gk[KR], bk[KR];
+  bool has[KR];                    // (only the last of a thread's channels can be missing)
 #pragma unroll
-  for (int k = 0; k < KR; ++k) { aw[k] = 0.f; ab[k] = 0.f; }
+  for (int k = 0; k < KR; ++k) {
+    const int c = cy + k * CY;
+    has[k] = k < KR - 1 || c < C;
+    aw[k] = 0.f;
+    ab[k] = 0.f;
+    gk[k] = KC > 0 && w && has[k] ? w[c] : 1.f;
+    bk[k] = KC > 0 && b && has[k] ? b[c] : 0.f;
+  }
+  const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
   if (KC == 0) {
     for (int c = threadIdx.x; c < 2 * C; c += blockDim.x) lacc[c] = 0.f;
     __syncthreads();
   }
   int turn = 0;
-  for (int tile = blockIdx.x; tile < (NV + 15) / 16; tile += gridDim.x, turn ^= 1) {
-    const tile_at at(tile, NV, MV, M);
-    const size_t off = (size_t)at.b * C * M + at.m0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+    const tile_at at(tile, per_cloud, M);
+    const T* const px_ = x + at.b * C * M_;
+    const T* const pd_ = dy + at.b * C * M_;
+    T* const po_ = dx + at.b * C * M_;
+    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> rx[KR], rd[KR];
     float mu[PTS], rs[PTS], s[2 * PTS];
 #pragma unroll
     for (int i = 0; i < PTS; ++i) {
-      const size_t mi = (size_t)at.b * M + at.m0 + i;
-      mu[i] = mean[mi];
-      rs[i] = rstd[mi];
+      mu[i] = mean[at.b * M_ + at.m0 + i];
+      rs[i] = rstd[at.b * M_ + at.m0 + i];
       s[i] = 0.f;
       s[PTS + i] = 0.f;
     }
     if (KC > 0) {
 #pragma unroll
       for (int k = 0; k < KR; ++k) {
-        const size_t o = off + (size_t)(cy + k * CY < C ? cy + k * CY : 0) * M;
-        rx[k] = *reinterpret_cast<const raw4<T>*>(x + o);
-        rd[k] = *reinterpret_cast<const raw4<T>*>(dy + o);
+        rx[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(px_ + k * slots, k < KR - 1 ? o : ol));
+        rd[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(pd_ + k * slots, k < KR - 1 ? o : ol));
       }
+      __builtin_amdgcn_sched_barrier(0);     // all loads on their way before anything waits for one
     }
-    // f(k, channel, xh, dz, weight) for each of the thread's channels; dz = 0 where the ReLU is off and in a lane without
-    // points
-    auto each = [&](auto f) {
-      float v[PTS], d[PTS];
-      auto one = [&](int k, int c) {
-        const float g = w ? w[c] : 1.f, be = b ? b[c] : 0.f;
-#pragma unroll
-        for (int i = 0; i < PTS; ++i) {
-          v[i] = (v[i] - mu[i]) * rs[i];
-          const bool off_ = relu && fmaf(v[i], g, be) <= 0.f;      // (a NaN passes, as in the forward)
-          d[i] = at.live && !off_ ? d[i] : 0.f;
-        }
-        f(k, c, v, d, g);
-      };
-      if (KC > 0) {
-#pragma unroll
-        for (int k = 0; k < KR; ++k) {
-          if (cy + k * CY < C) {
-            open<T>(rx[k], v);
-            open<T>(rd[k], d);
-            one(k, cy + k * CY);
-          }
-        }
-      } else {
-        for (int c = cy; c < C; c += CY) {
-          open<T>(*reinterpret_cast<const raw4<T>*>(x + off + (size_t)c * M), v);
-          open<T>(*reinterpret_cast<const raw4<T>*>(dy + off + (size_t)c * M), d);
-          one(0, c);
-        }
-      }
-    };
-    each([&](int k, int c, const float (&xh)[PTS], const float (&dz)[PTS], float g) {
-      float w1 = 0.f, b1 = 0.f;
+    // one channel's x, dy -> xh and dz, dz = 0 where the ReLU is off and in a lane without points
+    auto one = [&](float g, float be, float (&v)[PTS], float (&d)[PTS]) {
 #pragma unroll
       for (int i = 0; i < PTS; ++i) {
-        const float own = i >= at.skip ? dz[i] : 0.f;
+        v[i] = (v[i] - mu[i]) * rs[i];
+        const bool off_ = relu && fmaf(v[i], g, be) <= 0.f;        // (a NaN passes, as in the forward)
+        d[i] = at.live && !off_ ? d[i] : 0.f;
+      }
+    };
+    // its share of the sums over the channels, and of dw, db
+    auto add = [&](float g, const float (&xh)[PTS], const float (&dz)[PTS], float& w1, float& b1) {
+#pragma unroll
+      for (int i = 0; i < PTS; ++i) {
+        const float own = i >= at.skip ? dz[i] : 0.f, u = dz[i] * g;
         w1 = fmaf(own, xh[i], w1);
         b1 += own;
-        s[i] = fmaf(dz[i], g, s[i]);
-        s[PTS + i] = fmaf(dz[i] * g, xh[i], s[PTS + i]);
+        s[i] += u;
+        s[PTS + i] = fmaf(u, xh[i], s[PTS + i]);
       }
-      if (KC > 0) {
-        aw[k] += w1;
-        ab[k] += b1;
-      } else {
+    };
+    // dx = rstd (u - s1 / C - xh s2 / C), from x: rstd u - (x - mean) rstd^2 s2 / C - rstd s1 / C
+    auto out = [&](size_t at_c, float g, const float (&v)[PTS], const float (&dz)[PTS]) {
+      float e[PTS];
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-          w1 += __shfl_xor(w1, o, 64);
-          b1 += __shfl_xor(b1, o, 64);
+      for (int i = 0; i < PTS; ++i) e[i] = fmaf(rs[i], dz[i] * g, fmaf(v[i] - mu[i], s[PTS + i], s[i]));
+      if (at.live) *reinterpret_cast<raw4<T>*>(rv::at32(po_ + at_c, o)) = shut<T>(e);
+    };
+    float v[PTS], d[PTS];
+    if (KC > 0) {
+#pragma unroll
+      for (int k = 0; k < KR; ++k) {
+        if (has[k]) {
+          open<T>(rx[k], v);
+          open<T>(rd[k], d);
+          one(gk[k], bk[k], v, d);
+          rd[k] = shut<T>(d);                          // dy with the ReLU's zeros: the same values, exact
+          add(gk[k], v, d, aw[k], ab[k]);
+          asm volatile("" : "+v"(aw[k]), "+v"(ab[k]));     // summed here: put off behind the barrier, the terms stay alive
+          forget<T>(rx[k]);
+          forget<T>(rd[k]);
+          __builtin_amdgcn_sched_barrier(0);         // one channel after the other
         }
-        if (px == 0) {                               // the one thread that adds to this channel's words
+      }
+    } else {
+      size_t at_c = 0;
+      for (int c = cy; c < C; c += CY, at_c += slots) {
+        float w1 = 0.f, b1 = 0.f;
+        open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(px_ + at_c, o)), v);
+        open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(pd_ + at_c, o)), d);
+        one(w ? w[c] : 1.f, b ? b[c] : 0.f, v, d);
+        add(w ? w[c] : 1.f, v, d, w1, b1);
+        w1 = rv::lanes_sum<16>(w1);
+        b1 = rv::lanes_sum<16>(b1);
+        if (px == 0) {                                 // the one thread that adds to this channel's words
           lacc[c] += w1;
           lacc[C + c] += b1;
         }
       }
-    });
+    }
     if (!dx) continue;
     slot_sum<2 * PTS>(s, buf[turn]);
 #pragma unroll
-    for (int i = 0; i < 2 * PTS; ++i) s[i] *= rc;
-    each([&](int, int c, const float (&xh)[PTS], const float (&dz)[PTS], float g) {
-      float o[PTS];
+    for (int i = 0; i < PTS; ++i) {
+      s[i] *= -rc * rs[i];
+      s[PTS + i] *= -rc * rs[i] * rs[i];
+    }
+    if (KC > 0) {
 #pragma unroll
-      for (int i = 0; i < PTS; ++i) o[i] = rs[i] * (dz[i] * g - s[i] - xh[i] * s[PTS + i]);
-      if (at.live) *reinterpret_cast<raw4<T>*>(dx + off + (size_t)c * M) = shut<T>(o);
-    });
+      for (int k = 0; k < KR; ++k) {
+        if (has[k]) {
+          open<T>(rx[k], v);
+          open<T>(rd[k], d);
+          out(k * slots, gk[k], v, d);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    } else {
+      size_t at_c = 0;
+      for (int c = cy; c < C; c += CY, at_c += slots) {
+        const float g = w ? w[c] : 1.f;
+        float t[PTS];
+        open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(px_ + at_c, o)), v);
+        open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(pd_ + at_c, o)), d);
+#pragma unroll
+        for (int i = 0; i < PTS; ++i) t[i] = v[i];
+        one(g, b ? b[c] : 0.f, t, d);
+        out(at_c, g, v, d);
+      }
+    }
   }
   if (!part) return;
   float* const pw = part + (size_t)blockIdx.x * 2 * C;
   if (KC > 0) {
 #pragma unroll
     for (int k = 0; k < KR; ++k) {
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        aw[k] += __shfl_xor(aw[k], o, 64);
-        ab[k] += __shfl_xor(ab[k], o, 64);
-      }
+      aw[k] = rv::lanes_sum<16>(aw[k]);
+      ab[k] = rv::lanes_sum<16>(ab[k]);
       const int c = cy + k * CY;
-      if (px == 0 && c < C) {
+      if (px == 0 && has[k]) {
         pw[c] = aw[k];
         pw[C + c] = ab[k];
       }
@@ -276,24 +335,45 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int B, int C,
   }
 }
 
-// threads and channels per thread: 16 slots up to 128 channels, then 8 channels a slot up to 512
+// threads and channels per thread: 16 slots up to 128 channels, then eight channels a slot while 64 slots do (8 x 196 x
+// 16384 in bf16, backward: 39.5 us; with six channels a slot and more slots 51.4, with four 52.9)
 void chan_shape(int C, int& threads, int& kc) {
   int cy = 16;
   if (C > 128) cy = (C + 31) / 32 * 4;
-  if (C > 512) cy = 64;
+  if (cy > 64) cy = 64;
   threads = cy * 16;
-  const int k = (C + cy - 1) / cy;
-  kc = k <= 1 ? 1 : k <= 2 ? 2 : k <= 4 ? 4 : k <= 8 ? 8 : 0;
+  kc = (C + cy - 1) / cy;
+  if (kc > 8) kc = 0;
 }
-int points4(int M) { return (int)(((long long)M + PTS - 1) / PTS); }
-long long chan_tiles(int B, int M) { return ((long long)B * points4(M) + 15) / 16; }
-int chan_grad_parts(int B, int M) {
-  const long long n = chan_tiles(B, M);
-  return (int)(n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
+int cloud_tiles(int M) { return (int)(((long long)M + 16 * PTS - 1) / (16 * PTS)); }
+long long chan_tiles(int B, int M) { return (long long)B * cloud_tiles(M); }
+// workgroups of a backward launch: what is on the chip at once (every one starts with the parameters and ends with its
+// partial sums): by its registers 32 waves a CU with two or three channels a thread, 16 with more (one: 16 are
+// the faster, 24 x 16 x 65536 fp32 61 us against 72)
+int chan_grad_parts(int B, int C, int M) {
+  int threads, kc;
+  chan_shape(C, threads, kc);
+  const long long n = chan_tiles(B, M), most = 256 * (long long)((kc == 2 || kc == 3 ? 2048 : 1024) / threads);
+  return (int)(n < most ? n : most);
 }
+constexpr int MAX_POINTS = 1 << 24;        // per cloud: 64 channel slots of them are within 32-bit byte offsets
 bool chan_ok(int dtype, int B, int C, int M) {
-  return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || M >= PTS) && (long long)B * points4(M) < 0x7fffff00LL;
+  return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || (M >= PTS && M <= MAX_POINTS)) &&
+         chan_tiles(B, M) < 0x7fffffffLL - 16384;
 }
+
+#define LN_CHAN_PICK(CALL)      \
+  switch (kc) {                 \
+    case 1: CALL(1); break;     \
+    case 2: CALL(2); break;     \
+    case 3: CALL(3); break;     \
+    case 4: CALL(4); break;     \
+    case 5: CALL(5); break;     \
+    case 6: CALL(6); break;     \
+    case 7: CALL(7); break;     \
+    case 8: CALL(8); break;     \
+    default: CALL(0); break;    \
+  }
 
 template <typename T>
 int chan_forward(int B, int C, int M, const void* x, const float* w, const float* b, float eps, int relu, void* y,
@@ -301,17 +381,11 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
   int threads, kc;
   chan_shape(C, threads, kc);
   const long long tiles = chan_tiles(B, M);
-  const dim3 grid((unsigned)(tiles < 16384 ? tiles : 16384));
-#define LN_CALL(KC)                                                                                              \
-  hipLaunchKernelGGL((ln_chan_kernel<T, KC>), grid, dim3(threads), 0, st, B, C, M, points4(M), (const T*)x, w, b, \
-                     eps, relu, (T*)y, mean, rstd)
-  switch (kc) {
-    case 1: LN_CALL(1); break;
-    case 2: LN_CALL(2); break;
-    case 4: LN_CALL(4); break;
-    case 8: LN_CALL(8); break;
-    default: LN_CALL(0); break;
-  }
+  const dim3 grid((unsigned)(tiles < 8192 ? tiles : 8192));
+#define LN_CALL(KC)                                                                                                       \
+  hipLaunchKernelGGL((ln_chan_kernel<T, KC>), grid, dim3(threads), 0, st, (int)tiles, cloud_tiles(M), C, M, (const T*)x, w, \
+                     b, eps, relu, (T*)y, mean, rstd)
+  LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
   return 0;
@@ -322,20 +396,15 @@ int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x,
                   const float* mean, const float* rstd, int relu, void* dx, float* part, hipStream_t st) {
   int threads, kc;
   chan_shape(C, threads, kc);
-#define LN_CALL(KC, LDS)                                                                                             \
-  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC>), dim3(parts), dim3(threads), LDS, st, B, C, M, points4(M),        \
-                     (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, part)
-  switch (kc) {
-    case 1: LN_CALL(1, 0); break;
-    case 2: LN_CALL(2, 0); break;
-    case 4: LN_CALL(4, 0); break;
-    case 8: LN_CALL(8, 0); break;
-    default: {
-      const int rc = pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0>);
-      if (rc) return rc;
-      LN_CALL(0, 2 * C * sizeof(float));
-    }
+  const int lds = kc ? 0 : (int)(2 * C * sizeof(float));
+  if (!kc) {
+    const int rc = pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0>);
+    if (rc) return rc;
   }
+#define LN_CALL(KC)                                                                                                      \
+  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC>), dim3(parts), dim3(threads), lds, st, (int)chan_tiles(B, M),          \
+                     cloud_tiles(M), C, M, (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, part)
+  LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
   return 0;
@@ -345,7 +414,7 @@ int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x,
 
 extern "C" size_t pvn3d_layer_norm_chan_grad_workspace_bytes(int dtype, int B, int C, int M) {
   if (!chan_ok(dtype, B, C, M)) return 0;
-  return (size_t)chan_grad_parts(B, M) * 2 * C * sizeof(float);
+  return (size_t)chan_grad_parts(B, C, M) * 2 * C * sizeof(float);
 }
 
 extern "C" int pvn3d_layer_norm_chan(int dtype, int B, int C, int M, const void* x, const float* weight, const float* bias,
@@ -377,7 +446,7 @@ extern "C" int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const 
     return 0;
   }
   if (!dy || !x || !mean || !rstd) return (int)hipErrorInvalidValue;
-  const int parts = chan_grad_parts(B, M);
+  const int parts = chan_grad_parts(B, C, M);
   if (dweight && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float))) return (int)hipErrorInvalidValue;
   float* part = dweight ? (float*)workspace : nullptr;
   int rc;

@@ -13,14 +13,14 @@ using ln::row_sum;
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
-__global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, long long dys,
-                                                           const T* __restrict__ x, long long xs,
-                                                           const signed char* __restrict__ codes, long long pitch,
+__global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
+                                                           const T* __restrict__ x, int xs,
+                                                           const signed char* __restrict__ codes, int pitch,
                                                            const unsigned char* __restrict__ scales,
                                                            const unsigned char* __restrict__ mask,
                                                            const float* __restrict__ w, const float* __restrict__ b,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                           int relu, T* __restrict__ dx, long long dxs, int dxcols,
+                                                           int relu, T* __restrict__ dx, int dxs, int dxcols,
                                                            float* __restrict__ part) {
   constexpr int VEC = traits<T>::VEC;
   constexpr int RPB = 256 / TPR;
@@ -43,62 +43,73 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
     }
   const float rc = 1.f / (float)C;
   for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)gridDim.x * (RPB * R)) {
-    float v[R][K][VEC], d[R][K][VEC], mu[R], rs[R];
-    unsigned cw[R][K][VEC / 4], bits[R][K];
-    float step[R][K], step0[R][K];
+    const int last = (int)(rows - 1 - base < RPB * R - 1 ? rows - 1 - base : RPB * R - 1);
+    const T* const db = dy + base * dys;
+    const T* const xb = x + base * xs;
+    T* const ob = dx + base * dxs;
+    const signed char* const cb = codes + base * pitch;
+    const unsigned char* const sb = scales + base * G;
+    const unsigned char* const mb = mask + base * MB;
+    rv::u4_any rx[R][K], rd[R][K];
+    float mu[R], rs[R];
+    unsigned cw[R][K][VEC / 4];
+    unsigned char sc[R][K][2], mk[R][K][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long at = base + r * RPB + rg, row = at < rows ? at : rows - 1;
-      mu[r] = mean[row];
-      rs[r] = rstd[row];
+      const int rl = min(rg + r * RPB, last);
+      mu[r] = *rv::at32(mean + base, rl * 4u);
+      rs[r] = *rv::at32(rstd + base, rl * 4u);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        col.load(dy + row * dys, k, C, d[r][k]);
+        rd[r][k] = col.load(db, __umul24(rl, dys), k, C);
         if (FROM8) {
           // a window that repeats values of its neighbour may start in the group before its own
           const int c = min(col.c[k], (C - 1) & ~(VEC - 1)), at = col.at[k];
-          rv::load_codes(codes + row * pitch + at, cw[r][k]);
-          step[r][k] = rv::group_step(scales[row * G + c / rv::GROUP]);
-          step0[r][k] = ragged ? rv::group_step(scales[row * G + at / rv::GROUP]) : step[r][k];
-          bits[r][k] = 0xffffffffu;
-          if (mask) {
-            bits[r][k] = mask[row * MB + at / 8];
-            if (ragged) bits[r][k] |= (unsigned)mask[row * MB + min(at / 8 + 1, MB - 1)] << 8;
-            bits[r][k] >>= at & 7;
-          }
+          const unsigned srow = __umul24(rl, G), mrow = __umul24(rl, MB);
+          rv::load_codes(rv::at32(cb, __umul24(rl, pitch) + at), cw[r][k]);
+          sc[r][k][0] = *rv::at32(sb, srow + c / rv::GROUP);
+          if (ragged) sc[r][k][1] = *rv::at32(sb, srow + at / rv::GROUP);
+          if (mask) mk[r][k][0] = *rv::at32(mb, mrow + at / 8);
+          if (mask && ragged) mk[r][k][1] = *rv::at32(mb, mrow + min(at / 8 + 1, MB - 1));
         } else {
-          col.load(x + row * xs, k, C, v[r][k]);
+          rx[r][k] = col.load(xb, __umul24(rl, xs), k, C);
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);       // all loads on their way before anything waits for one
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = base + r * RPB + rg;
-      const bool live = row < rows;
-      float s1 = 0.f, s2 = 0.f;
+      const int rl = rg + r * RPB;
+      const bool live = rl <= last;
+      float v[K][VEC], d[K][VEC], s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const float a = FROM8 ? step[r][k] : 0.f, a0 = FROM8 ? step0[r][k] : 0.f;
+        traits<T>::unpack(rd[r][k], d[k]);
+        if (!FROM8) traits<T>::unpack(rx[r][k], v[k]);
+        const float a = FROM8 ? rv::group_step(sc[r][k][0]) : 0.f, a0 = FROM8 && ragged ? rv::group_step(sc[r][k][1]) : a;
+        unsigned bits = 0xffffffffu;
+        if (FROM8 && mask) bits = ((unsigned)mk[r][k][0] | (ragged ? (unsigned)mk[r][k][1] << 8 : 0u)) >> (col.at[k] & 7);
+        if (FROM8 && !live) bits = 0u;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float xm = FROM8 ? fmaf(rv::code_at(cw[r][k], i), i < col.skip[k] ? a0 : a, -mu[r]) : v[r][k][i] - mu[r];
+          const float xm = FROM8 ? fmaf(rv::code_at(cw[r][k], i), i < col.skip[k] ? a0 : a, -mu[r]) : v[k][i] - mu[r];
           const float xh = xm * rs[r];
           float dz;
           if (FROM8) {
             // bit i as a mask of the whole word
-            const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)(live ? bits[r][k] : 0u), i, 1);
-            dz = __uint_as_float(__float_as_uint(d[r][k][i]) & on);
+            const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)bits, i, 1);
+            dz = __uint_as_float(__float_as_uint(d[k][i]) & on);
           } else {
             const bool off_ = relu && fmaf(xh, g[k][i], be[k][i]) <= 0.f;          // (a NaN passes, as in the forward)
-            dz = live && !off_ ? d[r][k][i] : 0.f;
+            dz = live && !off_ ? d[k][i] : 0.f;
           }
           aw[k][i] = fmaf(dz, xh, aw[k][i]);
           ab[k][i] += dz;
           const float u = dz * g[k][i], um = u * col.own[k][i];
           s1 += um;
           s2 = fmaf(um, xh, s2);
-          d[r][k][i] = u;
-          v[r][k][i] = xh;
+          d[k][i] = u;
+          v[k][i] = xh;
         }
       }
       if (dx) {
@@ -108,11 +119,13 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
         for (int k = 0; k < K; ++k) {
           float o[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] = rs[r] * (d[r][k][i] - s1 - v[r][k][i] * s2);
-          if (live) col.store(dx + row * dxs, k, C, o);
+          for (int i = 0; i < VEC; ++i) o[i] = rs[r] * (d[k][i] - s1 - v[k][i] * s2);
+          if (live) col.store(ob, __umul24(rl, dxs), k, C, o);
         }
         if (dxcols > C && live)
-          for (int c = C + t; c < dxcols; c += TPR) traits<T>::store1(dx + row * dxs + c, 0.f);
+#pragma unroll 1
+          for (int c = C + t; c < dxcols; c += TPR)
+            traits<T>::store1(rv::at32(ob, (__umul24(rl, dxs) + c) * (unsigned)sizeof(T)), 0.f);
       }
     }
   }
@@ -170,14 +183,14 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
   do {                                                                                                                   \
     if (codes)                                                                                                           \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, true>), dim3(parts), dim3(256), 0, st, rows, C,              \
-                         (const T*)dy, dys, (const T*)nullptr, 0ll, (const signed char*)codes, pitch,                    \
-                         (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, dxs,  \
+                         (const T*)dy, (int)dys, (const T*)nullptr, 0, (const signed char*)codes, (int)pitch,                    \
+                         (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, (int)dxs,  \
                          dxcols, part);                                                                                  \
     else                                                                                                                 \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, false>), dim3(parts), dim3(256), 0, st, rows, C,             \
-                         (const T*)dy, dys, (const T*)x, xs, (const signed char*)nullptr, 0ll,                           \
+                         (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)nullptr, 0,                           \
                          (const unsigned char*)nullptr, (const unsigned char*)nullptr, w, b, mean, rstd, relu, (T*)dx,   \
-                         dxs, dxcols, part);                                                                             \
+                         (int)dxs, dxcols, part);                                                                             \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
@@ -197,6 +210,8 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
                                      const float* rstd, int relu, void* dx, long long dxs, int dx_cols, float* dweight,
                                      float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype < 0 || dtype > 2 || C <= 0 || C > ln::MAX_C || dys < 0 || xs < 0) return (int)hipErrorInvalidValue;
+  if (dys > ln::MAX_STRIDE || xs > ln::MAX_STRIDE || dxs > ln::MAX_STRIDE || pitch > ln::MAX_STRIDE)
+    return (int)hipErrorInvalidValue;
   if (dx && (dx_cols < C || dx_cols > C + 15 || dxs < dx_cols)) return (int)hipErrorInvalidValue;
   if ((dweight == nullptr) != (dbias == nullptr) || (!dx && !dweight)) return (int)hipErrorInvalidValue;
   if (codes && (!scales || (pitch & 15) || pitch < C || (relu != 0) != (mask != nullptr))) return (int)hipErrorInvalidValue;

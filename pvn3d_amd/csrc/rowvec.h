@@ -80,6 +80,12 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[tr
   *reinterpret_cast<u4_any*>(p) = traits<T>::pack(v);
 }
 
+// base + offset in bytes, base the same for the whole wave: one 32-bit register per lane for the address
+template <typename P>
+__device__ __forceinline__ P* at32(P* base, unsigned bytes) {
+  return (P*)((const char*)base + bytes);        // (pointer arithmetic: through an integer the access would be a flat one)
+}
+
 // A lane's chunk of a row of C >= VEC values: whole chunks start at c, a multiple of VEC; the last, partial one is taken as
 // the row's last VEC values instead -- it overlaps its neighbour by `skip` values, which this lane computes a second time
 // (the same bits) and leaves out of every sum.  So all loads and stores are whole and unconditional: a guarded load is a
@@ -126,12 +132,12 @@ __device__ __forceinline__ void group_codes(const float (&v)[VEC], unsigned scal
     w[q] = __builtin_amdgcn_perm(t[4 * q + 1], t[4 * q], 0x0c0c0400u) | __builtin_amdgcn_perm(t[4 * q + 3], t[4 * q + 2], 0x04000c0cu);
 }
 // a window's codes to their place: the values it skips are a neighbour's
-__device__ __forceinline__ void store_codes(signed char* __restrict__ row, int c, int skip, const unsigned (&w)[2]) {
+__device__ __forceinline__ void store_codes(signed char* __restrict__ p, int skip, const unsigned (&w)[2]) {
   const unsigned long long b = (((unsigned long long)w[1] << 32) | w[0]) >> (8 * (skip & 7));
-  *reinterpret_cast<uint2*>(row + c) = make_uint2((unsigned)b, (unsigned)(b >> 32));
+  *reinterpret_cast<uint2*>(p) = make_uint2((unsigned)b, (unsigned)(b >> 32));
 }
-__device__ __forceinline__ void store_codes(signed char* __restrict__ row, int c, int skip, const unsigned (&w)[1]) {
-  *reinterpret_cast<unsigned*>(row + c) = w[0] >> (8 * (skip & 3));
+__device__ __forceinline__ void store_codes(signed char* __restrict__ p, int skip, const unsigned (&w)[1]) {
+  *reinterpret_cast<unsigned*>(p) = w[0] >> (8 * (skip & 3));
 }
 // the codes of a window, at any alignment
 struct __attribute__((packed, aligned(1))) u2_byte { unsigned x, y; };

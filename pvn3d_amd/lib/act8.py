@@ -28,11 +28,14 @@ def _need(ok, what):
         raise RuntimeError(what)
 
 
-def _rows(t, name):
+MAX_STRIDE = 1 << 20        # row strides (in elements) that the kernels take; wider ones are copied
+
+
+def _rows(t):
     """(..., C) -> (2-D view or copy whose channels are contiguous, its row stride)."""
     C = t.size(-1)
-    m = t if t.dim() == 2 else t.reshape(-1, C) if C else t.reshape(0, 0)
-    if m.stride(1) != 1 and C > 1:
+    m = t if t.dim() == 2 else t.reshape(-1, C)
+    if (m.stride(1) != 1 and C > 1) or m.stride(0) > MAX_STRIDE:
         m = m.contiguous()
     return m, (m.stride(0) if m.size(0) > 1 else C)
 
@@ -88,7 +91,7 @@ def act8_pack(x):
     _need(x.dtype in DTYPES, "x must be a float32, bfloat16 or float16 tensor")
     _need(x.dim() >= 1 and x.size(-1) > 0, "x must have at least one channel")
     with on_device(x.device):
-        m, xs = _rows(x, "x")
+        m, xs = _rows(x)
         act = _empty_act8(m.size(0), m.size(1), x.shape, x.device)
         check(lib.pvn3d_act8_pack(DTYPES[x.dtype], m.size(0), m.size(1), m.data_ptr(), xs, act.codes.data_ptr(), act.pitch,
                                   act.scales.data_ptr(), _stream(x)), "act8_pack")
@@ -121,7 +124,7 @@ def linear8_weight_grad(dy, act):
     M = dy.size(-1)
     _need(dy.numel() == rows * M, "dy and act must have the same number of rows")
     with on_device(dy.device):
-        m, ds = _rows(dy, "dy")
+        m, ds = _rows(dy)
         dw = torch.empty((M, N), dtype=torch.float32, device=dy.device)
         wsb = lib.pvn3d_act8_wgrad_workspace_bytes(rows, M, N)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
@@ -166,7 +169,7 @@ class _Linear8(torch.autograd.Function):
     def forward(ctx, x, weight):
         N, C = weight.shape
         with on_device(x.device):
-            m, _ = _rows(x, "x")
+            m, _ = _rows(x)
             w = weight.detach().contiguous()
             y = _product(m, C, w, False)
             ctx.act = None
@@ -184,7 +187,7 @@ class _Linear8(torch.autograd.Function):
         dx = dw = None
         dy = dy.to(torch.bfloat16)
         with on_device(dy.device):
-            m, _ = _rows(dy, "dy")
+            m, _ = _rows(dy)
             if ctx.needs_input_grad[0]:
                 dx = _product(m, N, weight.detach().contiguous(), True).reshape(ctx.lead + (C,))
             if ctx.needs_input_grad[1]:

@@ -75,7 +75,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
         stat = torch.empty((2, n), dtype=torch.float32, device=dev)
         mean, rstd = stat[0], stat[1]
         if rows:
-            m, xs = _rows(v, "x")
+            m, xs = _rows(v)
             check(lib.pvn3d_layer_norm(DTYPES[v.dtype], n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), float(eps),
                                        1 if relu else 0, y.data_ptr(), C, C, mean.data_ptr(), rstd.data_ptr(), None, 0,
                                        None, None, _stream(x)), "layer_norm")
@@ -117,7 +117,7 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=Fa
         pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
         if rows:
             d = dy if v is x else dy.movedim(1, -1)
-            (m, xs), (g, gs) = _rows(v, "x"), _rows(d, "dy")
+            (m, xs), (g, gs) = _rows(v), _rows(d)
             wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
             ws = _workspace(wsb, dev)
             check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, m.data_ptr(), xs, None, 0, None, None, _ptr(w),
@@ -162,7 +162,7 @@ def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
     dev = x.device
     with on_device(dev):
-        m, xs = _rows(x, "x")
+        m, xs = _rows(x)
         n = m.size(0)
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         stat = torch.empty((2, n), dtype=torch.float32, device=dev)
@@ -186,7 +186,7 @@ def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True
     w = _param(weight, C, dy, "weight")
     dev, t = dy.device, DTYPES[dy.dtype]
     with on_device(dev):
-        g, gs = _rows(dy, "dy")
+        g, gs = _rows(dy)
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev) if need_dx else None
         dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
         wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
