@@ -19,8 +19,11 @@ GROUP = 32
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream       # torch.cuda.current_stream() builds a Stream object: 1.9 us a call
+
+
 def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
 
 
 def _need(ok, what):
@@ -40,61 +43,99 @@ def _rows(t):
     return m, (m.stride(0) if m.size(0) > 1 else C)
 
 
+def _like(m, shape):
+    """An uninitialised contiguous tensor of m's type and this shape."""
+    return torch.empty_like(m) if m.shape == shape and m.is_contiguous() else m.new_empty(shape)
+
+
+def _align16(n):
+    return (n + 15) & ~15
+
+
 class Act8(object):
     """A tensor (..., C) in the 8-bit form: `codes` int8 (rows, C), rows 16-byte aligned (pitch a multiple of 16, whole
     16-byte chunks in its storage), `scales` uint8 (rows, ceil(C / 32)) contiguous, `shape` of the tensor."""
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("_codes", "_scales", "_buf", "_at", "rows", "channels", "pitch", "shape", "device")
 
     def __init__(self, codes, scales, shape=None):
         _need(codes.dim() == 2 and codes.dtype == torch.int8, "codes must be an int8 matrix")
         rows, C = codes.shape
         _need(C > 0, "codes must have at least one channel")
-        _need(scales.dtype == torch.uint8 and tuple(scales.shape) == (rows, (C + GROUP - 1) // GROUP)
+        _need(scales.dtype == torch.uint8 and scales.shape == (rows, (C + GROUP - 1) // GROUP)
               and scales.is_contiguous(), "scales must be a contiguous uint8 (rows, ceil(channels / 32)) matrix")
         _need(codes.is_cuda and scales.is_cuda, "CPU not supported")
         _need(scales.device == codes.device, "scales must be on the codes' device")
         if rows > 0:
             _need((codes.stride(1) == 1 or C == 1) and codes.data_ptr() % 16 == 0, "codes must have 16-byte aligned rows")
             if rows > 1:
-                _need(codes.stride(0) % 16 == 0 and codes.stride(0) >= C, "codes must have 16-byte aligned rows")
-            last = codes.storage_offset() + (rows - 1) * codes.stride(0) + (C + 15) // 16 * 16
+                _need(codes.stride(0) % 16 == 0 and C <= codes.stride(0) <= MAX_STRIDE, "codes must have 16-byte aligned rows")
+            last = codes.storage_offset() + (rows - 1) * codes.stride(0) + _align16(C)
             _need(codes.untyped_storage().nbytes() >= last, "codes must end with a whole 16-byte chunk")
         if shape is not None:
             n = 1
             for v in shape[:-1]:
                 n *= v
             _need(len(shape) > 0 and shape[-1] == C and n == rows, "shape does not fit the codes")
-        self.codes, self.scales = codes, scales
+        self._codes, self._scales, self._buf, self._at = codes, scales, None, 0
+        self.rows, self.channels = rows, C
+        self.pitch = codes.stride(0) if rows > 1 else _align16(C)
         self.shape = torch.Size(shape) if shape is not None else codes.shape
+        self.device = codes.device
+
+    @staticmethod
+    def _in(buf, at, rows, C, shape):
+        """The codes from byte `at` (a multiple of 16) of a uint8 buffer on, the scales behind them; views of it are made
+        when they are asked for."""
+        act = object.__new__(Act8)
+        act._codes = act._scales = None
+        act._buf, act._at, act.rows, act.channels, act.pitch, act.shape = buf, at, rows, C, _align16(C), shape
+        act.device = buf.device
+        return act
+
+    @staticmethod
+    def _bytes(rows, C):
+        return rows * (_align16(C) + (C + GROUP - 1) // GROUP)
 
     @property
-    def pitch(self):
-        return self.codes.stride(0) if self.codes.size(0) > 1 else (self.codes.size(1) + 15) // 16 * 16
+    def codes(self):
+        if self._codes is None:
+            n = self.rows * self.pitch
+            self._codes = self._buf[self._at:self._at + n].view(torch.int8).view(self.rows, self.pitch)[:, :self.channels]
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            at, G = self._at + self.rows * self.pitch, (self.channels + GROUP - 1) // GROUP
+            self._scales = self._buf[at:at + self.rows * G].view(self.rows, G)
+        return self._scales
+
+    def _ptrs(self):
+        if self._buf is not None:
+            p = self._buf.data_ptr() + self._at
+            return p, p + self.rows * self.pitch
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     @property
     def nbytes(self):
-        return self.codes.size(0) * self.pitch + self.scales.numel()
+        return self.rows * (self.pitch + (self.channels + GROUP - 1) // GROUP)
 
     def unpack(self, dtype=torch.bfloat16):
         return act8_unpack(self, dtype)
 
 
-def _empty_act8(rows, C, shape, dev):
-    codes = torch.empty((rows, (C + 15) // 16 * 16), dtype=torch.int8, device=dev)[:, :C]
-    scales = torch.empty((rows, (C + GROUP - 1) // GROUP), dtype=torch.uint8, device=dev)
-    return Act8(codes, scales, shape)
-
-
 def act8_pack(x):
     """x (..., C) float32 / bfloat16 / float16 -> Act8."""
     _need(x.is_cuda, "CPU not supported")
-    _need(x.dtype in DTYPES, "x must be a float32, bfloat16 or float16 tensor")
+    t = DTYPES.get(x.dtype)
+    _need(t is not None, "x must be a float32, bfloat16 or float16 tensor")
     _need(x.dim() >= 1 and x.size(-1) > 0, "x must have at least one channel")
     with on_device(x.device):
         m, xs = _rows(x)
-        act = _empty_act8(m.size(0), m.size(1), x.shape, x.device)
-        check(lib.pvn3d_act8_pack(DTYPES[x.dtype], m.size(0), m.size(1), m.data_ptr(), xs, act.codes.data_ptr(), act.pitch,
-                                  act.scales.data_ptr(), _stream(x)), "act8_pack")
+        rows, C = m.shape
+        act = Act8._in(torch.empty(Act8._bytes(rows, C), dtype=torch.uint8, device=x.device), 0, rows, C, x.shape)
+        codes, scales = act._ptrs()
+        check(lib.pvn3d_act8_pack(t, rows, C, m.data_ptr(), xs, codes, act.pitch, scales, _stream(x)), "act8_pack")
     return act
 
 
@@ -102,13 +143,14 @@ def act8_unpack(act, dtype=torch.bfloat16):
     """Act8 -> the held values, a contiguous tensor of its shape.  bfloat16 and float32 hold every value exactly; float16
     does if the tensor was a float16 one (otherwise values are rounded, and overflow to infinity)."""
     _need(isinstance(act, Act8), "act must be an Act8")
-    _need(dtype in DTYPES, "dtype must be float32, bfloat16 or float16")
-    rows, C = act.codes.shape
-    dev = act.codes.device
+    t = DTYPES.get(dtype)
+    _need(t is not None, "dtype must be float32, bfloat16 or float16")
+    dev = act.device
     with on_device(dev):
         out = torch.empty(act.shape, dtype=dtype, device=dev)
-        check(lib.pvn3d_act8_unpack(DTYPES[dtype], rows, C, act.codes.data_ptr(), act.pitch, act.scales.data_ptr(),
-                                    out.data_ptr(), C, C, _stream(act.codes)), "act8_unpack")
+        codes, scales = act._ptrs()
+        check(lib.pvn3d_act8_unpack(t, act.rows, act.channels, codes, act.pitch, scales, out.data_ptr(), act.channels,
+                                    act.channels, _stream(out)), "act8_unpack")
     return out
 
 
@@ -118,18 +160,18 @@ def linear8_weight_grad(dy, act):
     _need(dy.is_cuda, "CPU not supported")
     _need(dy.dtype == torch.bfloat16, "dy must be a bfloat16 tensor")
     _need(isinstance(act, Act8), "act must be an Act8")
-    _need(act.codes.device == dy.device, "act must be on dy's device")
+    _need(act.device == dy.device, "act must be on dy's device")
     _need(dy.dim() >= 1 and dy.size(-1) > 0, "dy must have at least one channel")
-    rows, N = act.codes.shape
-    M = dy.size(-1)
+    rows, N, M = act.rows, act.channels, dy.size(-1)
     _need(dy.numel() == rows * M, "dy and act must have the same number of rows")
     with on_device(dy.device):
         m, ds = _rows(dy)
         dw = torch.empty((M, N), dtype=torch.float32, device=dy.device)
         wsb = lib.pvn3d_act8_wgrad_workspace_bytes(rows, M, N)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
-        check(lib.pvn3d_act8_wgrad(rows, M, N, m.data_ptr(), ds, act.codes.data_ptr(), act.pitch, act.scales.data_ptr(),
-                                   dw.data_ptr(), ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_wgrad")
+        codes, scales = act._ptrs()
+        check(lib.pvn3d_act8_wgrad(rows, M, N, m.data_ptr(), ds, codes, act.pitch, scales, dw.data_ptr(),
+                                   ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_wgrad")
     return dw
 
 

@@ -18,7 +18,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .._lib import lib, check, on_device
-from .act8 import Act8, DTYPES, _empty_act8, _need, _rows, _stream
+from .act8 import Act8, DTYPES, _like, _need, _rows, _stream
 
 MAX_CHANNELS = 8192
 
@@ -26,9 +26,9 @@ MAX_CHANNELS = 8192
 def _param(p, C, x, name):
     if p is None:
         return None
-    _need(p.dtype == torch.float32 and tuple(p.shape) == (C,), "%s must be a float32 tensor of the channels' length" % name)
+    _need(p.dtype is torch.float32 and p.shape == (C,), "%s must be a float32 tensor of the channels' length" % name)
     _need(p.device == x.device, "%s must be on x's device" % name)
-    return p.contiguous()
+    return p if p.is_contiguous() else p.contiguous()
 
 
 def _ptr(t):
@@ -37,7 +37,9 @@ def _ptr(t):
 
 def _check_x(x, name="x"):
     _need(x.is_cuda, "CPU not supported")
-    _need(x.dtype in DTYPES, "%s must be a float32, bfloat16 or float16 tensor" % name)
+    t = DTYPES.get(x.dtype)
+    _need(t is not None, "%s must be a float32, bfloat16 or float16 tensor" % name)
+    return t
 
 
 def _by_rows(x, channel_dim):
@@ -57,51 +59,52 @@ def _by_rows(x, channel_dim):
     return rows, x
 
 
-def _like(y, x):
-    """A channels-second result in x's layout: channel-major if x is, else the point-major view it is."""
+def _second(y, x):
+    """A channels-last result with its channels second, in x's layout: channel-major if x is, else the view it is."""
+    y = y.movedim(-1, 1)
     return y.contiguous() if x.is_contiguous() else y
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False):
     """-> (y like x, mean, rstd): the statistics are float32, one value per point in the points' order."""
-    _check_x(x)
+    t = _check_x(x)
     rows, v = _by_rows(x, channel_dim)
     C = v.size(-1) if rows else v.size(1)
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
-    dev = x.device
-    with on_device(dev):
+    with on_device(x.device):
         n = v.numel() // C
-        y = torch.empty(v.shape, dtype=v.dtype, device=dev)
-        stat = torch.empty((2, n), dtype=torch.float32, device=dev)
-        mean, rstd = stat[0], stat[1]
+        y = _like(v, v.shape)
+        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
         if rows:
             m, xs = _rows(v)
-            check(lib.pvn3d_layer_norm(DTYPES[v.dtype], n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), float(eps),
-                                       1 if relu else 0, y.data_ptr(), C, C, mean.data_ptr(), rstd.data_ptr(), None, 0,
-                                       None, None, _stream(x)), "layer_norm")
+            check(lib.pvn3d_layer_norm(t, n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), eps, 1 if relu else 0, y.data_ptr(), C, C,
+                                       mean.data_ptr(), rstd.data_ptr(), None, 0, None, None, _stream(x)), "layer_norm")
             if v is not x:
-                y = _like(y.movedim(-1, 1), x)
+                y = _second(y, x)
         else:
-            check(lib.pvn3d_layer_norm_chan(DTYPES[v.dtype], v.size(0), C, n // max(v.size(0), 1), v.data_ptr(), _ptr(w),
-                                            _ptr(b), float(eps), 1 if relu else 0, y.data_ptr(), mean.data_ptr(),
-                                            rstd.data_ptr(), _stream(x)), "layer_norm_chan")
+            check(lib.pvn3d_layer_norm_chan(t, v.size(0), C, n // max(v.size(0), 1), v.data_ptr(), _ptr(w), _ptr(b), eps,
+                                            1 if relu else 0, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(x)),
+                  "layer_norm_chan")
     return y, mean, rstd
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _grad_buffers(C, wsb, dev):
+    """dweight, dbias and the workspace of their partial sums."""
+    dw, db = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    return dw, db, ws, dw.data_ptr(), db.data_ptr(), _ptr(ws)
 
 
 def _check_stats(mean, rstd, n, x):
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous() and t.device == x.device,
+        _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.device == x.device,
               "%s must be a contiguous float32 tensor with one value per point" % name)
 
 
 def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=False, need_dx=True, need_dparams=True):
     """-> (dx like x or None, dweight (C,), dbias (C,) float32 or None, None).  mean, rstd: the forward's; relu: the
     derivative is taken where weight xh + bias > 0."""
-    _check_x(x)
+    t = _check_x(x)
     _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device, "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
     rows, v = _by_rows(x, channel_dim)
@@ -109,54 +112,75 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=Fa
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
     n = v.numel() // C
     _check_stats(mean, rstd, n, x)
-    dev, t = x.device, DTYPES[v.dtype]
+    dev = x.device
+    dx = dw = db = ws = pw = pb = pws = None
+    wsb = 0
     with on_device(dev):
-        st = _stream(x)
-        dx = torch.empty(v.shape, dtype=v.dtype, device=dev) if need_dx else None
-        dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
-        pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
+        if need_dx:
+            dx = _like(v, v.shape)
         if rows:
             d = dy if v is x else dy.movedim(1, -1)
             (m, xs), (g, gs) = _rows(v), _rows(d)
-            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
-            ws = _workspace(wsb, dev)
+            if need_dparams:
+                wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C)
+                dw, db, ws, pw, pb, pws = _grad_buffers(C, wsb, dev)
             check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, m.data_ptr(), xs, None, 0, None, None, _ptr(w),
                                             _ptr(b), mean.data_ptr(), rstd.data_ptr(), 1 if relu else 0, _ptr(dx), C, C,
-                                            pw, pb, _ptr(ws), wsb, st), "layer_norm_grad")
+                                            pw, pb, pws, wsb, _stream(x)), "layer_norm_grad")
             if need_dx and v is not x:
-                dx = _like(dx.movedim(-1, 1), x)
+                dx = _second(dx, x)
         else:
             g = dy.contiguous()
             B = v.size(0)
-            wsb = lib.pvn3d_layer_norm_chan_grad_workspace_bytes(t, B, C, n // max(B, 1)) if need_dparams else 0
-            ws = _workspace(wsb, dev)
-            check(lib.pvn3d_layer_norm_chan_grad(t, B, C, n // max(B, 1), g.data_ptr(), v.data_ptr(), _ptr(w), _ptr(b),
-                                                 mean.data_ptr(), rstd.data_ptr(), 1 if relu else 0, _ptr(dx), pw, pb,
-                                                 _ptr(ws), wsb, st), "layer_norm_chan_grad")
-    return (dx, dp[0], dp[1]) if need_dparams else (dx, None, None)
+            M = n // max(B, 1)
+            if need_dparams:
+                wsb = lib.pvn3d_layer_norm_chan_grad_workspace_bytes(t, B, C, M)
+                dw, db, ws, pw, pb, pws = _grad_buffers(C, wsb, dev)
+            check(lib.pvn3d_layer_norm_chan_grad(t, B, C, M, g.data_ptr(), v.data_ptr(), _ptr(w), _ptr(b), mean.data_ptr(),
+                                                 rstd.data_ptr(), 1 if relu else 0, _ptr(dx), pw, pb, pws, wsb, _stream(x)),
+                  "layer_norm_chan_grad")
+    return dx, dw, db
 
 
 class Saved8(object):
-    """What layer_norm_forward8 keeps for the backward pass: x in 8 bits, the statistics, and with a ReLU one bit per
-    value (mask (rows, ceil(C / 8)) uint8, bit i of byte j: channel 8 j + i is on)."""
-    __slots__ = ("act", "mask", "mean", "rstd", "dtype")
+    """What layer_norm_forward8 keeps for the backward pass: x in 8 bits (`act`), the statistics `mean` and `rstd`, and with
+    a ReLU one bit per value, `mask` (rows, ceil(C / 8)) uint8: bit i of byte j: channel 8 j + i is on.  One buffer: codes,
+    scales, mask, statistics; views of it are made when they are asked for."""
+    __slots__ = ("act", "dtype", "relu", "_buf", "_mask", "_stat")
 
-    def __init__(self, act, mask, mean, rstd, dtype):
-        rows, C = act.codes.shape
-        if mask is not None:
-            _need(mask.dtype == torch.uint8 and tuple(mask.shape) == (rows, (C + 7) // 8) and mask.is_contiguous()
-                  and mask.device == act.codes.device, "mask must be a contiguous uint8 (rows, ceil(channels / 8)) matrix")
-        _check_stats(mean, rstd, rows, act.codes)
-        self.act, self.mask, self.mean, self.rstd, self.dtype = act, mask, mean, rstd, dtype
+    def __init__(self, rows, C, shape, dtype, relu, dev):
+        mask = (Act8._bytes(rows, C) + 3) & ~3
+        stat = (mask + (rows * ((C + 7) // 8) if relu else 0) + 3) & ~3
+        self._buf = torch.empty(stat + 8 * rows, dtype=torch.uint8, device=dev)
+        self._mask, self._stat, self.dtype, self.relu = mask, stat, dtype, relu
+        self.act = Act8._in(self._buf, 0, rows, C, shape)
+
+    def _ptrs(self):
+        p = self._buf.data_ptr()
+        return p + self._stat, p + self._stat + 4 * self.act.rows, p + self._mask if self.relu else None
+
+    @property
+    def mask(self):
+        a = self.act
+        n = (a.channels + 7) // 8
+        return self._buf[self._mask:self._mask + a.rows * n].view(a.rows, n) if self.relu else None
+
+    @property
+    def mean(self):
+        return self._buf[self._stat:self._stat + 4 * self.act.rows].view(torch.float32)
+
+    @property
+    def rstd(self):
+        return self._buf[self._stat + 4 * self.act.rows:].view(torch.float32)
 
     @property
     def nbytes(self):
-        return self.act.nbytes + (self.mask.numel() if self.mask is not None else 0) + 8 * self.mean.numel()
+        return self._buf.numel()
 
 
 def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
     """x (..., C) -> (y like x, Saved8).  y is layer_norm_forward's, bit for bit."""
-    _check_x(x)
+    t = _check_x(x)
     _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
     C = x.size(-1)
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
@@ -164,39 +188,38 @@ def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
     with on_device(dev):
         m, xs = _rows(x)
         n = m.size(0)
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        stat = torch.empty((2, n), dtype=torch.float32, device=dev)
-        act = _empty_act8(n, C, x.shape, dev)
-        mask = torch.empty((n, (C + 7) // 8), dtype=torch.uint8, device=dev) if relu else None
-        check(lib.pvn3d_layer_norm(DTYPES[x.dtype], n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), float(eps), 1 if relu else 0,
-                                   y.data_ptr(), C, C, stat[0].data_ptr(), stat[1].data_ptr(), act.codes.data_ptr(),
-                                   act.pitch, act.scales.data_ptr(), _ptr(mask), _stream(x)), "layer_norm")
-        saved = Saved8(act, mask, stat[0], stat[1], x.dtype)
+        y = _like(x, x.shape)
+        saved = Saved8(n, C, x.shape, x.dtype, bool(relu), dev)
+        (codes, scales), (mean, rstd, mask) = saved.act._ptrs(), saved._ptrs()
+        check(lib.pvn3d_layer_norm(t, n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), eps, 1 if relu else 0, y.data_ptr(), C, C,
+                                   mean, rstd, codes, saved.act.pitch, scales, mask, _stream(x)), "layer_norm")
     return y, saved
 
 
 def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True):
     """layer_norm_backward with xh = (held x - mean) rstd from the 8-bit form and the ReLU from its bits."""
     _need(isinstance(saved, Saved8), "saved must be what layer_norm_forward8 returned")
-    _check_x(dy, "dy")
+    t = _check_x(dy, "dy")
     act = saved.act
-    _need(dy.shape == act.shape and dy.dtype == saved.dtype and dy.device == act.codes.device, "dy must be like x")
+    _need(dy.shape == act.shape and dy.dtype == saved.dtype and dy.device == act.device, "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
-    n, C = act.codes.shape
+    n, C = act.rows, act.channels
     w = _param(weight, C, dy, "weight")
-    dev, t = dy.device, DTYPES[dy.dtype]
+    dev = dy.device
+    dx = dw = db = ws = pw = pb = pws = None
+    wsb = 0
     with on_device(dev):
         g, gs = _rows(dy)
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev) if need_dx else None
-        dp = torch.empty((2, C), dtype=torch.float32, device=dev) if need_dparams else None
-        wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C) if need_dparams else 0
-        ws = _workspace(wsb, dev)
-        pw, pb = (dp[0].data_ptr(), dp[1].data_ptr()) if need_dparams else (None, None)
-        check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, None, 0, act.codes.data_ptr(), act.pitch,
-                                        act.scales.data_ptr(), _ptr(saved.mask), _ptr(w), None, saved.mean.data_ptr(),
-                                        saved.rstd.data_ptr(), 1 if saved.mask is not None else 0, _ptr(dx), C, C, pw, pb,
-                                        _ptr(ws), wsb, _stream(dy)), "layer_norm_grad")
-    return (dx, dp[0], dp[1]) if need_dparams else (dx, None, None)
+        if need_dx:
+            dx = _like(dy, dy.shape)
+        if need_dparams:
+            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C)
+            dw, db, ws, pw, pb, pws = _grad_buffers(C, wsb, dev)
+        (codes, scales), (mean, rstd, mask) = act._ptrs(), saved._ptrs()
+        check(lib.pvn3d_layer_norm_grad(t, n, C, g.data_ptr(), gs, None, 0, codes, act.pitch, scales, mask, _ptr(w), None,
+                                        mean, rstd, 1 if saved.relu else 0, _ptr(dx), C, C, pw, pb, pws, wsb, _stream(dy)),
+              "layer_norm_grad")
+    return dx, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
