@@ -669,7 +669,7 @@ int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const void* dy, c
  * with a whole 16-byte chunk too), scales [rows][ceil(C / 32)].  Codes behind C are not read as values.
  * pvn3d_act8_unpack writes the held values (exact in fp32 and bf16), zeros in columns C .. y_cols - 1.
  * pvn3d_act8_wgrad: dW [M][N] fp32 = dY^T X, dY bf16 [rows] of stride dys (M columns), X = the held values [rows][N], on
- * v_mfma_f32_32x32x16_bf16; fixed order of the sums.  No rows: zeros. */
+ * v_mfma_f32_32x32x16_bf16; fixed order of the sums; strides up to 2^20.  No rows: zeros. */
 int pvn3d_act8_pack(int dtype, long long rows, int C, const void* x, long long xs, void* codes, long long pitch, void* scales,
                     void* stream);
 int pvn3d_act8_unpack(int dtype, long long rows, int C, const void* codes, long long pitch, const void* scales, void* y,

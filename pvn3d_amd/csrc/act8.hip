@@ -86,13 +86,13 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C,
 
 // ------------------------------------------------------------------------------------------------ weight gradient
 // dW[m][n] = sum over rows r of dY[r][m] X[r][n].  Rows are the contraction and both operands hold them as their slow
-// dimension; a matrix instruction wants eight of them per lane.  A step of 32 rows is staged in LDS as it lies in memory (X
+// dimension; a matrix instruction wants eight of them per lane.  A step of 32 or 64 rows is staged in LDS as it lies in memory (X
 // converted to bf16 on the way) and read back with ds_read_b64_tr_b16, which hands a group of 16 lanes a 4 x 16 block
 // transposed.  Row strides of 64 bytes times an odd number keep the four rows of such a block in different banks.
-// A workgroup owns a (32 MB WM) x (32 NB WN) tile of dW and steps s, s + S, ...: WM WN waves share a step's staging (a
-// barrier per step), or, with WM = WN = 1, each of the four waves stages its own steps.  S partial tiles go to the
+// A workgroup owns a (32 MB WM) x (32 NB WN) tile of dW and steps s, s + S, ... of ROWS rows: WM WN waves share a step's
+// staging (a barrier per step), or, with WM = WN = 1, each of four waves stages its own steps.  S partial tiles go to the
 // workspace, summed in a fixed order by rowvec.h's fold (S = 1: straight to dW).
-constexpr int WG_ROWS = 32;
+
 
 __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride, int lane) {
   // lane l of a 16-lane group reads 8 bytes of row (l & 15) >> 2, columns 4 (l & 3) ..; it receives column l & 15, four rows
@@ -111,18 +111,31 @@ constexpr int odd64(int cols) {                                  // row stride i
   return ((cols / 32) & 1) ? cols : cols + 32;
 }
 
-template <int MB, int NB, int WM, int WN>
-__global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, int N, const bf16* __restrict__ dY,
-                                                         long long dys, const signed char* __restrict__ codes,
-                                                         long long pitch, const unsigned char* __restrict__ scales,
-                                                         float* __restrict__ out, int S, int tiles_n) {
-  constexpr bool SHARED = WM * WN == 4;                          // four waves share the staged step
-  static_assert(SHARED || (WM == 1 && WN == 1), "either the waves tile the output or each has steps of its own");
+// 8 values that start `skip` places late, moved down (the places freed get zeros)
+__device__ __forceinline__ uint4 shift_down(const rv::u4_any& v, int skip) {
+  const unsigned long long lo = ((unsigned long long)v.y << 32) | v.x, hi = ((unsigned long long)v.w << 32) | v.z;
+  const int b = 16 * (skip & 3);
+  unsigned long long l = b ? (lo >> b) | (hi << (64 - b)) : lo, h = hi >> b;
+  if (skip & 4) { l = h; h = 0; }
+  return make_uint4((unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32));
+}
+
+// Every load is whole and unconditional -- rows behind the last repeat it (their dY is zeroed and their scale set to 1 when
+// they are staged), columns behind the last repeat others and end in columns of the tile that are not stored -- and its
+// address is a base the workgroup shares plus a 32-bit offset.  RAGGED: M is no multiple of 8.
+template <int MB, int NB, int WM, int WN, int ROWS, bool RAGGED>
+__global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_kernel(long long rows, int M, int N, const bf16* __restrict__ dY, int dys,
+                                                         const signed char* __restrict__ codes, int pitch,
+                                                         const unsigned char* __restrict__ scales, float* __restrict__ out,
+                                                         int S, int tiles_n) {
+  constexpr bool SHARED = WM * WN > 1;                           // the waves share the staged step
+  static_assert(SHARED || ROWS == 32, "a wave on its own takes 32 rows a step");
   constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN;
   constexpr int LA = odd64(TM), LB = odd64(TN);
-  constexpr int STEP = WG_ROWS * (LA + LB);                      // elements of one staged step
-  constexpr int NT = SHARED ? 256 : 64;                          // threads that stage a step
-  constexpr int QA = WG_ROWS * TM / 8 / NT, QB = (WG_ROWS * TN / 16 + NT - 1) / NT;
+  constexpr int STEP = ROWS * (LA + LB);                      // elements of one staged step
+  constexpr int NT = 64 * WM * WN;                              // threads that stage a step
+  constexpr int QA = ROWS * TM / 8 / NT, QB = ROWS * TN / 16 / NT;
+  static_assert(QA >= 1 && QB >= 1, "every thread has a chunk of both");
   constexpr int BUFS = SHARED ? 2 : 4;
   constexpr int FOLD = SHARED ? 0 : TM * TN * 2;                 // the four waves' tiles are added in LDS at the end
   __shared__ __attribute__((aligned(16))) unsigned short lds[(BUFS * STEP > FOLD ? BUFS * STEP : FOLD)];
@@ -131,8 +144,8 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, 
   const int tile = blockIdx.x / S, split = blockIdx.x - tile * S;
   const int m0 = (tile / tiles_n) * TM, n0 = (tile - (tile / tiles_n) * tiles_n) * TN;
   const int G = (N + rv::GROUP - 1) / rv::GROUP;
-  const long long steps = (rows + WG_ROWS - 1) / WG_ROWS;
-  const long long first = SHARED ? split : (long long)split * 4 + wave, stride = SHARED ? S : (long long)S * 4;
+  const int whole = (int)(rows / ROWS), rest = (int)(rows - (long long)whole * ROWS);
+  const int first = SHARED ? split : __builtin_amdgcn_readfirstlane(split * 4 + wave), stride = SHARED ? S : S * 4;
   const int wm = SHARED ? (wave % WM) * 32 * MB : 0, wn = SHARED ? (wave / WM) * 32 * NB : 0;
   f32x16 acc[MB][NB];
 #pragma unroll
@@ -142,99 +155,154 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  rv::u4_any ra[QA];
-  uint4 rb[QB];
-  unsigned rs[QB];
-  auto fetch = [&](long long step) {
+  // this thread's chunks: row of the step, column (in memory: the window that holds it)
+  int ar[QA], ac[QA], askip[QA], br[QB], bc[QB];
+#pragma unroll
+  for (int i = 0; i < QA; ++i) {
+    const int q = i * NT + tid, c = m0 + q % (TM / 8) * 8;
+    ar[i] = q / (TM / 8);
+    ac[i] = min(c, max(M - 8, 0));
+    askip[i] = min(c - ac[i], 8);
+  }
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = i * NT + tid;
+    br[i] = q / (TN / 16);
+    bc[i] = min(n0 + q % (TN / 16) * 16, (N - 1) & ~15);         // (the pitch is a multiple of 16: whole chunks)
+  }
+  struct held {
+    rv::u4_any a[QA];
+    uint4 b[QB];
+    unsigned char s[QB];
+  };
+  // last_step: the step of the rows behind the last whole one
+  auto fetch = [&](int step, held& h, bool last_step) {
+    const bf16* const pa = dY + (long long)step * ROWS * dys;
+    const signed char* const pb = codes + (long long)step * ROWS * pitch;
+    const unsigned char* const ps = scales + (long long)step * ROWS * G;
 #pragma unroll
     for (int i = 0; i < QA; ++i) {
-      const int q = i * NT + tid, r = q / (TM / 8), c = m0 + (q - r * (TM / 8)) * 8;
-      const long long row = step * WG_ROWS + r;
-      ra[i] = rv::u4_any{0, 0, 0, 0};
-      if (row < rows && c < M) {
-        const bf16* p = dY + row * dys + c;
-        if (c + 8 <= M) {
-          ra[i] = *reinterpret_cast<const rv::u4_any*>(p);
-        } else {                                                 // the last columns of a row, never past its end
-          unsigned h[8];
+      const bf16* const p = rv::at32(pa, (__umul24(last_step ? min(ar[i], rest - 1) : ar[i], dys) + ac[i]) * 2u);
+      if (RAGGED && M < 8) {                                     // rows shorter than a chunk: value by value
+        unsigned v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = c + e < M ? p[e].u : 0u;
-          ra[i] = rv::u4_any{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+        for (int e = 0; e < 8; ++e) v[e] = p[min(e, M - 1)].u;
+        h.a[i] = rv::u4_any{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+      } else {
+        h.a[i] = *reinterpret_cast<const rv::u4_any*>(p);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      const int r = last_step ? min(br[i], rest - 1) : br[i];
+      h.b[i] = *reinterpret_cast<const uint4*>(rv::at32(pb, __umul24(r, pitch) + bc[i]));
+      h.s[i] = *rv::at32(ps, __umul24(r, G) + bc[i] / rv::GROUP);
+    }
+  };
+  auto stage = [&](unsigned short* to, const held& h, bool last_step) {
+#pragma unroll
+    for (int i = 0; i < QA; ++i) {
+      uint4 v = make_uint4(h.a[i].x, h.a[i].y, h.a[i].z, h.a[i].w);
+      if (RAGGED && M >= 8) v = shift_down(h.a[i], askip[i]);
+      if (last_step && ar[i] >= rest) v = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(to + ar[i] * LA + (i * NT + tid) % (TM / 8) * 8) = v;
+    }
+    unsigned short* const tb = to + ROWS * LA;
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      const float two = rv::group_step(last_step && br[i] >= rest ? 1u : h.s[i]);
+      const unsigned wd[4] = {h.b[i].x, h.b[i].y, h.b[i].z, h.b[i].w};
+      unsigned v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = traits<bf16>::p2(rv::code_at(wd, 2 * e) * two, rv::code_at(wd, 2 * e + 1) * two);
+      uint4* const p = reinterpret_cast<uint4*>(tb + br[i] * LB + (i * NT + tid) % (TN / 16) * 16);
+      p[0] = make_uint4(v[0], v[1], v[2], v[3]);
+      p[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+  };
+  constexpr int KS = 2;
+  struct frags { bf16x8 a[KS][MB], b[KS][NB]; };
+  auto read = [&](const unsigned short* from, frags& f, int k0) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) f.b[k][j] = tr_frag(from + ROWS * LA + (k0 + k * 16) * LB + wn + j * 32, LB, lane);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) f.a[k][i] = tr_frag(from + (k0 + k * 16) * LA + wm + i * 32, LA, lane);
+    }
+  };
+  auto multiply = [&](const frags& f) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[k][i], f.b[k][j], acc[i][j], 0, 0, 0);
+  };
+
+  const int n = first < whole ? (whole - 1 - first) / stride + 1 : 0;          // whole steps of this workgroup (wave)
+  held h;
+  if (SHARED) {
+    // One barrier a step: behind it the step's fragments are read, the next step (in registers since the last barrier) is
+    // converted into the other buffer -- which every wave has read before it came to this barrier -- and the products run
+    // beside that.  What is fetched and staged ahead of the last step is never multiplied.
+    if (n > 0) {
+      auto step_at = [&](int i) { return first + min(i, n - 1) * stride; };
+      fetch(step_at(0), h, false);
+      stage(lds, h, false);
+      fetch(step_at(1), h, false);
+      for (int i = 0; i < n; i += 2) {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          if (i + d < n) {           // (the same for the whole workgroup)
+            frags f;
+            __syncthreads();
+            read(lds + (d & 1) * STEP, f, 0);
+            stage(lds + ((d & 1) ^ 1) * STEP, h, false);
+            fetch(step_at(i + d + 2), h, false);
+            multiply(f);
+#pragma unroll
+            for (int k = 32; k < ROWS; k += 32) {
+              read(lds + (d & 1) * STEP, f, k);
+              multiply(f);
+            }
+          }
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      const int q = i * NT + tid, r = q / (TN / 16), c = n0 + (q - r * (TN / 16)) * 16;
-      const long long row = step * WG_ROWS + r;
-      const bool in = row < rows && c < N && r < WG_ROWS;
-      rb[i] = make_uint4(0, 0, 0, 0);
-      rs[i] = 1;
-      if (in) {                                                  // (the pitch is a multiple of 16: whole chunks)
-        rb[i] = *reinterpret_cast<const uint4*>(codes + row * pitch + c);
-        rs[i] = scales[row * G + c / rv::GROUP];
-      }
-    }
-  };
-  auto stage = [&](unsigned short* to) {
-#pragma unroll
-    for (int i = 0; i < QA; ++i) {
-      const int q = i * NT + tid, r = q / (TM / 8), c = (q - r * (TM / 8)) * 8;
-      *reinterpret_cast<uint4*>(to + r * LA + c) = make_uint4(ra[i].x, ra[i].y, ra[i].z, ra[i].w);
-    }
-    unsigned short* const tb = to + WG_ROWS * LA;
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      const int q = i * NT + tid, r = q / (TN / 16), c = (q - r * (TN / 16)) * 16;
-      if (WG_ROWS * TN / 16 % NT == 0 || r < WG_ROWS) {
-        const float step = rv::group_step(rs[i]);
-        const unsigned wd[4] = {rb[i].x, rb[i].y, rb[i].z, rb[i].w};
-        float v[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = rv::code_at(wd, e) * step;
-        typedef traits<bf16> tb16;
-        *reinterpret_cast<uint4*>(tb + r * LB + c) =
-            make_uint4(tb16::p2(v[0], v[1]), tb16::p2(v[2], v[3]), tb16::p2(v[4], v[5]), tb16::p2(v[6], v[7]));
-        *reinterpret_cast<uint4*>(tb + r * LB + c + 8) =
-            make_uint4(tb16::p2(v[8], v[9]), tb16::p2(v[10], v[11]), tb16::p2(v[12], v[13]), tb16::p2(v[14], v[15]));
-      }
-    }
-  };
-  auto multiply = [&](const unsigned short* from) {
-#pragma unroll
-    for (int ks = 0; ks < WG_ROWS; ks += 16) {
-      bf16x8 b[NB];
-#pragma unroll
-      for (int j = 0; j < NB; ++j) b[j] = tr_frag(from + WG_ROWS * LA + ks * LB + wn + j * 32, LB, lane);
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const bf16x8 a = tr_frag(from + ks * LA + wm + i * 32, LA, lane);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-      }
-    }
-  };
-
-  if (SHARED) {
-    // every thread of the workgroup runs the same number of steps
-    int at = 0;
-    if (first < steps) fetch(first);
-    for (long long s = first; s < steps; s += stride, at ^= 1) {
-      stage(lds + at * STEP);
+    if (rest && whole % S == split) {                            // the rows behind the last whole step
+      frags f;
       __syncthreads();
-      if (s + stride < steps) fetch(s + stride);
-      multiply(lds + at * STEP);      // the other buffer is written next; this one again after the barrier that follows
+      fetch(whole, h, true);
+      stage(lds, h, true);
+      __syncthreads();
+      for (int k = 0; k < ROWS; k += 32) {
+        read(lds, f, k);
+        multiply(f);
+      }
     }
   } else {
     unsigned short* const mine = lds + wave * STEP;
-    if (first < steps) fetch(first);
-    for (long long s = first; s < steps; s += stride) {
-      stage(mine);
-      if (s + stride < steps) fetch(s + stride);
+    if (n > 0) fetch(first, h, false);
+    for (int i = 0; i < n; ++i) {
+      frags f;
+      stage(mine, h, false);
+      fetch(first + min(i + 1, n - 1) * stride, h, false);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");     // a wave's own LDS writes and reads: in order
       __builtin_amdgcn_wave_barrier();
-      multiply(mine);
+      read(mine, f, 0);
+      multiply(f);
       __builtin_amdgcn_wave_barrier();
+    }
+    if (rest && whole % (S * 4) == first) {
+      frags f;
+      fetch(whole, h, true);
+      stage(mine, h, true);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      read(mine, f, 0);
+      multiply(f);
     }
   }
 
@@ -276,24 +344,32 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(long long rows, int M, 
   }
 }
 
-// tile and number of row splits of a call
+// Tile, rows of a step and number of row splits of a call.  Every split leaves a partial tile that is written and read
+// again, so there are no more workgroups than keep the chip busy: one of eight waves per CU for the 256 x 128 tile (33 MB of
+// partial sums at most; 98304 x 512 x 512: 81 us, 93 us with two per CU), two of four waves for 128 x 128 (91 us; 101 us with
+// three), three for the narrow tiles, whose waves work for themselves.  The 256 x 128 tile converts each code for twice the
+// output; up to 128 output channels half of it would be empty (393216 x 128 x 128: 128 x 128).
 struct wg_plan { int kind, tm, tn, S; };
 
 wg_plan wgrad_plan(long long rows, int M, int N) {
   wg_plan p;
-  if (M > 64 && N > 64) { p.kind = 0; p.tm = 128; p.tn = 128; }
-  else if (M > 32 && N > 32) { p.kind = 1; p.tm = 64; p.tn = 64; }
-  else if (M > 32) { p.kind = 2; p.tm = 64; p.tn = 32; }
-  else if (N > 32) { p.kind = 3; p.tm = 32; p.tn = 64; }
-  else { p.kind = 4; p.tm = 32; p.tn = 32; }
+  int step = 32, wgs = 768, per = 16;                            // per: steps a workgroup should have at least
+  if (M > 128 && N > 64) { p.kind = 0; p.tm = 256; p.tn = 128; step = 64; wgs = 256; per = 4; }
+  else if (M > 64 && N > 64) { p.kind = 1; p.tm = 128; p.tn = 128; step = 64; wgs = 512; per = 4; }
+  else if (M > 32 && N > 32) { p.kind = 2; p.tm = 64; p.tn = 64; }
+  else if (M > 32) { p.kind = 3; p.tm = 64; p.tn = 32; }
+  else if (N > 32) { p.kind = 4; p.tm = 32; p.tn = 64; }
+  else { p.kind = 5; p.tm = 32; p.tn = 32; }
   const long long tiles = (long long)pvn3d_ceil_div(M, p.tm) * pvn3d_ceil_div(N, p.tn);
-  const long long steps = (rows + WG_ROWS - 1) / WG_ROWS;
-  const long long per = p.kind == 0 ? 4 : 16;                    // steps a workgroup should have at least
-  long long S = 768 / tiles;
+  const long long steps = (rows + step - 1) / step;
+  long long S = wgs / tiles;
   if (S > (steps + per - 1) / per) S = (steps + per - 1) / per;
   p.S = (int)(S < 1 ? 1 : S);
   return p;
 }
+
+constexpr long long MAX_STRIDE = 1 << 20;      // a step's rows are within 32-bit offsets of its base
+constexpr long long MAX_ROWS = 1ll << 35;      // steps are counted in 32 bits
 
 #define A8_ST ((hipStream_t)stream)
 
@@ -361,7 +437,8 @@ extern "C" size_t pvn3d_act8_wgrad_workspace_bytes(long long rows, int M, int N)
 extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, long long dys, const void* codes,
                                 long long pitch, const void* scales, float* dW, void* workspace, size_t workspace_bytes,
                                 void* stream) {
-  if (M < 0 || N < 0 || dys < 0 || (pitch & 15) || pitch < N) return (int)hipErrorInvalidValue;
+  if (M < 0 || N < 0 || dys < 0 || (pitch & 15) || pitch < N || dys > MAX_STRIDE || pitch > MAX_STRIDE)
+    return (int)hipErrorInvalidValue;
   if (M == 0 || N == 0) return 0;
   if (!dW) return (int)hipErrorInvalidValue;
   if (rows <= 0) {
@@ -369,7 +446,7 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
     PVN3D_LAUNCH_CHECK();
     return 0;
   }
-  if (!dY || !codes || !scales) return (int)hipErrorInvalidValue;
+  if (!dY || !codes || !scales || rows > MAX_ROWS) return (int)hipErrorInvalidValue;
   const wg_plan p = wgrad_plan(rows, M, N);
   const size_t count = (size_t)M * N;
   if (p.S > 1 && (!workspace || workspace_bytes < p.S * count * sizeof(float))) return (int)hipErrorInvalidValue;
@@ -377,16 +454,24 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
   const int tn = pvn3d_ceil_div(N, p.tn);
   const long long blocks = (long long)pvn3d_ceil_div(M, p.tm) * tn * p.S;
   if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidValue;
-#define A8_CALL(MB, NB, WM, WN)                                                                                      \
-  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN>), dim3((unsigned)blocks), dim3(256), 0, A8_ST, rows, M, N,  \
-                     (const bf16*)dY, dys, (const signed char*)codes, pitch, (const unsigned char*)scales, out, p.S, tn)
+#define A8_ONE(MB, NB, WM, WN, ROWS, RAG)                                                                                    \
+  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN, ROWS, RAG>), dim3((unsigned)blocks), dim3(WM * WN > 1 ? 64 * WM * WN : 256), 0, A8_ST, rows, M, N, \
+                     (const bf16*)dY, (int)dys, (const signed char*)codes, (int)pitch, (const unsigned char*)scales, out,  \
+                     p.S, tn)
+#define A8_CALL(MB, NB, WM, WN, ROWS)              \
+  do {                                           \
+    if (M & 7) A8_ONE(MB, NB, WM, WN, ROWS, true); \
+    else A8_ONE(MB, NB, WM, WN, ROWS, false);      \
+  } while (0)
   switch (p.kind) {
-    case 0: A8_CALL(2, 2, 2, 2); break;
-    case 1: A8_CALL(2, 2, 1, 1); break;
-    case 2: A8_CALL(2, 1, 1, 1); break;
-    case 3: A8_CALL(1, 2, 1, 1); break;
-    default: A8_CALL(1, 1, 1, 1); break;
+    case 0: A8_CALL(2, 2, 4, 2, 64); break;
+    case 1: A8_CALL(2, 2, 2, 2, 64); break;
+    case 2: A8_CALL(2, 2, 1, 1, 32); break;
+    case 3: A8_CALL(2, 1, 1, 1, 32); break;
+    case 4: A8_CALL(1, 2, 1, 1, 32); break;
+    default: A8_CALL(1, 1, 1, 1, 32); break;
   }
+#undef A8_ONE
 #undef A8_CALL
   PVN3D_LAUNCH_CHECK();
   return p.S > 1 ? rv::fold(p.S, count, count, (const float*)workspace, dW, nullptr, A8_ST) : 0;

@@ -192,45 +192,77 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v) {
 }
 
 // ---------------------------------------------------------------------------------------------- partial sums
-// out[e] = sum over p of part[p][count], e < count, in a fixed order: SL slices of p a workgroup, 1024 / SL columns, eight
-// loads in flight per thread.  e < first goes to a, the rest to b.
-template <int SL>
+// out[e] = sum over p of part[p][count], e < count, in a fixed order: SL slices of p a workgroup, 1024 / SL threads across,
+// W (1 or 4) columns each, eight loads in flight per thread.  e < first goes to a, the rest to b.
+template <int SL, int W>
 __global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t first, const float* __restrict__ part,
                                                     float* __restrict__ a, float* __restrict__ b) {
-  constexpr int COLS = 1024 / SL;
-  __shared__ float s[SL][COLS];
-  const int col = threadIdx.x % COLS, sl = threadIdx.x / COLS;
-  const size_t e = (size_t)blockIdx.x * COLS + col;
-  float v = 0.f;
+  constexpr int TX = 1024 / SL;
+  __shared__ float s[SL][TX * W];
+  const int tx = threadIdx.x % TX, sl = threadIdx.x / TX;
+  const size_t e = ((size_t)blockIdx.x * TX + tx) * W;
+  float v[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = 0.f;
+  auto get = [&](int p, float (&f)[W]) {
+    const float* q = part + (size_t)p * count + e;
+    if (W == 4) {
+      const float4 r = *reinterpret_cast<const float4*>(q);
+      f[0] = r.x; f[W > 1 ? 1 : 0] = r.y; f[W > 2 ? 2 : 0] = r.z; f[W > 3 ? 3 : 0] = r.w;
+    } else {
+      f[0] = *q;
+    }
+  };
   if (e < count) {
-    const float* p = part + e;
     int i = sl;
     for (; i + 7 * SL < P; i += 8 * SL) {
-      float f[8];
+      float f[8][W];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = p[(size_t)(i + j * SL) * count];
-      v += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+      for (int j = 0; j < 8; ++j) get(i + j * SL, f[j]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] += ((f[0][j] + f[1][j]) + (f[2][j] + f[3][j])) + ((f[4][j] + f[5][j]) + (f[6][j] + f[7][j]));
     }
-    for (; i < P; i += SL) v += p[(size_t)i * count];
-  }
-  s[sl][col] = v;
-  __syncthreads();
+    for (; i < P; i += SL) {
+      float f[W];
+      get(i, f);
 #pragma unroll
-  for (int o = SL / 2; o >= 1; o >>= 1) {
-    if (sl < o) s[sl][col] += s[sl + o][col];
-    __syncthreads();
+      for (int j = 0; j < W; ++j) v[j] += f[j];
+    }
   }
-  if (sl == 0 && e < count) (e < first ? a[e] : b[e - first]) = s[0][col];
+  if (SL > 1) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) s[sl][tx * W + j] = v[j];
+    __syncthreads();
+#pragma unroll
+    for (int o = SL / 2; o >= 1; o >>= 1) {
+      if (sl < o) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) s[sl][tx * W + j] += s[sl + o][tx * W + j];
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = s[sl][tx * W + j];
+  }
+  if (sl == 0 && e < count) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) (e + j < first ? a[e + j] : b[e + j - first]) = v[j];
+  }
 }
 static inline int fold(int P, size_t count, size_t first, const float* part, float* a, float* b, hipStream_t st) {
-  // slices: as many as leave a thread about eight partial sums (64 slices of 16 columns still read whole 64-byte lines)
-#define RV_FOLD(SL)                                                                                                   \
-  hipLaunchKernelGGL((fold_kernel<SL>), dim3((unsigned)((count + 1024 / SL - 1) / (1024 / SL))), dim3(1024), 0, st, P, \
-                     count, first, part, a, b)
-  if (P >= 256) RV_FOLD(64);
-  else if (P >= 64) RV_FOLD(32);
-  else if (P >= 16) RV_FOLD(8);
-  else RV_FOLD(2);
+  // slices: as many as leave a thread about eight partial sums (64 slices of 16 columns still read whole 64-byte lines);
+  // four columns a thread for few sums of many columns (16 of 512 x 1536: 50 MB)
+#define RV_FOLD(SL, W)                                                                                                    \
+  hipLaunchKernelGGL((fold_kernel<SL, W>), dim3((unsigned)((count + W * 1024 / SL - 1) / (W * 1024 / SL))), dim3(1024), 0, \
+                     st, P, count, first, part, a, b)
+  const bool wide = count >= 32768 && (count & 3) == 0;
+  if (wide && P >= 64) RV_FOLD(16, 4);
+  else if (wide && P >= 16) RV_FOLD(4, 4);
+  else if (wide) RV_FOLD(2, 4);
+  else if (P >= 256) RV_FOLD(64, 1);
+  else if (P >= 64) RV_FOLD(32, 1);
+  else if (P >= 16) RV_FOLD(8, 1);
+  else RV_FOLD(2, 1);
 #undef RV_FOLD
   PVN3D_LAUNCH_CHECK();
   return 0;
