@@ -84,31 +84,33 @@ class GraphedForward(object):
 
 
 class Pointnet2MSG(nn.Module):
-    def __init__(self, input_channels=6, use_xyz=True):
+    """norm: "batch" (the reference's) or "layer": a layer norm over each point's channels in every SharedMLP layer."""
+
+    def __init__(self, input_channels=6, use_xyz=True, norm="batch"):
         super(Pointnet2MSG, self).__init__()
         self.SA_modules = nn.ModuleList()
         c_in = input_channels
         self.SA_modules.append(PointnetSAModuleMSG(
             npoint=2048, radii=[0.0175, 0.025], nsamples=[16, 32],
-            mlps=[[c_in, 16, 16, 32], [c_in, 32, 32, 64]], use_xyz=use_xyz))
+            mlps=[[c_in, 16, 16, 32], [c_in, 32, 32, 64]], use_xyz=use_xyz, norm=norm))
         c_out_0 = 32 + 64
         self.SA_modules.append(PointnetSAModuleMSG(
             npoint=1024, radii=[0.025, 0.05], nsamples=[16, 32],
-            mlps=[[c_out_0, 64, 64, 128], [c_out_0, 64, 96, 128]], use_xyz=use_xyz))
+            mlps=[[c_out_0, 64, 64, 128], [c_out_0, 64, 96, 128]], use_xyz=use_xyz, norm=norm))
         c_out_1 = 128 + 128
         self.SA_modules.append(PointnetSAModuleMSG(
             npoint=512, radii=[0.05, 0.1], nsamples=[16, 32],
-            mlps=[[c_out_1, 128, 196, 256], [c_out_1, 128, 196, 256]], use_xyz=use_xyz))
+            mlps=[[c_out_1, 128, 196, 256], [c_out_1, 128, 196, 256]], use_xyz=use_xyz, norm=norm))
         c_out_2 = 256 + 256
         self.SA_modules.append(PointnetSAModuleMSG(
             npoint=128, radii=[0.1, 0.2], nsamples=[16, 32],
-            mlps=[[c_out_2, 256, 256, 512], [c_out_2, 256, 384, 512]], use_xyz=use_xyz))
+            mlps=[[c_out_2, 256, 256, 512], [c_out_2, 256, 384, 512]], use_xyz=use_xyz, norm=norm))
         c_out_3 = 512 + 512
         self.FP_modules = nn.ModuleList()
-        self.FP_modules.append(PointnetFPModule(mlp=[256 + input_channels, 128, 128]))
-        self.FP_modules.append(PointnetFPModule(mlp=[512 + c_out_0, 256, 256]))
-        self.FP_modules.append(PointnetFPModule(mlp=[512 + c_out_1, 512, 512]))
-        self.FP_modules.append(PointnetFPModule(mlp=[c_out_3 + c_out_2, 512, 512]))
+        self.FP_modules.append(PointnetFPModule(mlp=[256 + input_channels, 128, 128], norm=norm))
+        self.FP_modules.append(PointnetFPModule(mlp=[512 + c_out_0, 256, 256], norm=norm))
+        self.FP_modules.append(PointnetFPModule(mlp=[512 + c_out_1, 512, 512], norm=norm))
+        self.FP_modules.append(PointnetFPModule(mlp=[c_out_3 + c_out_2, 512, 512], norm=norm))
 
         # inference: the SA levels and the intermediate FP levels hand point-major buffers (as transposed
         # views) to the next level; the last one (FP_modules[0]) returns the reference's contiguous (B, 128, N)

@@ -1,4 +1,5 @@
-"""Training-mode SharedMLP on the hand-written bf16 MFMA kernels (csrc/mlp_train.hip).
+"""Training-mode SharedMLP on the hand-written bf16 MFMA kernels (csrc/mlp_train.hip; with norm = "layer" also
+csrc/layer_norm.hip, and csrc/act8.hip where inputs are kept in 8 bits).
 
 Replaces, when a set-abstraction / feature-propagation module is in training mode on the GPU, the reference's
     grouped (B, C, npoint, nsample) tensor -> [Conv2d 1x1 -> BatchNorm2d(batch stats) -> ReLU] x L -> max_pool2d
@@ -16,6 +17,8 @@ import torch
 import torch.nn as nn
 
 from ..._lib import lib, check, on_device
+from ..act8 import Act8, act8_pack, linear8_weight_grad
+from ..layer_norm import LayerNorm, Saved8
 from . import _ext
 
 # Which SharedMLP path SA / FP modules take in training mode:
@@ -25,6 +28,13 @@ from . import _ext
 #   True:    explicit opt-in, the bf16 chain whatever the autocast state;
 #   False:   always the reference's op-by-op composition (torch Conv2d / BatchNorm2d).
 TRAIN_FUSED = "auto"
+
+# What a chain keeps of its layers' inputs between the forward and the backward pass:
+#   False (default): the bf16 matrices;
+#   True: their 8-bit form (lib/act8.py) -- 33/32 bytes per value instead of 2, the weight gradients are taken from it (a
+#         value is off by at most 1/128 of the largest of its 32 channels); layers with a LayerNorm keep the norm's input
+#         that way too, with one bit per value for the ReLU.  Outputs, and with BatchNorm the input gradients, do not change.
+ACT_CKPT8 = False
 
 
 def train_fused_enabled():
@@ -45,6 +55,7 @@ def _bump_version(t):
 
 # kernel limits of csrc/mlp_train.hip (pool / BatchNorm passes): beyond them the modules keep the op-by-op composition
 MAX_NSAMPLE = 256
+MAX_NSAMPLE_LN = 255        # layer-norm chains: the stand-alone pool kernel holds a neighbour's index in a byte
 MAX_LD = 2048
 
 
@@ -57,11 +68,19 @@ def _strides3(t):
     return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
 
 
+def _ln_of(norm):
+    """The LayerNorm of a SharedMLP layer's norm (channels second, fp32 parameters, ReLU left to the layer), or None."""
+    ln = getattr(norm, "ln", None) if norm is not None else None
+    ok = (isinstance(ln, LayerNorm) and ln.channel_dim == 1 and not ln.relu and ln.weight.dtype == torch.float32
+          and ln.bias.dtype == torch.float32)
+    return ln if ok else None
+
+
 def shared_mlp_layers(mlp):
     """SharedMLP -> [(conv, bn)] when every layer is exactly [1x1 Conv2d without bias] -> BatchNorm2d -> ReLU
     (the only form PVN3D builds) with the BatchNorm in training mode (a frozen / eval BatchNorm inside a module that
     is in training mode normalises with its running statistics and must not update them: that composition is left
-    to torch); None otherwise."""
+    to torch), or [(conv, ln)] when the norm of every layer is a LayerNorm; None otherwise."""
     out = []
     for layer in mlp.children():
         names = [n for n, _ in layer.named_children()]
@@ -71,11 +90,23 @@ def shared_mlp_layers(mlp):
         act = getattr(layer, "activation", None)
         if (names[:1] != ["conv"] or not isinstance(conv, nn.Conv2d) or conv.kernel_size != (1, 1)
                 or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1 or conv.bias is not None
-                or not isinstance(bn, nn.BatchNorm2d) or not bn.affine or not bn.track_running_stats
-                or bn.momentum is None or not bn.training or not isinstance(act, nn.ReLU)):
+                or not isinstance(act, nn.ReLU)):
+            return None
+        ln = _ln_of(norm)
+        if ln is not None:
+            out.append((conv, ln))
+            continue
+        if (not isinstance(bn, nn.BatchNorm2d) or not bn.affine or not bn.track_running_stats
+                or bn.momentum is None or not bn.training):
             return None
         out.append((conv, bn))
+    if len({isinstance(n, LayerNorm) for _, n in out}) > 1:
+        return None
     return out or None
+
+
+def _is_ln(layers):
+    return isinstance(layers[0][1], LayerNorm)
 
 
 class _Chain(object):
@@ -85,28 +116,43 @@ class _Chain(object):
     def __init__(self, x0, c_in, weights, gammas, betas, bns):
         self.dev = x0.device
         self.rows = x0.size(0)
-        self.x0 = x0
+        self.x0 = x0                     # the forward's input; given up once it is kept in `inputs`
         self.c = [int(c_in)] + [int(w.size(0)) for w in weights]
         self.weights, self.gammas, self.betas, self.bns = weights, gammas, betas, bns
-        self.y, self.h, self.mean, self.invstd, self.a = [], [], [], [], []
+        self.ckpt8 = bool(ACT_CKPT8)
+        self.inputs = []                 # per layer, for its weight gradient: the bf16 matrix or its Act8
+        self.y, self.mean = [], []
+
+    def _keep_input(self, li, prev):
+        self.inputs.append(act8_pack(prev[:, :self.c[li]]) if self.ckpt8 else prev)
+
+    def _product(self, li, prev, y, ps, st):
+        """y = prev . W_li^T; ps: partial column sums for BatchNorm, or None."""
+        cin, cout = self.c[li], self.c[li + 1]
+        ldi, ldo = _ld(cin), _ld(cout)
+        wb = torch.empty((cout, ldi), dtype=torch.bfloat16, device=self.dev)
+        check(lib.pvn3d_mt_pack_weight(cout, cin, self.weights[li].data_ptr(), cin, 0, wb.data_ptr(), cout, ldi, st),
+              "mt_pack_weight")
+        check(lib.pvn3d_mt_gemm_nt(self.rows, cout, ldi, prev.data_ptr(), ldi, wb.data_ptr(), ldi, y.data_ptr(), ldo,
+                                   ps[0].data_ptr() if ps is not None else None,
+                                   ps[1].data_ptr() if ps is not None else None, ldo if ps is not None else 0, st),
+              "mt_gemm_nt")
 
     def forward(self, update_running=True, pool=None):
         """pool = (G, ns, out_ptr, out_ld, arg): the last layer's ReLU output goes straight into the max-pool (its
         matrix is not materialised); returns None then."""
         dev, rows, st = self.dev, self.rows, None
-        prev = self.x0
+        prev, self.x0 = self.x0, None
         L = len(self.weights)
-        for li, w in enumerate(self.weights):
-            cin, cout = self.c[li], self.c[li + 1]
-            ldi, ldo = _ld(cin), _ld(cout)
+        for li in range(L):
+            cout = self.c[li + 1]
+            ldo = _ld(cout)
             st = _stream(prev)
-            wb = torch.empty((cout, ldi), dtype=torch.bfloat16, device=dev)
-            check(lib.pvn3d_mt_pack_weight(cout, cin, w.data_ptr(), cin, 0, wb.data_ptr(), cout, ldi, st), "mt_pack_weight")
             y = torch.empty((rows, ldo), dtype=torch.bfloat16, device=dev)
             P = lib.pvn3d_mt_gemm_nt_stat_rows(rows)
             ps = torch.empty((2, P, ldo), dtype=torch.float32, device=dev)
-            check(lib.pvn3d_mt_gemm_nt(rows, cout, ldi, prev.data_ptr(), ldi, wb.data_ptr(), ldi, y.data_ptr(), ldo,
-                                       ps[0].data_ptr(), ps[1].data_ptr(), ldo, st), "mt_gemm_nt")
+            self._product(li, prev, y, ps, st)
+            self._keep_input(li, prev)
             bn = self.bns[li]
             stats = torch.empty((4, ldo), dtype=torch.float32, device=dev)      # mean, invstd, a, b
             track = update_running and bn.running_mean is not None
@@ -129,26 +175,70 @@ class _Chain(object):
                 G, ns, out_ptr, out_ld, arg = pool
                 check(lib.pvn3d_mt_bn_relu_pool(G, ns, ldo, cout, y.data_ptr(), stats[2].data_ptr(), stats[3].data_ptr(),
                                                 out_ptr, out_ld, arg.data_ptr(), st), "mt_bn_relu_pool")
-                self.h.append(None)
                 return None
             h = torch.empty((rows, ldo), dtype=torch.bfloat16, device=dev)
             check(lib.pvn3d_mt_bn_relu_apply(rows, ldo, y.data_ptr(), stats[2].data_ptr(), stats[3].data_ptr(),
                                              h.data_ptr(), st), "mt_bn_relu_apply")
-            self.h.append(h)
             prev = h
         return prev
+
+    def _weight_grad(self, li, dy, st):
+        """dW (cout, cin) = dY^T . H_prev, K = rows."""
+        dev, rows = self.dev, self.rows
+        cin, cout = self.c[li], self.c[li + 1]
+        ldi, ldo = _ld(cin), _ld(cout)
+        prev = self.inputs[li]
+        if isinstance(prev, Act8):
+            return linear8_weight_grad(dy[:, :cout], prev)
+        dw = torch.zeros((cout, cin), dtype=torch.float32, device=dev)
+        if WGRAD_TN and lib.pvn3d_mt_wgrad_tn_ok(cout, cin):
+            # straight from the row-major matrices (no transposed copies)
+            check(lib.pvn3d_mt_wgrad_tn(rows, cout, cin, dy.data_ptr(), ldo, prev.data_ptr(), ldi, dw.data_ptr(), cin, st),
+                  "mt_wgrad_tn")
+        else:
+            # the transposed copies hold the contraction dimension (rows) contiguously: it has to be a multiple of
+            # 16 (8 rows per 16-byte store of the transpose, K % 16 of the GEMM) -- zero rows add nothing to dW
+            r16 = (rows + 15) // 16 * 16
+            dy_s, pv_s = dy, prev
+            if r16 != rows:
+                dy_s = torch.zeros((r16, ldo), dtype=torch.bfloat16, device=dev)
+                dy_s[:rows] = dy
+                pv_s = torch.zeros((r16, ldi), dtype=torch.bfloat16, device=dev)
+                pv_s[:rows] = prev
+            dyt = torch.empty((ldo, r16), dtype=torch.bfloat16, device=dev)
+            pvt = torch.empty((ldi, r16), dtype=torch.bfloat16, device=dev)
+            check(lib.pvn3d_mt_transpose(r16, ldo, dy_s.data_ptr(), dyt.data_ptr(), r16, st), "mt_transpose")
+            check(lib.pvn3d_mt_transpose(r16, ldi, pv_s.data_ptr(), pvt.data_ptr(), r16, st), "mt_transpose")
+            tiles = ((cout + 127) // 128) * ((cin + 127) // 128)
+            ksplit = max(1, min(r16 // 512, 1024 // tiles))
+            check(lib.pvn3d_mt_gemm_nt_splitk(cout, cin, r16, dyt.data_ptr(), r16, pvt.data_ptr(), r16,
+                                              dw.data_ptr(), cin, ksplit, st), "mt_gemm_nt_splitk")
+        return dw
+
+    def _input_grad(self, li, dy, st):
+        """dH_prev (rows, ldi) = dY . W."""
+        dev = self.dev
+        cin, cout = self.c[li], self.c[li + 1]
+        ldi, ldo = _ld(cin), _ld(cout)
+        wt = torch.empty((cin, ldo), dtype=torch.bfloat16, device=dev)
+        check(lib.pvn3d_mt_pack_weight(cout, cin, self.weights[li].data_ptr(), cin, 1, wt.data_ptr(), cin, ldo, st),
+              "mt_pack_weight")
+        dprev = torch.empty((self.rows, ldi), dtype=torch.bfloat16, device=dev)
+        check(lib.pvn3d_mt_gemm_nt(self.rows, cin, ldo, dy.data_ptr(), ldo, wt.data_ptr(), ldo, dprev.data_ptr(), ldi,
+                                   None, None, 0, st), "mt_gemm_nt")
+        return dprev
 
     def backward(self, dh, need_input_grad, pooled=None):
         """dh: bf16 (rows, ld_L) gradient w.r.t. the last layer's output, or None with pooled = (G, ns, dout_ptr,
         out_ld, arg): that gradient is the max-pool backward of dout and is never materialised.  Returns (dX0 or
         None, [dW], [dgamma], [dbeta])."""
         dev, rows = self.dev, self.rows
-        st = _stream(self.x0)
+        st = torch.cuda.current_stream(dev).cuda_stream
         L = len(self.weights)
         dws, dgs, dbs = [None] * L, [None] * L, [None] * L
         for li in range(L - 1, -1, -1):
-            cin, cout = self.c[li], self.c[li + 1]
-            ldi, ldo = _ld(cin), _ld(cout)
+            cout = self.c[li + 1]
+            ldo = _ld(cout)
             y, stats = self.y[li], self.mean[li]
             use_pool = pooled is not None and li == L - 1
             if use_pool:
@@ -181,45 +271,88 @@ class _Chain(object):
                                                 stats[3].data_ptr(), kk[0].data_ptr(), kk[1].data_ptr(), dy.data_ptr(), st),
                       "mt_bn_bwd_apply")
             dgs[li], dbs[li] = dgb[0], dgb[1]
-            # weight gradient: dW (cout, cin) = dY^T . H_prev, K = rows
-            prev = self.h[li - 1] if li > 0 else self.x0
-            dw = torch.zeros((cout, cin), dtype=torch.float32, device=dev)
-            if WGRAD_TN and lib.pvn3d_mt_wgrad_tn_ok(cout, cin):
-                # straight from the row-major matrices (no transposed copies)
-                check(lib.pvn3d_mt_wgrad_tn(rows, cout, cin, dy.data_ptr(), ldo, prev.data_ptr(), ldi, dw.data_ptr(), cin,
-                                            st), "mt_wgrad_tn")
-            else:
-                # the transposed copies hold the contraction dimension (rows) contiguously: it has to be a multiple of
-                # 16 (8 rows per 16-byte store of the transpose, K % 16 of the GEMM) -- zero rows add nothing to dW
-                r16 = (rows + 15) // 16 * 16
-                dy_s, pv_s = dy, prev
-                if r16 != rows:
-                    dy_s = torch.zeros((r16, ldo), dtype=torch.bfloat16, device=dev)
-                    dy_s[:rows] = dy
-                    pv_s = torch.zeros((r16, ldi), dtype=torch.bfloat16, device=dev)
-                    pv_s[:rows] = prev
-                dyt = torch.empty((ldo, r16), dtype=torch.bfloat16, device=dev)
-                pvt = torch.empty((ldi, r16), dtype=torch.bfloat16, device=dev)
-                check(lib.pvn3d_mt_transpose(r16, ldo, dy_s.data_ptr(), dyt.data_ptr(), r16, st), "mt_transpose")
-                check(lib.pvn3d_mt_transpose(r16, ldi, pv_s.data_ptr(), pvt.data_ptr(), r16, st), "mt_transpose")
-                tiles = ((cout + 127) // 128) * ((cin + 127) // 128)
-                ksplit = max(1, min(r16 // 512, 1024 // tiles))
-                check(lib.pvn3d_mt_gemm_nt_splitk(cout, cin, r16, dyt.data_ptr(), r16, pvt.data_ptr(), r16,
-                                                  dw.data_ptr(), cin, ksplit, st), "mt_gemm_nt_splitk")
-                del dyt, pvt, dy_s, pv_s
-            dws[li] = dw
-            # input gradient: dH_prev (rows, ldi) = dY . W
-            if li > 0 or need_input_grad:
-                wt = torch.empty((cin, ldo), dtype=torch.bfloat16, device=dev)
-                check(lib.pvn3d_mt_pack_weight(cout, cin, self.weights[li].data_ptr(), cin, 1, wt.data_ptr(), cin, ldo,
-                                               st), "mt_pack_weight")
-                dprev = torch.empty((rows, ldi), dtype=torch.bfloat16, device=dev)
-                check(lib.pvn3d_mt_gemm_nt(rows, cin, ldo, dy.data_ptr(), ldo, wt.data_ptr(), ldo, dprev.data_ptr(), ldi,
-                                           None, None, 0, st), "mt_gemm_nt")
-                dh = dprev
-            else:
-                dh = None
+            dws[li] = self._weight_grad(li, dy, st)
+            dh = self._input_grad(li, dy, st) if li > 0 or need_input_grad else None
         return dh, dws, dgs, dbs
+
+
+class _LNChain(_Chain):
+    """The same with a layer norm over every row's channels: [GEMM -> LayerNorm -> ReLU] x L, one launch for norm and ReLU
+    (csrc/layer_norm.hip) and no state beside the parameters.  Kept per layer: the norm's input and its statistics, with
+    ACT_CKPT8 in the 8-bit form together with the ReLU's bits."""
+
+    def forward(self, update_running=True, pool=None):
+        dev, rows = self.dev, self.rows
+        prev, self.x0 = self.x0, None
+        st = _stream(prev)
+        L = len(self.weights)
+        for li in range(L):
+            cout = self.c[li + 1]
+            ldo = _ld(cout)
+            y = torch.empty((rows, ldo), dtype=torch.bfloat16, device=dev)
+            self._product(li, prev, y, None, st)
+            self._keep_input(li, prev)
+            h = torch.empty((rows, ldo), dtype=torch.bfloat16, device=dev)
+            codes, pitch, scales, mask = None, 0, None, None
+            if self.ckpt8:
+                kept = Saved8(rows, cout, (rows, cout), torch.bfloat16, True, dev)
+                (codes, scales), (mean, rstd, mask) = kept.act._ptrs(), kept._ptrs()
+                pitch = kept.act.pitch
+            else:
+                stat = torch.empty((2, rows), dtype=torch.float32, device=dev)
+                mean, rstd = stat.data_ptr(), stat.data_ptr() + 4 * rows
+                kept = (y, stat)
+            check(lib.pvn3d_layer_norm(1, rows, cout, y.data_ptr(), ldo, self.gammas[li].data_ptr(),
+                                       self.betas[li].data_ptr(), float(self.bns[li].eps), 1, h.data_ptr(), ldo, ldo, mean,
+                                       rstd, codes, pitch, scales, mask, st), "layer_norm")
+            self.y.append(kept)
+            prev = h
+        if pool is None:
+            return prev
+        G, ns, out_ptr, out_ld, arg = pool
+        check(lib.pvn3d_mt_pool_max(G, ns, _ld(self.c[-1]), self.c[-1], prev.data_ptr(), out_ptr, out_ld, arg.data_ptr(), st),
+              "mt_pool_max")
+        return None
+
+    def backward(self, dh, need_input_grad, pooled=None):
+        dev, rows = self.dev, self.rows
+        st = torch.cuda.current_stream(dev).cuda_stream
+        L = len(self.weights)
+        dws, dgs, dbs = [None] * L, [None] * L, [None] * L
+        if pooled is not None:
+            G, ns, dout_ptr, out_ld, arg = pooled
+            dh = torch.empty((rows, _ld(self.c[-1])), dtype=torch.bfloat16, device=dev)
+            check(lib.pvn3d_mt_pool_bwd(G, ns, _ld(self.c[-1]), self.c[-1], dout_ptr, out_ld, arg.data_ptr(), dh.data_ptr(),
+                                        st), "mt_pool_bwd")
+        for li in range(L - 1, -1, -1):
+            cout = self.c[li + 1]
+            ldo = _ld(cout)
+            x, codes, pitch, scales, mask = None, None, 0, None, None
+            kept, self.y[li] = self.y[li], None
+            if isinstance(kept, Saved8):
+                (codes, scales), (mean, rstd, mask) = kept.act._ptrs(), kept._ptrs()
+                pitch = kept.act.pitch
+            else:
+                x = kept[0].data_ptr()
+                mean, rstd = kept[1].data_ptr(), kept[1].data_ptr() + 4 * rows
+            dgb = torch.empty((2, cout), dtype=torch.float32, device=dev)
+            dy = torch.empty((rows, ldo), dtype=torch.bfloat16, device=dev)
+            wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(1, rows, cout)
+            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+            check(lib.pvn3d_layer_norm_grad(1, rows, cout, dh.data_ptr(), ldo, x, ldo, codes, pitch, scales, mask,
+                                            self.gammas[li].data_ptr(), self.betas[li].data_ptr(), mean, rstd, 1,
+                                            dy.data_ptr(), ldo, ldo, dgb[0].data_ptr(), dgb[1].data_ptr(), ws.data_ptr(),
+                                            wsb, st), "layer_norm_grad")
+            dgs[li], dbs[li] = dgb[0], dgb[1]
+            del kept
+            dws[li] = self._weight_grad(li, dy, st)
+            self.inputs[li] = None
+            dh = self._input_grad(li, dy, st) if li > 0 or need_input_grad else None
+        return dh, dws, dgs, dbs
+
+
+def _chain(x0, c_in, weights, gammas, betas, layers):
+    return (_LNChain if _is_ln(layers) else _Chain)(x0, c_in, weights, gammas, betas, [norm for _, norm in layers])
 
 
 # Backward of the layer-0 gathers through inverted index lists (csrc/mlp_train.hip mt_csr_build / mt_inv_gather)
@@ -285,7 +418,8 @@ class SALevelTrain(torch.autograd.Function):
                 check(lib.pvn3d_mt_gather_sa(B, N, m, ns, C, 1 if use_xyz else 0, xyz.data_ptr(), new_xyz.data_ptr(), fp,
                                              fsb, fsc, fsn, idx.data_ptr(), x0.data_ptr(), _ld(c0), _stream(xyz)),
                       "mt_gather_sa")
-                ch = _Chain(x0, c0, ws, gs, bs, [bn for _, bn in layers])
+                ch = _chain(x0, c0, ws, gs, bs, layers)
+                del x0
                 arg = torch.empty((B * m, _ld(width)), dtype=torch.uint8, device=dev)
                 ch.forward(pool=(B * m, ns, out.data_ptr() + 4 * off, total, arg))
                 chains.append(ch)
@@ -359,7 +493,8 @@ class FPTrain(torch.autograd.Function):
             up, usb, usc, usn = _strides3(uf) if uf is not None else (None, 0, 0, 0)
             check(lib.pvn3d_mt_gather_fp(B, n, mk, C2, C1, kp, ksb, ksc, ksn, up, usb, usc, usn, idx.data_ptr(),
                                          weight.data_ptr(), x0.data_ptr(), _ld(c0), st), "mt_gather_fp")
-            ch = _Chain(x0, c0, ws, gs, bs, [bn for _, bn in layers])
+            ch = _chain(x0, c0, ws, gs, bs, layers)
+            del x0
             h = ch.forward()
             cout = ch.c[-1]
             if channel_major:        # the reference's contiguous (B, C_out, n)
@@ -426,7 +561,7 @@ def sa_level_train(module, xyz, new_xyz, features, idxs):
         layers = shared_mlp_layers(mlp)
         if layers is None or not isinstance(grouper, pointnet2_utils.QueryAndGroup) or idx is None:
             return None
-        if idx.size(2) > MAX_NSAMPLE or max([c_feat + 3] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16:
+        if idx.size(2) > (MAX_NSAMPLE_LN if _is_ln(layers) else MAX_NSAMPLE) or max([c_feat + 3] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16:
             return None
         if features is None and not grouper.use_xyz:
             return None

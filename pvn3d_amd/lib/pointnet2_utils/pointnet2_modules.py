@@ -51,6 +51,12 @@ def _stage(name):
     return hook(name) if hook is not None else _NULL_STAGE
 
 
+def _shared_mlp(spec, bn, norm):
+    if norm not in ("batch", "layer"):
+        raise ValueError("norm must be \"batch\" or \"layer\", not %r" % (norm,))
+    return pt_utils.SharedMLP(spec, bn=bn and norm == "batch", ln=norm == "layer")
+
+
 def _no_grad_needed(*tensors):
     if not torch.is_grad_enabled():
         return True
@@ -242,9 +248,10 @@ class PointnetSAModuleMSG(_PointnetSAModuleBase):
 
     npoint: number of sampled centres; radii / nsamples / mlps: one entry per scale;
     ``mlps[i][0]`` is increased by 3 in place when use_xyz (reference :108-109).
+    norm: "batch" (the reference's; `bn` says whether there is one) or "layer" (a layer norm over each point's channels).
     """
 
-    def __init__(self, npoint, radii, nsamples, mlps, bn=True, use_xyz=True):
+    def __init__(self, npoint, radii, nsamples, mlps, bn=True, use_xyz=True, norm="batch"):
         super(PointnetSAModuleMSG, self).__init__()
         assert len(radii) == len(nsamples) == len(mlps)
         self.npoint = npoint
@@ -256,23 +263,23 @@ class PointnetSAModuleMSG(_PointnetSAModuleBase):
                 if npoint is not None else pointnet2_utils.GroupAll(use_xyz))
             if use_xyz:
                 spec[0] += 3
-            self.mlps.append(pt_utils.SharedMLP(spec, bn=bn))
+            self.mlps.append(_shared_mlp(spec, bn, norm))
 
 
 class PointnetSAModule(PointnetSAModuleMSG):
     """Single-scale set abstraction (one radius / nsample / mlp)."""
 
-    def __init__(self, mlp, npoint=None, radius=None, nsample=None, bn=True, use_xyz=True):
+    def __init__(self, mlp, npoint=None, radius=None, nsample=None, bn=True, use_xyz=True, norm="batch"):
         super(PointnetSAModule, self).__init__(
-            mlps=[mlp], npoint=npoint, radii=[radius], nsamples=[nsample], bn=bn, use_xyz=use_xyz)
+            mlps=[mlp], npoint=npoint, radii=[radius], nsamples=[nsample], bn=bn, use_xyz=use_xyz, norm=norm)
 
 
 class PointnetFPModule(nn.Module):
-    """Feature propagation: inverse-distance interpolation from `known` to `unknown`, then MLP."""
+    """Feature propagation: inverse-distance interpolation from `known` to `unknown`, then MLP (norm: as above)."""
 
-    def __init__(self, mlp, bn=True):
+    def __init__(self, mlp, bn=True, norm="batch"):
         super(PointnetFPModule, self).__init__()
-        self.mlp = pt_utils.SharedMLP(mlp, bn=bn)
+        self.mlp = _shared_mlp(mlp, bn, norm)
 
     @staticmethod
     def neighbours(unknown, known):

@@ -36,10 +36,10 @@ class PointVoteNet(nn.Module):
     """Pointnet2MSG backbone + per-point keypoint-offset and centre-offset heads.
     forward(pointcloud (B, N, 3 + C)) -> pred_kp_of (B, K, N, 3), pred_ctr_of (B, 1, N, 3)."""
 
-    def __init__(self, input_channels=6, n_kps=8, width=128):
+    def __init__(self, input_channels=6, n_kps=8, width=128, norm="batch"):
         super(PointVoteNet, self).__init__()
         self.n_kps = n_kps
-        self.backbone = Pointnet2MSG(input_channels=input_channels)
+        self.backbone = Pointnet2MSG(input_channels=input_channels, norm=norm)
         self.kp_head = nn.Sequential(nn.Conv1d(128, width, 1), nn.BatchNorm1d(width), nn.ReLU(inplace=True),
                                      nn.Conv1d(width, n_kps * 3, 1))
         self.ctr_head = nn.Sequential(nn.Conv1d(128, width, 1), nn.BatchNorm1d(width), nn.ReLU(inplace=True),
