@@ -16,71 +16,110 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------------------------------------------ pack / unpack
-// tpr threads across a row (a power of two that covers whole groups or the row), 256 / tpr rows per workgroup.  Chunks are
-// windows (rowvec.h); a row shorter than one is read value by value.
-template <typename T>
-__device__ __forceinline__ void load_any(const T* __restrict__ row, int at, int C, float (&v)[traits<T>::VEC]) {
-  constexpr int VEC = traits<T>::VEC;
-  if (C >= VEC) {
-    rv::load_vec<T>(row + at, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(row + i) : 0.f;
-  }
-}
+// tpr threads across a row (a power of two that covers the row, or whole groups of it), 256 / tpr rows a pass and two passes
+// in flight.  Chunks are windows (rowvec.h), addresses a base the workgroup shares plus a 32-bit offset; a row shorter than a
+// chunk is read value by value.  LPG: lanes per group, fewer than a whole group's if the row is shorter.
+constexpr int FLY = 2;
 
-template <typename T>
-__global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, int tpr, const T* __restrict__ x,
-                                                        long long xs, signed char* __restrict__ codes, long long pitch,
+template <typename T, int LPG>
+__global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, int tpr, const T* __restrict__ x, int xs,
+                                                        signed char* __restrict__ codes, int pitch,
                                                         unsigned char* __restrict__ scales) {
-  constexpr int VEC = traits<T>::VEC, LPG = rv::GROUP / VEC;
+  constexpr int VEC = traits<T>::VEC;
   const int t = threadIdx.x & (tpr - 1), rg = threadIdx.x / tpr, rpb = 256 / tpr;
-  const int G = (C + rv::GROUP - 1) / rv::GROUP;
-  for (long long row = (long long)blockIdx.x * rpb + rg; row < rows; row += (long long)gridDim.x * rpb) {
-    for (int c = t * VEC; c < G * rv::GROUP; c += tpr * VEC) {      // whole groups: every lane of one takes part
+  const int G = (C + rv::GROUP - 1) / rv::GROUP, across = (C + LPG * VEC - 1) / (LPG * VEC) * (LPG * VEC);
+  for (long long base = (long long)blockIdx.x * rpb * FLY; base < rows; base += (long long)gridDim.x * rpb * FLY) {
+    const int last = (int)(rows - 1 - base < rpb * FLY - 1 ? rows - 1 - base : rpb * FLY - 1);
+    const T* const xb = x + base * xs;
+    signed char* const cb = codes + base * pitch;
+    unsigned char* const sb = scales + base * G;
+    for (int c = t * VEC; c < across; c += tpr * VEC) {             // whole groups: every lane of one takes part
       const int at = C >= VEC ? min(c, C - VEC) : 0, skip = C >= VEC ? min(c - at, VEC) : (c ? VEC : 0);
-      float v[VEC];
-      load_any<T>(x + row * xs, at, C, v);
-      unsigned big = 0, wd[VEC / 4];
+      rv::u4_any raw[FLY];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {                               // as integers: NaN is the largest
-        const unsigned a = __float_as_uint(v[i]) & 0x7fffffffu;
-        big = max(big, i >= skip ? a : 0u);
+      for (int r = 0; r < FLY; ++r) {
+        const T* const p = rv::at32(xb, (__umul24(min(rg + r * rpb, last), xs) + at) * (unsigned)sizeof(T));
+        if (C >= VEC) {
+          raw[r] = *reinterpret_cast<const rv::u4_any*>(p);
+        } else {
+          float v[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(p + i) : 0.f;
+          raw[r] = traits<T>::pack(v);
+        }
       }
-      const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
-      rv::group_codes<VEC>(v, sc, wd);
-      if (c < C) rv::store_codes(codes + row * pitch + c, skip, wd);
-      if ((c & (rv::GROUP - 1)) == 0) scales[row * G + c / rv::GROUP] = (unsigned char)sc;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < FLY; ++r) {
+        const int rl = rg + r * rpb;
+        float v[VEC];
+        traits<T>::unpack(raw[r], v);
+        unsigned big = 0, wd[VEC / 4];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {                             // as integers: NaN is the largest
+          const unsigned a = __float_as_uint(v[i]) & 0x7fffffffu;
+          big = max(big, i >= skip ? a : 0u);
+        }
+        const unsigned sc = rv::group_scale(rv::lanes_max<LPG>(big));
+        rv::group_codes<VEC>(v, sc, wd);
+        if (rl <= last && c < C) {
+          rv::store_codes(rv::at32(cb, __umul24(rl, pitch) + c), skip, wd);
+          if ((c & (rv::GROUP - 1)) == 0) *rv::at32(sb, __umul24(rl, G) + c / rv::GROUP) = (unsigned char)sc;
+        }
+      }
     }
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C, int tpr, const signed char* __restrict__ codes,
-                                                          long long pitch, const unsigned char* __restrict__ scales,
-                                                          T* __restrict__ y, long long ys, int ycols) {
+                                                          int pitch, const unsigned char* __restrict__ scales,
+                                                          T* __restrict__ y, int ys, int ycols) {
   constexpr int VEC = traits<T>::VEC;
   const int t = threadIdx.x & (tpr - 1), rg = threadIdx.x / tpr, rpb = 256 / tpr;
   const int G = (C + rv::GROUP - 1) / rv::GROUP;
-  for (long long row = (long long)blockIdx.x * rpb + rg; row < rows; row += (long long)gridDim.x * rpb) {
+  for (long long base = (long long)blockIdx.x * rpb * FLY; base < rows; base += (long long)gridDim.x * rpb * FLY) {
+    const int last = (int)(rows - 1 - base < rpb * FLY - 1 ? rows - 1 - base : rpb * FLY - 1);
+    const signed char* const cb = codes + base * pitch;
+    const unsigned char* const sb = scales + base * G;
+    T* const yb = y + base * ys;
     for (int c = t * VEC; c < C; c += tpr * VEC) {
       const int at = C >= VEC ? min(c, C - VEC) : 0, skip = c - at;
-      unsigned wd[VEC / 4];
-      rv::load_codes(codes + row * pitch + at, wd);
-      const float s1 = rv::group_step(scales[row * G + c / rv::GROUP]), s0 = rv::group_step(scales[row * G + at / rv::GROUP]);
-      float v[VEC];
+      unsigned wd[FLY][VEC / 4];
+      unsigned char s0[FLY], s1[FLY];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = rv::code_at(wd, i) * (i < skip ? s0 : s1);
-      if (C >= VEC) {
-        rv::store_vec<T>(y + row * ys + at, v);
-      } else {
+      for (int r = 0; r < FLY; ++r) {
+        const int rl = min(rg + r * rpb, last);
+        rv::load_codes(rv::at32(cb, __umul24(rl, pitch) + at), wd[r]);
+        s1[r] = *rv::at32(sb, __umul24(rl, G) + c / rv::GROUP);
+        s0[r] = *rv::at32(sb, __umul24(rl, G) + at / rv::GROUP);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (i < C) traits<T>::store1(y + row * ys + i, v[i]);
+      for (int r = 0; r < FLY; ++r) {
+        const int rl = rg + r * rpb;
+        const float f1 = rv::group_step(s1[r]), f0 = rv::group_step(s0[r]);
+        float v[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = rv::code_at(wd[r], i) * (i < skip ? f0 : f1);
+        if (rl <= last) {
+          T* const p = rv::at32(yb, (__umul24(rl, ys) + at) * (unsigned)sizeof(T));
+          if (C >= VEC) {
+            rv::store_vec<T>(p, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              if (i < C) traits<T>::store1(p + i, v[i]);
+          }
+        }
       }
     }
-    if (ycols > C)
-      for (int c = C + t; c < ycols; c += tpr) traits<T>::store1(y + row * ys + c, 0.f);
+    if (ycols > C) {
+      for (int rl = rg; rl <= last; rl += rpb)
+#pragma unroll 1
+        for (int c = C + t; c < ycols; c += tpr)
+          traits<T>::store1(rv::at32(yb, (__umul24(rl, ys) + c) * (unsigned)sizeof(T)), 0.f);
+    }
   }
 }
 
@@ -356,10 +395,12 @@ wg_plan wgrad_plan(long long rows, int M, int N) {
   int step = 32, wgs = 768, per = 16;                            // per: steps a workgroup should have at least
   if (M > 128 && N > 64) { p.kind = 0; p.tm = 256; p.tn = 128; step = 64; wgs = 256; per = 4; }
   else if (M > 64 && N > 64) { p.kind = 1; p.tm = 128; p.tn = 128; step = 64; wgs = 512; per = 4; }
-  else if (M > 32 && N > 32) { p.kind = 2; p.tm = 64; p.tn = 64; }
-  else if (M > 32) { p.kind = 3; p.tm = 64; p.tn = 32; }
-  else if (N > 32) { p.kind = 4; p.tm = 32; p.tn = 64; }
-  else { p.kind = 5; p.tm = 32; p.tn = 32; }
+  else if (M > 32 && N > 64) { p.kind = 2; p.tm = 64; p.tn = 128; step = 64; wgs = 512; per = 4; }
+  else if (M > 64 && N > 32) { p.kind = 3; p.tm = 128; p.tn = 64; step = 64; wgs = 512; per = 4; }
+  else if (M > 32 && N > 32) { p.kind = 4; p.tm = 64; p.tn = 64; }
+  else if (M > 32) { p.kind = 5; p.tm = 64; p.tn = 32; }
+  else if (N > 32) { p.kind = 6; p.tm = 32; p.tn = 64; }
+  else { p.kind = 7; p.tm = 32; p.tn = 32; }
   const long long tiles = (long long)pvn3d_ceil_div(M, p.tm) * pvn3d_ceil_div(N, p.tn);
   const long long steps = (rows + step - 1) / step;
   long long S = wgs / tiles;
@@ -368,35 +409,43 @@ wg_plan wgrad_plan(long long rows, int M, int N) {
   return p;
 }
 
-constexpr long long MAX_STRIDE = 1 << 20;      // a step's rows are within 32-bit offsets of its base
+constexpr long long MAX_STRIDE = 1 << 20;      // a workgroup's rows are within 32-bit offsets of their base
 constexpr long long MAX_ROWS = 1ll << 35;      // steps are counted in 32 bits
 
 #define A8_ST ((hipStream_t)stream)
 
-int pack_threads(int C, int vec) {
-  int t = 32 / vec;                                              // a whole group at least
+int row_threads(int C, int vec) {                                // threads across a row
+  int t = 1;
   while (t < 64 && t * vec < C) t <<= 1;
   return t;
 }
 unsigned row_grid(long long rows, int tpr) {
-  const long long n = (rows + 256 / tpr - 1) / (256 / tpr);
-  return (unsigned)(n < 8192 ? n : 8192);
+  const int per = 256 / tpr * FLY;
+  const long long n = (rows + per - 1) / per;
+  return (unsigned)(n < 16384 ? n : 16384);
 }
 
 template <typename T>
 int run_pack(long long rows, int C, const void* x, long long xs, void* codes, long long pitch, void* scales, hipStream_t st) {
-  const int tpr = pack_threads(C, traits<T>::VEC);
-  hipLaunchKernelGGL((act8_pack_kernel<T>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr, (const T*)x, xs,
-                     (signed char*)codes, pitch, (unsigned char*)scales);
+  const int tpr = row_threads(C, traits<T>::VEC);
+#define A8_PACK(LPG)                                                                                                        \
+  hipLaunchKernelGGL((act8_pack_kernel<T, LPG>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr, (const T*)x,    \
+                     (int)xs, (signed char*)codes, (int)pitch, (unsigned char*)scales)
+  const int lpg = tpr < rv::GROUP / traits<T>::VEC ? tpr : rv::GROUP / traits<T>::VEC;
+  if (lpg == 1) A8_PACK(1);
+  else if (lpg == 2) A8_PACK(2);
+  else if (lpg == 4) A8_PACK(4);
+  else A8_PACK((traits<T>::VEC == 4 ? 8 : 4));
+#undef A8_PACK
   PVN3D_LAUNCH_CHECK();
   return 0;
 }
 template <typename T>
 int run_unpack(long long rows, int C, const void* codes, long long pitch, const void* scales, void* y, long long ys, int ycols,
                hipStream_t st) {
-  const int tpr = pack_threads(ycols, traits<T>::VEC);
+  const int tpr = row_threads(C, traits<T>::VEC);
   hipLaunchKernelGGL((act8_unpack_kernel<T>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr,
-                     (const signed char*)codes, pitch, (const unsigned char*)scales, (T*)y, ys, ycols);
+                     (const signed char*)codes, (int)pitch, (const unsigned char*)scales, (T*)y, (int)ys, ycols);
   PVN3D_LAUNCH_CHECK();
   return 0;
 }
@@ -405,7 +454,8 @@ int run_unpack(long long rows, int C, const void* codes, long long pitch, const 
 
 extern "C" int pvn3d_act8_pack(int dtype, long long rows, int C, const void* x, long long xs, void* codes, long long pitch,
                                void* scales, void* stream) {
-  if (dtype < 0 || dtype > 2 || C <= 0 || xs < 0 || (pitch & 15) || pitch < C) return (int)hipErrorInvalidValue;
+  if (dtype < 0 || dtype > 2 || C <= 0 || xs < 0 || (pitch & 15) || pitch < C || xs > MAX_STRIDE || pitch > MAX_STRIDE)
+    return (int)hipErrorInvalidValue;
   if (rows <= 0) return 0;
   if (!x || !codes || !scales) return (int)hipErrorInvalidValue;
   switch (dtype) {
@@ -417,7 +467,8 @@ extern "C" int pvn3d_act8_pack(int dtype, long long rows, int C, const void* x, 
 
 extern "C" int pvn3d_act8_unpack(int dtype, long long rows, int C, const void* codes, long long pitch, const void* scales,
                                  void* y, long long ys, int y_cols, void* stream) {
-  if (dtype < 0 || dtype > 2 || C <= 0 || (pitch & 15) || pitch < C || y_cols < C || ys < y_cols)
+  if (dtype < 0 || dtype > 2 || C <= 0 || (pitch & 15) || pitch < C || y_cols < C || ys < y_cols || ys > MAX_STRIDE ||
+      pitch > MAX_STRIDE)
     return (int)hipErrorInvalidValue;
   if (rows <= 0) return 0;
   if (!codes || !scales || !y) return (int)hipErrorInvalidValue;
@@ -466,9 +517,11 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
   switch (p.kind) {
     case 0: A8_CALL(2, 2, 4, 2, 64); break;
     case 1: A8_CALL(2, 2, 2, 2, 64); break;
-    case 2: A8_CALL(2, 2, 1, 1, 32); break;
-    case 3: A8_CALL(2, 1, 1, 1, 32); break;
-    case 4: A8_CALL(1, 2, 1, 1, 32); break;
+    case 2: A8_CALL(1, 2, 2, 2, 64); break;
+    case 3: A8_CALL(2, 1, 2, 2, 64); break;
+    case 4: A8_CALL(2, 2, 1, 1, 32); break;
+    case 5: A8_CALL(2, 1, 1, 1, 32); break;
+    case 6: A8_CALL(1, 2, 1, 1, 32); break;
     default: A8_CALL(1, 1, 1, 1, 32); break;
   }
 #undef A8_ONE

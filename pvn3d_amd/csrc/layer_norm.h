@@ -91,12 +91,12 @@ struct lane_cols {
 
 inline int vec_of(int dtype) { return dtype == 0 ? 4 : 8; }
 
-// threads per row: the power of two whose chunks cover it, 64 at most; a workgroup where four chunks a lane do not
+// threads per row: the power of two whose chunks cover it, 64 at most with up to two chunks each; beyond that a workgroup
 inline int rows_threads(int C, int vec) {
   const int chunks = (C + vec - 1) / vec;
   int t = 1;
   while (t < chunks && t < 64) t <<= 1;
-  return chunks > 4 * 64 ? 256 : t;
+  return chunks > 2 * 64 ? 256 : t;
 }
 inline long long rows_blocks(long long rows, int tpr, int r) {
   const long long per = (long long)(256 / tpr) * r;
@@ -116,8 +116,9 @@ inline long long rows_blocks(long long rows, int tpr, int r) {
     else if (tpr__ == 16) CALL(T, 16, 1, 2);                              \
     else if (tpr__ == 32) CALL(T, 32, 1, 2);                              \
     else if (tpr__ == 64 && k__ == 1) CALL(T, 64, 1, 2);                  \
-    else if (tpr__ == 64 && k__ == 2) CALL(T, 64, 2, 1);                  \
-    else if (tpr__ == 64) CALL(T, 64, 4, 1);                              \
+    else if (tpr__ == 64) CALL(T, 64, 2, 1);                              \
+    else if (k__ == 1) CALL(T, 256, 1, 2);                                \
+    else if (k__ == 2) CALL(T, 256, 2, 1);                                \
     else if (vec__ == 8 || k__ <= 4) CALL(T, 256, 4, 1);                  \
     else CALL(T, 256, (vec__ == 8 ? 4 : 8), 1);                           \
   } while (0)

@@ -1,7 +1,7 @@
 // layer_norm_chan.hip -- layer norm over the channels of (B, C, M) tensors, M contiguous: the layout in which the modules
 // hand features on.  The formulas are those of layer_norm.hip.
 //
-// A tile is 64 consecutive points of one cloud: 16 lanes x 4 points across, blockDim.x / 16 channel slots down.  A thread
+// A tile is 64 (32) consecutive points of one cloud: PX = 16 (8) lanes x 4 points across, blockDim.x / PX channel slots down.  A thread
 // holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
 // is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
 // every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
@@ -56,12 +56,13 @@ __device__ __forceinline__ void forget<float>(raw4<float>& a) {
 // Chunks are whole and unconditional: the last, partial one of a row of points is taken as its last four points, which
 // overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.  Lanes behind the
 // cloud's last point repeat its last four without a store.
+template <int PX>
 struct tile_at {
   int b, m0, skip;
   bool live;
   __device__ __forceinline__ tile_at(int tile, int per_cloud, int M) {
     b = tile / per_cloud;
-    const int m = ((tile - b * per_cloud) * 16 + (threadIdx.x & 15)) * PTS;
+    const int m = ((tile - b * per_cloud) * PX + (threadIdx.x & (PX - 1))) * PTS;
     live = m < M;
     m0 = min(m, M - PTS);
     skip = m - m0;
@@ -69,12 +70,15 @@ struct tile_at {
 };
 
 // s[i] -> sum over the workgroup's channel slots of s[i], for the thread's own points
-template <int N>
-__device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[16 * N]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane & 15, waves = blockDim.x >> 6;
+template <int N, int PX>
+__device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[PX * N]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane & (PX - 1), waves = blockDim.x >> 6;
 #pragma unroll
-  for (int i = 0; i < N; ++i) s[i] = rv::add32(rv::add16(s[i]));
-  if (lane < 16) {
+  for (int i = 0; i < N; ++i) {
+    if (PX == 8) s[i] += __uint_as_float(rv::turn8(__float_as_uint(s[i])));
+    s[i] = rv::add32(rv::add16(s[i]));
+  }
+  if (lane < PX) {
 #pragma unroll
     for (int i = 0; i < N; ++i) buf[wave][px * N + i] = s[i];
   }
@@ -86,14 +90,14 @@ __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[16 * N]) {
     for (int i = 0; i < N; ++i) s[i] += buf[wv][px * N + i];
 }
 
-template <typename T, int KC>
+template <typename T, int KC, int PX>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per_cloud, int C, int M, const T* __restrict__ x,
                                                               const float* __restrict__ w, const float* __restrict__ b,
                                                               float eps, int relu, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int KR = KC > 0 ? KC : 1;
-  __shared__ float buf[2][MAX_THREADS / 64][16 * PTS];
-  const int cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
+  __shared__ float buf[2][MAX_THREADS / 64][PX * PTS];
+  const int cy = threadIdx.x / PX, CY = blockDim.x / PX;
   const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
   const float rc = 1.f / (float)C;
   float low = relu ? 0.f : -__builtin_inff();
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
   }
   const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const tile_at at(tile, per_cloud, M);
+    const tile_at<PX> at(tile, per_cloud, M);
     const T* const p = x + at.b * C * M_;
     T* const q = y + at.b * C * M_;
     const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
@@ -143,14 +147,14 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
 #pragma unroll
       for (int i = 0; i < PTS; ++i) s[i] += v[i];
     });
-    slot_sum<PTS>(s, buf[0]);
+    slot_sum<PTS, PX>(s, buf[0]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) { mu[i] = s[i] * rc; s[i] = 0.f; }
     each([&](int, size_t, int, const float (&v)[PTS]) {
 #pragma unroll
       for (int i = 0; i < PTS; ++i) s[i] = fmaf(v[i] - mu[i], v[i] - mu[i], s[i]);
     });
-    slot_sum<PTS>(s, buf[1]);
+    slot_sum<PTS, PX>(s, buf[1]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) rs[i] = __builtin_amdgcn_rsqf(fmaf(s[i], rc, eps));       // v_rsq_f32: within one ulp
     if (at.live && cy == 0) {
@@ -173,17 +177,18 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
 
 // dw / db: a thread has the same channels for all its tiles: a register each, summed over the 16 lanes at the end (KC = 0:
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
-template <typename T, int KC>
+template <typename T, int KC, int PX>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int per_cloud, int C, int M,
                                                                    const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ w,
                                                                    const float* __restrict__ b,
                                                                    const float* __restrict__ mean,
                                                                    const float* __restrict__ rstd, int relu,
-                                                                   T* __restrict__ dx, float* __restrict__ part) {
+                                                                   T* __restrict__ dx, float* __restrict__ part_w,
+                                                                   float* __restrict__ part_b, size_t part_stride) {
   constexpr int KR = KC > 0 ? KC : 1;
-  __shared__ float buf[2][MAX_THREADS / 64][16 * 2 * PTS];
+  __shared__ float buf[2][MAX_THREADS / 64][PX * 2 * PTS];
   extern __shared__ float lacc[];
-  const int px = threadIdx.x & 15, cy = threadIdx.x >> 4, CY = blockDim.x >> 4;
+  const int px = threadIdx.x & (PX - 1), cy = threadIdx.x / PX, CY = blockDim.x / PX;
   const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
   const float rc = 1.f / (float)C;
   float aw[KR], ab[KR], gk[KR], bk[KR];
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
   }
   int turn = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-    const tile_at at(tile, per_cloud, M);
+    const tile_at<PX> at(tile, per_cloud, M);
     const T* const px_ = x + at.b * C * M_;
     const T* const pd_ = dy + at.b * C * M_;
     T* const po_ = dx + at.b * C * M_;
@@ -277,8 +282,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
         open<T>(*reinterpret_cast<const raw4<T>*>(rv::at32(pd_ + at_c, o)), d);
         one(w ? w[c] : 1.f, b ? b[c] : 0.f, v, d);
         add(w ? w[c] : 1.f, v, d, w1, b1);
-        w1 = rv::lanes_sum<16>(w1);
-        b1 = rv::lanes_sum<16>(b1);
+        w1 = rv::lanes_sum<PX>(w1);
+        b1 = rv::lanes_sum<PX>(b1);
         if (px == 0) {                                 // the one thread that adds to this channel's words
           lacc[c] += w1;
           lacc[C + c] += b1;
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
       }
     }
     if (!dx) continue;
-    slot_sum<2 * PTS>(s, buf[turn]);
+    slot_sum<2 * PTS, PX>(s, buf[turn]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) {
       s[i] *= -rc * rs[i];
@@ -316,75 +321,88 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
       }
     }
   }
-  if (!part) return;
-  float* const pw = part + (size_t)blockIdx.x * 2 * C;
+  if (!part_w) return;
+  float* const pw = part_w + blockIdx.x * part_stride;
+  float* const pb = part_b + blockIdx.x * part_stride;
   if (KC > 0) {
 #pragma unroll
     for (int k = 0; k < KR; ++k) {
-      aw[k] = rv::lanes_sum<16>(aw[k]);
-      ab[k] = rv::lanes_sum<16>(ab[k]);
+      aw[k] = rv::lanes_sum<PX>(aw[k]);
+      ab[k] = rv::lanes_sum<PX>(ab[k]);
       const int c = cy + k * CY;
       if (px == 0 && has[k]) {
         pw[c] = aw[k];
-        pw[C + c] = ab[k];
+        pb[c] = ab[k];
       }
     }
   } else {
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * C; c += blockDim.x) pw[c] = lacc[c];
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      pw[c] = lacc[c];
+      pb[c] = lacc[C + c];
+    }
   }
 }
 
-// threads and channels per thread: 16 slots up to 128 channels, then eight channels a slot while 64 slots do (8 x 196 x
-// 16384 in bf16, backward: 39.5 us; with six channels a slot and more slots 51.4, with four 52.9)
-void chan_shape(int C, int& threads, int& kc) {
+// lanes across, threads and channels per thread: 16 lanes and 16 channel slots up to 128 channels, then eight channels a
+// slot (8 x 196 x 16384 in bf16, backward: 39.5 us; with six channels a slot and more slots 51.4, with four 52.9); from 257
+// channels 8 lanes, so that two workgroups of them still share a CU; beyond 1024 channels x is read again for every pass
+struct chan_plan { int px, threads, kc; };
+chan_plan chan_shape(int C) {
+  chan_plan p;
+  p.px = C > 256 && C <= 1024 ? 8 : 16;
   int cy = 16;
-  if (C > 128) cy = (C + 31) / 32 * 4;
-  if (cy > 64) cy = 64;
-  threads = cy * 16;
-  kc = (C + cy - 1) / cy;
-  if (kc > 8) kc = 0;
+  if (p.px == 8) cy = (C + 63) / 64 * 8;
+  else if (C > 1024) cy = 64;
+  else if (C > 128) cy = (C + 31) / 32 * 4;
+  p.threads = cy * p.px;
+  p.kc = C > 1024 ? 0 : (C + cy - 1) / cy;
+  return p;
 }
-int cloud_tiles(int M) { return (int)(((long long)M + 16 * PTS - 1) / (16 * PTS)); }
-long long chan_tiles(int B, int M) { return (long long)B * cloud_tiles(M); }
+int cloud_tiles(int C, int M) { return (int)(((long long)M + chan_shape(C).px * PTS - 1) / (chan_shape(C).px * PTS)); }
+long long chan_tiles(int B, int C, int M) { return (long long)B * cloud_tiles(C, M); }
 // workgroups of a backward launch: what is on the chip at once (every one starts with the parameters and ends with its
 // partial sums): by its registers 32 waves a CU with two or three channels a thread, 16 with more (one: 16 are
-// the faster, 24 x 16 x 65536 fp32 61 us against 72)
+// the faster, 24 x 16 x 65536 fp32 61 us against 72).  A few tiles are one workgroup's, which writes dw and db itself.
 int chan_grad_parts(int B, int C, int M) {
-  int threads, kc;
-  chan_shape(C, threads, kc);
-  const long long n = chan_tiles(B, M), most = 256 * (long long)((kc == 2 || kc == 3 ? 2048 : 1024) / threads);
-  return (int)(n < most ? n : most);
+  const chan_plan p = chan_shape(C);
+  const long long n = chan_tiles(B, C, M), most = 256 * (long long)((p.kc == 2 || p.kc == 3 ? 2048 : 1024) / p.threads);
+  return (int)(n <= 4 ? 1 : n < most ? n : most);
 }
 constexpr int MAX_POINTS = 1 << 24;        // per cloud: 64 channel slots of them are within 32-bit byte offsets
 bool chan_ok(int dtype, int B, int C, int M) {
   return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || (M >= PTS && M <= MAX_POINTS)) &&
-         chan_tiles(B, M) < 0x7fffffffLL - 16384;
+         chan_tiles(B, C, M) < 0x7fffffffLL - 16384;
 }
 
-#define LN_CHAN_PICK(CALL)      \
-  switch (kc) {                 \
-    case 1: CALL(1); break;     \
-    case 2: CALL(2); break;     \
-    case 3: CALL(3); break;     \
-    case 4: CALL(4); break;     \
-    case 5: CALL(5); break;     \
-    case 6: CALL(6); break;     \
-    case 7: CALL(7); break;     \
-    case 8: CALL(8); break;     \
-    default: CALL(0); break;    \
+// (8 lanes: seven or eight channels a slot come of 257 to 1024 channels)
+#define LN_CHAN_PICK(CALL)                          \
+  if (p.px == 8) {                                  \
+    if (p.kc <= 7) CALL(7, 8);                      \
+    else CALL(8, 8);                                \
+  } else {                                          \
+    switch (p.kc) {                                 \
+      case 1: CALL(1, 16); break;                   \
+      case 2: CALL(2, 16); break;                   \
+      case 3: CALL(3, 16); break;                   \
+      case 4: CALL(4, 16); break;                   \
+      case 5: CALL(5, 16); break;                   \
+      case 6: CALL(6, 16); break;                   \
+      case 7: CALL(7, 16); break;                   \
+      case 8: CALL(8, 16); break;                   \
+      default: CALL(0, 16); break;                  \
+    }                                               \
   }
 
 template <typename T>
 int chan_forward(int B, int C, int M, const void* x, const float* w, const float* b, float eps, int relu, void* y,
                  float* mean, float* rstd, hipStream_t st) {
-  int threads, kc;
-  chan_shape(C, threads, kc);
-  const long long tiles = chan_tiles(B, M);
+  const chan_plan p = chan_shape(C);
+  const long long tiles = chan_tiles(B, C, M);
   const dim3 grid((unsigned)(tiles < 8192 ? tiles : 8192));
-#define LN_CALL(KC)                                                                                                       \
-  hipLaunchKernelGGL((ln_chan_kernel<T, KC>), grid, dim3(threads), 0, st, (int)tiles, cloud_tiles(M), C, M, (const T*)x, w, \
-                     b, eps, relu, (T*)y, mean, rstd)
+#define LN_CALL(KC, PX)                                                                                                     \
+  hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX>), grid, dim3(p.threads), 0, st, (int)tiles, cloud_tiles(C, M), C, M,        \
+                     (const T*)x, w, b, eps, relu, (T*)y, mean, rstd)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
@@ -393,17 +411,16 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
 
 template <typename T>
 int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x, const float* w, const float* b,
-                  const float* mean, const float* rstd, int relu, void* dx, float* part, hipStream_t st) {
-  int threads, kc;
-  chan_shape(C, threads, kc);
-  const int lds = kc ? 0 : (int)(2 * C * sizeof(float));
-  if (!kc) {
-    const int rc = pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0>);
+                  const float* mean, const float* rstd, int relu, void* dx, float* pw, float* pb, size_t ps, hipStream_t st) {
+  const chan_plan p = chan_shape(C);
+  const int lds = p.kc ? 0 : (int)(2 * C * sizeof(float));
+  if (!p.kc) {
+    const int rc = pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16>);
     if (rc) return rc;
   }
-#define LN_CALL(KC)                                                                                                      \
-  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC>), dim3(parts), dim3(threads), lds, st, (int)chan_tiles(B, M),          \
-                     cloud_tiles(M), C, M, (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, part)
+#define LN_CALL(KC, PX)                                                                                                     \
+  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX>), dim3(parts), dim3(p.threads), lds, st, (int)chan_tiles(B, C, M),     \
+                     cloud_tiles(C, M), C, M, (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, pw, pb, ps)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
   PVN3D_LAUNCH_CHECK();
@@ -413,8 +430,9 @@ int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x,
 }  // namespace
 
 extern "C" size_t pvn3d_layer_norm_chan_grad_workspace_bytes(int dtype, int B, int C, int M) {
-  if (!chan_ok(dtype, B, C, M)) return 0;
-  return (size_t)chan_grad_parts(B, C, M) * 2 * C * sizeof(float);
+  if (!chan_ok(dtype, B, C, M) || B == 0 || M == 0) return 0;
+  const int parts = chan_grad_parts(B, C, M);
+  return parts > 1 ? (size_t)parts * 2 * C * sizeof(float) : 0;
 }
 
 extern "C" int pvn3d_layer_norm_chan(int dtype, int B, int C, int M, const void* x, const float* weight, const float* bias,
@@ -447,14 +465,18 @@ extern "C" int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const 
   }
   if (!dy || !x || !mean || !rstd) return (int)hipErrorInvalidValue;
   const int parts = chan_grad_parts(B, C, M);
-  if (dweight && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float))) return (int)hipErrorInvalidValue;
-  float* part = dweight ? (float*)workspace : nullptr;
+  if (dweight && parts > 1 && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
+    return (int)hipErrorInvalidValue;
+  float* const part = (float*)workspace;
+  float* const pw = !dweight ? nullptr : parts > 1 ? part : dweight;
+  float* const pb = !dweight ? nullptr : parts > 1 ? part + C : dbias;
+  const size_t ps = parts > 1 ? 2 * (size_t)C : 0;
   int rc;
   switch (dtype) {
-    case 0: rc = chan_backward<float>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, part, st); break;
-    case 1: rc = chan_backward<bf16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, part, st); break;
-    default: rc = chan_backward<fp16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, part, st); break;
+    case 0: rc = chan_backward<float>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
+    case 1: rc = chan_backward<bf16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
+    default: rc = chan_backward<fp16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
   }
-  if (rc || !dweight) return rc;
+  if (rc || !dweight || parts == 1) return rc;
   return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, st);
 }

@@ -21,7 +21,8 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
                                                            const float* __restrict__ w, const float* __restrict__ b,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                            int relu, T* __restrict__ dx, int dxs, int dxcols,
-                                                           float* __restrict__ part) {
+                                                           float* __restrict__ part_w, float* __restrict__ part_b,
+                                                           size_t part_stride) {
   constexpr int VEC = traits<T>::VEC;
   constexpr int RPB = 256 / TPR;
   constexpr int COLS = TPR * K * VEC;
@@ -129,8 +130,9 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       }
     }
   }
-  if (!part) return;
-  float* const pw = part + (size_t)blockIdx.x * 2 * C;
+  if (!part_w) return;
+  float* const pw = part_w + blockIdx.x * part_stride;
+  float* const pb = part_b + blockIdx.x * part_stride;
   if (TPR > 64) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       for (int i = 0; i < VEC; ++i)
         if (col.own[k][i] != 0.f) {
           pw[col.at[k] + i] = aw[k][i];
-          pw[C + col.at[k] + i] = ab[k][i];
+          pb[col.at[k] + i] = ab[k][i];
         }
     return;
   }
@@ -164,33 +166,34 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
     }
     __syncthreads();
     for (int c = threadIdx.x; c < C; c += 256)
-      pw[which * C + c] = (fold[c] + fold[COLS + c]) + (fold[2 * COLS + c] + fold[3 * COLS + c]);
+      (which ? pb : pw)[c] = (fold[c] + fold[COLS + c]) + (fold[2 * COLS + c] + fold[3 * COLS + c]);
   }
 }
 
-// workgroups of a rows backward launch = its partial sums
+// workgroups of a rows backward launch = its partial sums; a call of a few passes' rows is one workgroup's, which writes dw
+// and db itself (no second launch)
 int rows_grad_parts(int dtype, long long rows, int C) {
   const long long n = ln::rows_blocks(rows, ln::rows_threads(C, ln::vec_of(dtype)), 1);
-  return (int)(n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
+  return (int)(n <= 8 ? 1 : n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
 }
 
 template <typename T>
 int rows_backward(int parts, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
                   const void* codes, long long pitch, const void* scales, const void* mask, const float* w, const float* b,
-                  const float* mean, const float* rstd, int relu, void* dx, long long dxs, int dxcols, float* part,
-                  hipStream_t st) {
+                  const float* mean, const float* rstd, int relu, void* dx, long long dxs, int dxcols, float* pw, float* pb,
+                  size_t ps, hipStream_t st) {
 #define LN_CALL(T, TPR, K, R)                                                                                            \
   do {                                                                                                                   \
     if (codes)                                                                                                           \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, true>), dim3(parts), dim3(256), 0, st, rows, C,              \
                          (const T*)dy, (int)dys, (const T*)nullptr, 0, (const signed char*)codes, (int)pitch,                    \
                          (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, (int)dxs,  \
-                         dxcols, part);                                                                                  \
+                         dxcols, pw, pb, ps);                                                                               \
     else                                                                                                                 \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, false>), dim3(parts), dim3(256), 0, st, rows, C,             \
                          (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)nullptr, 0,                           \
                          (const unsigned char*)nullptr, (const unsigned char*)nullptr, w, b, mean, rstd, relu, (T*)dx,   \
-                         (int)dxs, dxcols, part);                                                                             \
+                         (int)dxs, dxcols, pw, pb, ps);                                                                          \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
@@ -202,7 +205,8 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
 
 extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C) {
   if (rows <= 0 || C <= 0 || C > ln::MAX_C || dtype < 0 || dtype > 2) return 0;
-  return (size_t)rows_grad_parts(dtype, rows, C) * 2 * C * sizeof(float);
+  const int parts = rows_grad_parts(dtype, rows, C);
+  return parts > 1 ? (size_t)parts * 2 * C * sizeof(float) : 0;
 }
 extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x,
                                      long long xs, const void* codes, long long pitch, const void* scales,
@@ -225,14 +229,18 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
   }
   if (!dy || (!x && !codes) || !mean || !rstd) return (int)hipErrorInvalidValue;
   const int parts = rows_grad_parts(dtype, rows, C);
-  if (dweight && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float))) return (int)hipErrorInvalidValue;
-  float* part = dweight ? (float*)workspace : nullptr;
+  if (dweight && parts > 1 && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
+    return (int)hipErrorInvalidValue;
+  float* const part = (float*)workspace;
+  float* const pw = !dweight ? nullptr : parts > 1 ? part : dweight;
+  float* const pb = !dweight ? nullptr : parts > 1 ? part + C : dbias;
+  const size_t ps = parts > 1 ? 2 * (size_t)C : 0;
   int rc;
   switch (dtype) {
-    case 0: rc = rows_backward<float>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, part, (hipStream_t)stream); break;
-    case 1: rc = rows_backward<bf16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, part, (hipStream_t)stream); break;
-    default: rc = rows_backward<fp16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, part, (hipStream_t)stream); break;
+    case 0: rc = rows_backward<float>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
+    case 1: rc = rows_backward<bf16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
+    default: rc = rows_backward<fp16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
   }
-  if (rc || !dweight) return rc;
+  if (rc || !dweight || parts == 1) return rc;
   return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, (hipStream_t)stream);
 }

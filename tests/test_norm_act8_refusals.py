@@ -20,10 +20,11 @@ def test_layer_norm_entry_points_refuse():
                                     a["mask"], None)
     for kw in (dict(dtype=3), dict(dtype=-1), dict(C=0), dict(C=8193), dict(yc=7), dict(yc=24), dict(ys=7), dict(xs=-1),
                dict(x=None), dict(y=None), dict(mean=None), dict(rstd=None), dict(codes=P, pitch=16),
-               dict(codes=P, scales=P, pitch=8), dict(codes=P, scales=P, pitch=0)):
+               dict(codes=P, scales=P, pitch=8), dict(codes=P, scales=P, pitch=0), dict(xs=(1 << 20) + 1),
+               dict(ys=(1 << 20) + 1)):
         assert call(**kw) != 0, kw
     assert call(rows=0) == 0
-    g = dict(dtype=1, rows=4, C=8, dy=P, dys=8, x=P, xs=8, codes=None, pitch=0, scales=None, mask=None, w=None, b=None, mean=P,
+    g = dict(dtype=1, rows=100000, C=8, dy=P, dys=8, x=P, xs=8, codes=None, pitch=0, scales=None, mask=None, w=None, b=None, mean=P,
              rstd=P, relu=0, dx=P, dxs=8, dxc=8, dw=P, db=P, ws=P, wsb=1 << 20)
 
     def grad(**kw):
@@ -36,16 +37,18 @@ def test_layer_norm_entry_points_refuse():
                dict(wsb=4), dict(codes=P, scales=P, pitch=16, relu=1), dict(codes=P, scales=P, pitch=16, mask=P),
                dict(codes=P, pitch=16), dict(codes=P, scales=P, pitch=4)):
         assert grad(**kw) != 0, kw
-    for kw in (dict(dtype=7), dict(B=-1), dict(C=0), dict(M=-1), dict(C=8200), dict(B=1 << 30, M=64)):
+    for kw in (dict(dtype=7), dict(B=-1), dict(C=0), dict(M=-1), dict(M=3), dict(M=(1 << 24) + 1), dict(C=8200),
+               dict(B=1 << 30, M=1 << 10)):
         a = dict(dict(dtype=0, B=2, C=8, M=4), **kw)
         assert lib.pvn3d_layer_norm_chan(a["dtype"], a["B"], a["C"], a["M"], P, None, None, 1e-5, 0, P, P, P, None) != 0
         assert lib.pvn3d_layer_norm_chan_grad(a["dtype"], a["B"], a["C"], a["M"], P, P, None, None, P, P, 0, P, P, P, P,
                                               1 << 20, None) != 0
-    assert lib.pvn3d_layer_norm_chan_grad(0, 2, 8, 4, P, P, None, None, P, P, 0, P, P, P, None, 0, None) != 0
+    assert lib.pvn3d_layer_norm_chan_grad(0, 200, 8, 400, P, P, None, None, P, P, 0, P, P, P, None, 0, None) != 0
     assert lib.pvn3d_layer_norm_chan(0, 0, 8, 4, P, None, None, 1e-5, 0, P, P, P, None) == 0
     # the workspace holds a partial dweight and dbias per workgroup
     assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 10 ** 6, 64) % (2 * 64 * 4) == 0
     assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 0, 64) == 0
+    assert lib.pvn3d_layer_norm_grad_workspace_bytes(1, 100, 64) == 0        # one workgroup: none
 
 
 def test_act8_entry_points_refuse():
