@@ -56,6 +56,26 @@ __device__ __forceinline__ void forget<float>(raw4<float>& a) {
 // Chunks are whole and unconditional: the last, partial one of a row of points is taken as its last four points, which
 // overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.  Lanes behind the
 // cloud's last point repeat its last four without a store.
+// Tiles of a workgroup: workgroups are dealt to the eight XCDs in turn, and neighbouring tiles share the cache lines that
+// their rows' ends lie in (all of them, in part, if M is odd), so each XCD -- its own L2 -- gets a run of tiles: XCD x
+// walks x per, x per + 1, ... with all its workgroups.  (Grids of fewer than eight, or no multiple of it: in turn.)
+struct tile_walk {
+  int at, step, end;
+  __device__ __forceinline__ explicit tile_walk(int tiles) {
+    const int g = gridDim.x, b = blockIdx.x;
+    if (g & 7) {
+      at = b;
+      step = g;
+      end = tiles;
+    } else {
+      const int per = (tiles + 7) >> 3, x = b & 7;
+      at = x * per + (b >> 3);
+      step = g >> 3;
+      end = min(tiles, (x + 1) * per);
+    }
+  }
+};
+
 template <int PX>
 struct tile_at {
   int b, m0, skip;
@@ -112,7 +132,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
     bk[k] = KC > 0 && b && has[k] ? b[c] : 0.f;
   }
   const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  const tile_walk walk(tiles);
+  for (int tile = walk.at; tile < walk.end; tile += walk.step) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const p = x + at.b * C * M_;
     T* const q = y + at.b * C * M_;
@@ -208,7 +229,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     __syncthreads();
   }
   int turn = 0;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+  const tile_walk walk(tiles);
+  for (int tile = walk.at; tile < walk.end; tile += walk.step, turn ^= 1) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const px_ = x + at.b * C * M_;
     const T* const pd_ = dy + at.b * C * M_;
@@ -367,7 +389,7 @@ long long chan_tiles(int B, int C, int M) { return (long long)B * cloud_tiles(C,
 int chan_grad_parts(int B, int C, int M) {
   const chan_plan p = chan_shape(C);
   const long long n = chan_tiles(B, C, M), most = 256 * (long long)((p.kc == 2 || p.kc == 3 ? 2048 : 1024) / p.threads);
-  return (int)(n <= 4 ? 1 : n < most ? n : most);
+  return (int)(n <= 4 ? 1 : n < 8 ? n : n < most ? (n + 7) / 8 * 8 : most);
 }
 constexpr int MAX_POINTS = 1 << 24;        // per cloud: 64 channel slots of them are within 32-bit byte offsets
 bool chan_ok(int dtype, int B, int C, int M) {
@@ -399,7 +421,7 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
                  float* mean, float* rstd, hipStream_t st) {
   const chan_plan p = chan_shape(C);
   const long long tiles = chan_tiles(B, C, M);
-  const dim3 grid((unsigned)(tiles < 8192 ? tiles : 8192));
+  const dim3 grid((unsigned)(tiles < 8 ? tiles : tiles < 8192 ? (tiles + 7) / 8 * 8 : 8192));
 #define LN_CALL(KC, PX)                                                                                                     \
   hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX>), grid, dim3(p.threads), 0, st, (int)tiles, cloud_tiles(C, M), C, M,        \
                      (const T*)x, w, b, eps, relu, (T*)y, mean, rstd)
