@@ -23,29 +23,32 @@ _raw_stream = torch._C._cuda_getCurrentRawStream       # torch.cuda.current_stre
 
 
 def _stream(t):
-    return _raw_stream(t.device.index)
+    return _raw_stream(t.get_device())
 
 
-def _need(ok, what):
+def _need(ok, what, *args):
     if not ok:
-        raise RuntimeError(what)
+        raise RuntimeError(what % args if args else what)
 
 
 MAX_STRIDE = 1 << 20        # row strides (in elements) that the kernels take; wider ones are copied
 
 
 def _rows(t):
-    """(..., C) -> (2-D view or copy whose channels are contiguous, its row stride)."""
+    """(..., C) -> (a tensor that starts with its rows -- t itself, a 2-D view or a copy, channels contiguous --, the rows'
+    stride)."""
     C = t.size(-1)
+    if t.is_contiguous():
+        return t, C
     m = t if t.dim() == 2 else t.reshape(-1, C)
     if (m.stride(1) != 1 and C > 1) or m.stride(0) > MAX_STRIDE:
         m = m.contiguous()
     return m, (m.stride(0) if m.size(0) > 1 else C)
 
 
-def _like(m, shape):
-    """An uninitialised contiguous tensor of m's type and this shape."""
-    return torch.empty_like(m) if m.shape == shape and m.is_contiguous() else m.new_empty(shape)
+def _like(m):
+    """An uninitialised contiguous tensor of m's type and shape."""
+    return torch.empty_like(m) if m.is_contiguous() else m.new_empty(m.shape)
 
 
 def _align16(n):
@@ -132,7 +135,8 @@ def act8_pack(x):
     _need(x.dim() >= 1 and x.size(-1) > 0, "x must have at least one channel")
     with on_device(x.device):
         m, xs = _rows(x)
-        rows, C = m.shape
+        C = x.size(-1)
+        rows = x.numel() // C
         act = Act8._in(torch.empty(Act8._bytes(rows, C), dtype=torch.uint8, device=x.device), 0, rows, C, x.shape)
         codes, scales = act._ptrs()
         check(lib.pvn3d_act8_pack(t, rows, C, m.data_ptr(), xs, codes, act.pitch, scales, _stream(x)), "act8_pack")
@@ -166,7 +170,7 @@ def linear8_weight_grad(dy, act):
     _need(dy.numel() == rows * M, "dy and act must have the same number of rows")
     with on_device(dy.device):
         m, ds = _rows(dy)
-        dw = torch.empty((M, N), dtype=torch.float32, device=dy.device)
+        dw = torch.empty(M, N, dtype=torch.float32, device=dy.device)
         wsb = lib.pvn3d_act8_wgrad_workspace_bytes(rows, M, N)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
         codes, scales = act._ptrs()
@@ -182,7 +186,8 @@ def _ld(c):
 def _padded(m, C):
     """(rows, C) bfloat16 -> (matrix whose rows hold a multiple of 16 channels, zeros behind C, 16-byte aligned; its row
     stride): what the matrix kernel reads."""
-    if C % 16 == 0 and m.data_ptr() % 16 == 0 and (m.size(0) <= 1 or m.stride(0) % 8 == 0):
+    if (C % 16 == 0 and m.stride(1) == 1 and m.data_ptr() % 16 == 0
+            and (m.size(0) <= 1 or (m.stride(0) % 8 == 0 and C <= m.stride(0) < 2 ** 31))):
         return m, (m.stride(0) if m.size(0) > 1 else C)
     out = torch.zeros((m.size(0), _ld(C)), dtype=torch.bfloat16, device=m.device)
     out[:, :C] = m
@@ -208,14 +213,13 @@ def _product(m, C, weight, transpose):
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight):
+    def forward(ctx, x, weight, keep):
         N, C = weight.shape
         with on_device(x.device):
-            m, _ = _rows(x)
             w = weight.detach().contiguous()
-            y = _product(m, C, w, False)
+            y = _product(x.reshape(-1, C), C, w, False)
             ctx.act = None
-            if ctx.needs_input_grad[1]:
+            if keep and ctx.needs_input_grad[1]:
                 ctx.act = act8_pack(x.detach())
         ctx.save_for_backward(weight)
         ctx.lead = x.shape[:-1]
@@ -229,12 +233,12 @@ class _Linear8(torch.autograd.Function):
         dx = dw = None
         dy = dy.to(torch.bfloat16)
         with on_device(dy.device):
-            m, _ = _rows(dy)
+            m = dy.reshape(-1, N)
             if ctx.needs_input_grad[0]:
                 dx = _product(m, N, weight.detach().contiguous(), True).reshape(ctx.lead + (C,))
             if ctx.needs_input_grad[1]:
                 dw = linear8_weight_grad(m, ctx.act)
-        return dx, dw
+        return dx, dw, None
 
 
 def linear8(x, weight):
@@ -248,4 +252,4 @@ def linear8(x, weight):
     _need(weight.dim() == 2 and weight.dtype == torch.float32, "weight must be a float32 matrix")
     _need(x.dim() >= 1 and x.size(-1) == weight.size(1) and weight.numel() > 0, "x and weight must have the same channels")
     _need(x.numel() // x.size(-1) < 2 ** 31, "too many rows")
-    return _Linear8.apply(x, weight)
+    return _Linear8.apply(x, weight, torch.is_grad_enabled())

@@ -26,8 +26,9 @@ MAX_CHANNELS = 8192
 def _param(p, C, x, name):
     if p is None:
         return None
-    _need(p.dtype is torch.float32 and p.shape == (C,), "%s must be a float32 tensor of the channels' length" % name)
-    _need(p.device == x.device, "%s must be on x's device" % name)
+    _need(p.dtype is torch.float32 and p.dim() == 1 and p.numel() == C,
+          "%s must be a float32 tensor of the channels' length", name)
+    _need(p.get_device() == x.get_device(), "%s must be on x's device", name)
     return p if p.is_contiguous() else p.contiguous()
 
 
@@ -38,15 +39,16 @@ def _ptr(t):
 def _check_x(x, name="x"):
     _need(x.is_cuda, "CPU not supported")
     t = DTYPES.get(x.dtype)
-    _need(t is not None, "%s must be a float32, bfloat16 or float16 tensor" % name)
+    _need(t is not None, "%s must be a float32, bfloat16 or float16 tensor", name)
     return t
 
 
 def _by_rows(x, channel_dim):
     """-> (True, x with the channels last) or (False, contiguous (B, C, ...)); refuses what is neither."""
-    _need(x.dim() >= 1, "x must have a channel dimension")
-    d = channel_dim + x.dim() if channel_dim < 0 else channel_dim
-    if d == x.dim() - 1:
+    n = x.dim()
+    _need(n >= 1, "x must have a channel dimension")
+    d = channel_dim + n if channel_dim < 0 else channel_dim
+    if d == n - 1:
         rows, C = True, x.size(-1)
     else:
         _need(d == 1, "channel_dim must be 1 or the last dimension")
@@ -55,7 +57,7 @@ def _by_rows(x, channel_dim):
         few = x.numel() // max(1, x.size(0) * C) < 4
         rows = few or (x.movedim(1, -1).is_contiguous() and not x.is_contiguous())
         x = x.movedim(1, -1) if rows else x.contiguous()
-    _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
+    _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels", MAX_CHANNELS)
     return rows, x
 
 
@@ -73,8 +75,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
     with on_device(x.device):
         n = v.numel() // C
-        y = _like(v, v.shape)
-        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
+        y = _like(v)
+        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device).unbind()
         if rows:
             m, xs = _rows(v)
             check(lib.pvn3d_layer_norm(t, n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), eps, 1 if relu else 0, y.data_ptr(), C, C,
@@ -90,22 +92,22 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
 
 def _grad_buffers(C, wsb, dev):
     """dweight, dbias and the workspace of their partial sums."""
-    dw, db = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0)
+    dw, db = torch.empty(2, C, dtype=torch.float32, device=dev).unbind()
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     return dw, db, ws, dw.data_ptr(), db.data_ptr(), _ptr(ws)
 
 
 def _check_stats(mean, rstd, n, x):
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.device == x.device,
-              "%s must be a contiguous float32 tensor with one value per point" % name)
+        _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == x.get_device(),
+              "%s must be a contiguous float32 tensor with one value per point", name)
 
 
 def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=False, need_dx=True, need_dparams=True):
     """-> (dx like x or None, dweight (C,), dbias (C,) float32 or None, None).  mean, rstd: the forward's; relu: the
     derivative is taken where weight xh + bias > 0."""
     t = _check_x(x)
-    _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device, "dy must be like x")
+    _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.get_device() == x.get_device(), "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
     rows, v = _by_rows(x, channel_dim)
     C = v.size(-1) if rows else v.size(1)
@@ -117,7 +119,7 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=Fa
     wsb = 0
     with on_device(dev):
         if need_dx:
-            dx = _like(v, v.shape)
+            dx = _like(v)
         if rows:
             d = dy if v is x else dy.movedim(1, -1)
             (m, xs), (g, gs) = _rows(v), _rows(d)
@@ -181,14 +183,14 @@ class Saved8(object):
 def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
     """x (..., C) -> (y like x, Saved8).  y is layer_norm_forward's, bit for bit."""
     t = _check_x(x)
-    _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, "layer norm takes 1 to %d channels" % MAX_CHANNELS)
+    _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, "layer norm takes 1 to %d channels", MAX_CHANNELS)
     C = x.size(-1)
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
     dev = x.device
     with on_device(dev):
         m, xs = _rows(x)
-        n = m.size(0)
-        y = _like(x, x.shape)
+        n = x.numel() // C
+        y = _like(x)
         saved = Saved8(n, C, x.shape, x.dtype, bool(relu), dev)
         (codes, scales), (mean, rstd, mask) = saved.act._ptrs(), saved._ptrs()
         check(lib.pvn3d_layer_norm(t, n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), eps, 1 if relu else 0, y.data_ptr(), C, C,
@@ -211,7 +213,7 @@ def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True
     with on_device(dev):
         g, gs = _rows(dy)
         if need_dx:
-            dx = _like(dy, dy.shape)
+            dx = _like(dy)
         if need_dparams:
             wsb = lib.pvn3d_layer_norm_grad_workspace_bytes(t, n, C)
             dw, db, ws, pw, pb, pws = _grad_buffers(C, wsb, dev)
@@ -261,7 +263,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False, 
     """Differentiable layer norm (see the top of this file).  ckpt8: keep x for the backward pass in 8 bits instead of
     holding on to it (channels last only); the output is the same, the gradients take xh from the 8-bit form."""
     _check_x(x)
-    return _LayerNorm.apply(x, weight, bias, eps, channel_dim, bool(relu), bool(ckpt8))
+    return _LayerNorm.apply(x, weight, bias, eps, channel_dim, bool(relu), bool(ckpt8) and torch.is_grad_enabled())
 
 
 class LayerNorm(nn.Module):
