@@ -56,14 +56,13 @@ __device__ __forceinline__ void forget<float>(raw4<float>& a) {
 // Chunks are whole and unconditional: the last, partial one of a row of points is taken as its last four points, which
 // overlap the neighbour's -- computed and stored twice, with the same bits, and left out of dw and db.  Lanes behind the
 // cloud's last point repeat its last four without a store.
-// Tiles of a workgroup: workgroups are dealt to the eight XCDs in turn, and neighbouring tiles share the cache lines that
-// their rows' ends lie in (all of them, in part, if M is odd), so each XCD -- its own L2 -- gets a run of tiles: XCD x
-// walks x per, x per + 1, ... with all its workgroups.  (Grids of fewer than eight, or no multiple of it: in turn.)
+// Tiles of a workgroup.  In turn, or in runs: workgroups are dealt to the eight XCDs in turn, each with an L2 of its own, and
+// where neighbouring tiles share memory lines each XCD walks a run of an eighth of the tiles with all its workgroups.
 struct tile_walk {
   int at, step, end;
-  __device__ __forceinline__ explicit tile_walk(int tiles) {
+  __device__ __forceinline__ tile_walk(int tiles, int runs) {
     const int g = gridDim.x, b = blockIdx.x;
-    if (g & 7) {
+    if (!runs) {
       at = b;
       step = g;
       end = tiles;
@@ -111,7 +110,8 @@ __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[PX * N]) {
 }
 
 template <typename T, int KC, int PX>
-__global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per_cloud, int C, int M, const T* __restrict__ x,
+__global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int runs, int per_cloud, int C, int M,
+                                                              const T* __restrict__ x,
                                                               const float* __restrict__ w, const float* __restrict__ b,
                                                               float eps, int relu, T* __restrict__ y,
                                                               float* __restrict__ mean, float* __restrict__ rstd) {
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
     bk[k] = KC > 0 && b && has[k] ? b[c] : 0.f;
   }
   const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
-  const tile_walk walk(tiles);
+  const tile_walk walk(tiles, runs);
   for (int tile = walk.at; tile < walk.end; tile += walk.step) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const p = x + at.b * C * M_;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int per
 // dw / db: a thread has the same channels for all its tiles: a register each, summed over the 16 lanes at the end (KC = 0:
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
 template <typename T, int KC, int PX>
-__global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int per_cloud, int C, int M,
+__global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int runs, int per_cloud, int C, int M,
                                                                    const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ w,
                                                                    const float* __restrict__ b,
                                                                    const float* __restrict__ mean,
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     __syncthreads();
   }
   int turn = 0;
-  const tile_walk walk(tiles);
+  const tile_walk walk(tiles, runs);
   for (int tile = walk.at; tile < walk.end; tile += walk.step, turn ^= 1) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const px_ = x + at.b * C * M_;
@@ -383,6 +383,13 @@ chan_plan chan_shape(int C) {
 }
 int cloud_tiles(int C, int M) { return (int)(((long long)M + chan_shape(C).px * PTS - 1) / (chan_shape(C).px * PTS)); }
 long long chan_tiles(int B, int C, int M) { return (long long)B * cloud_tiles(C, M); }
+// Whether neighbouring tiles share lines of `line` bytes: their rows start or end within one (23 x 313 x 2324 in bf16: forward
+// 30.7 us in turn, 19.7 in runs; backward 50.9, 36.5).  Where they do not, runs are the slower, 24 x 64 x 65536 backward 143 us
+// against 133 -- except for the forward and tiles of 128 bytes (24 x 256 x 12288 in bf16 67.4 us, 62.4), so it asks for 256.
+bool chan_runs(int elem, int C, int M, int line, long long grid) {
+  const long long tile = (long long)chan_shape(C).px * PTS * elem;
+  return (grid & 7) == 0 && (tile % line != 0 || (long long)M * elem % line != 0);
+}
 // workgroups of a backward launch: what is on the chip at once (every one starts with the parameters and ends with its
 // partial sums): by its registers 32 waves a CU with two or three channels a thread, 16 with more (one: 16 are
 // the faster, 24 x 16 x 65536 fp32 61 us against 72).  A few tiles are one workgroup's, which writes dw and db itself.
@@ -423,7 +430,8 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
   const long long tiles = chan_tiles(B, C, M);
   const dim3 grid((unsigned)(tiles < 8 ? tiles : tiles < 8192 ? (tiles + 7) / 8 * 8 : 8192));
 #define LN_CALL(KC, PX)                                                                                                     \
-  hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX>), grid, dim3(p.threads), 0, st, (int)tiles, cloud_tiles(C, M), C, M,        \
+  hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX>), grid, dim3(p.threads), 0, st, (int)tiles,                                 \
+                     (int)chan_runs(sizeof(T), C, M, 256, grid.x), cloud_tiles(C, M), C, M,                                 \
                      (const T*)x, w, b, eps, relu, (T*)y, mean, rstd)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
@@ -442,6 +450,7 @@ int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x,
   }
 #define LN_CALL(KC, PX)                                                                                                     \
   hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX>), dim3(parts), dim3(p.threads), lds, st, (int)chan_tiles(B, C, M),     \
+                     (int)chan_runs(sizeof(T), C, M, 128, parts),                                                           \
                      cloud_tiles(C, M), C, M, (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, pw, pb, ps)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
