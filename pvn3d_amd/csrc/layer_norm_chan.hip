@@ -7,6 +7,8 @@
 // every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
 // exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more channels than the registers of 1024 threads hold
 // -- x is read again for every pass.
+// Bound by HBM.  fp32 24 x 128 x 12288 forward 61 us = 5.0 TB/s; bf16 8 x 196 x 16384 backward 38 us = 4.0 TB/s (two
+// workgroups a CU load, add up and store in turn).
 #include "layer_norm.h"
 
 namespace {

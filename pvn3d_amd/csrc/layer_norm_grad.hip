@@ -11,6 +11,8 @@ using ln::row_sum;
 // ------------------------------------------------------------------------------------------------ rows, backward
 // As the forward; a thread's channels are the same for all its rows, so dw and db are summed in its registers over the
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
+// Bound by HBM: dy and x read, dx written, once each.  bf16 786432 x 128: 115 us = 5.2 TB/s; 393216 x 196 from 8 bits: 100 us
+// = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of 1024 to 2048 partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
 __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
