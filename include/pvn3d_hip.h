@@ -646,7 +646,7 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
  *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C) names, 4-byte aligned, needed for dweight
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
- * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^24 (or 0); mean, rstd (B, M). */
+ * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^23 (or 0); mean, rstd (B, M). */
 int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
                      float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
                      long long pitch, void* scales, void* mask, void* stream);

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
   constexpr int KR = KC > 0 ? KC : 1;
   __shared__ float buf[2][MAX_THREADS / 64][PX * PTS];
   const int cy = threadIdx.x / PX, CY = blockDim.x / PX;
-  const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
+  const size_t M_ = M, cloud = C * M_, slots = (size_t)CY * M;      // slots: elements between a thread's channels
   const float rc = 1.f / (float)C;
   float low = relu ? 0.f : -__builtin_inff();
   asm("" : "+v"(low));             // a register, not a choice of two constants at every use
@@ -137,8 +137,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
   const tile_walk walk(tiles, runs);
   for (int tile = walk.at; tile < walk.end; tile += walk.step) {
     const tile_at<PX> at(tile, per_cloud, M);
-    const T* const p = x + at.b * C * M_;
-    T* const q = y + at.b * C * M_;
+    const T* const p = x + at.b * cloud;
+    T* const q = y + at.b * cloud;
     const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> r[KR];
     float s[PTS] = {0.f, 0.f, 0.f, 0.f}, mu[PTS], rs[PTS];
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
   __shared__ float buf[2][MAX_THREADS / 64][PX * 2 * PTS];
   extern __shared__ float lacc[];
   const int px = threadIdx.x & (PX - 1), cy = threadIdx.x / PX, CY = blockDim.x / PX;
-  const size_t M_ = M, slots = (size_t)CY * M;               // elements from one of a thread's channels to the next
+  const size_t M_ = M, cloud = C * M_, slots = (size_t)CY * M;      // slots: elements between a thread's channels
   const float rc = 1.f / (float)C;
   float aw[KR], ab[KR], gk[KR], bk[KR];
   bool has[KR];                    // (only the last of a thread's channels can be missing)
@@ -234,9 +234,9 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
   const tile_walk walk(tiles, runs);
   for (int tile = walk.at; tile < walk.end; tile += walk.step, turn ^= 1) {
     const tile_at<PX> at(tile, per_cloud, M);
-    const T* const px_ = x + at.b * C * M_;
-    const T* const pd_ = dy + at.b * C * M_;
-    T* const po_ = dx + at.b * C * M_;
+    const T* const px_ = x + at.b * cloud;
+    const T* const pd_ = dy + at.b * cloud;
+    T* const po_ = dx + at.b * cloud;
     const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> rx[KR], rd[KR];
     float mu[PTS], rs[PTS], s[2 * PTS];
@@ -400,7 +400,7 @@ int chan_grad_parts(int B, int C, int M) {
   const long long n = chan_tiles(B, C, M), most = 256 * (long long)((p.kc == 2 || p.kc == 3 ? 2048 : 1024) / p.threads);
   return (int)(n <= 4 ? 1 : n < 8 ? n : n < most ? (n + 7) / 8 * 8 : most);
 }
-constexpr int MAX_POINTS = 1 << 24;        // per cloud: 64 channel slots of them are within 32-bit byte offsets
+constexpr int MAX_POINTS = 1 << 23;        // per cloud: 128 channel slots (chan_shape) of them are within 32-bit byte offsets
 bool chan_ok(int dtype, int B, int C, int M) {
   return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || (M >= PTS && M <= MAX_POINTS)) &&
          chan_tiles(B, C, M) < 0x7fffffffLL - 16384;

@@ -21,6 +21,7 @@ from .._lib import lib, check, on_device
 from .act8 import Act8, DTYPES, _like, _need, _rows, _stream
 
 MAX_CHANNELS = 8192
+MAX_POINTS = 1 << 23         # per cloud, of the channel-major kernels
 
 
 def _param(p, C, x, name):
@@ -53,9 +54,10 @@ def _by_rows(x, channel_dim):
     else:
         _need(d == 1, "channel_dim must be 1 or the last dimension")
         C = x.size(1)
-        # a point-major view in place; fewer points than a chunk of the channel-major kernel: as rows of a copy
-        few = x.numel() // max(1, x.size(0) * C) < 4
-        rows = few or (x.movedim(1, -1).is_contiguous() and not x.is_contiguous())
+        # a point-major view in place; fewer points than a chunk of the channel-major kernel, or more than it addresses:
+        # as rows of a copy
+        M = x.numel() // max(1, x.size(0) * C)
+        rows = not 4 <= M <= MAX_POINTS or (x.movedim(1, -1).is_contiguous() and not x.is_contiguous())
         x = x.movedim(1, -1) if rows else x.contiguous()
     _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels", MAX_CHANNELS)
     return rows, x

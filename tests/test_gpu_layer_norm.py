@@ -374,6 +374,34 @@ def test_more_than_32_bits_of_elements(dev):
     assert torch.equal(dx[pick], ln.layer_norm_backward(s, s, None, None, ms, rs)[0])
 
 
+def test_more_than_32_bits_of_channel_rows(dev):
+    """(B, C, M) with B C beyond 2^31 (17 GB a tensor): the last clouds as on their own."""
+    B, C, M = (1 << 18) + 1, 8192, 4
+    x = torch.zeros((B, C, M), dtype=torch.bfloat16, device=dev)
+    x[-2:] = torch.randn(2, C, M, generator=torch.Generator().manual_seed(5)).to(dev)
+    y, mean, rstd = ln.layer_norm_forward(x, channel_dim=1)
+    s = x[-2:].clone()
+    ys, ms, rs = ln.layer_norm_forward(s, channel_dim=1)
+    assert torch.equal(y[-2:], ys) and torch.equal(mean[-2 * M:], ms) and torch.equal(rstd[-2 * M:], rs)
+    del y
+    dx = ln.layer_norm_backward(x, x, None, None, mean, rstd, channel_dim=1, need_dparams=False)[0]
+    assert torch.equal(dx[-2:], ln.layer_norm_backward(s, s, None, None, ms, rs, channel_dim=1, need_dparams=False)[0])
+
+
+def test_clouds_of_many_points(dev):
+    """More points than the channel-major kernels address: taken as rows."""
+    B, C, M = 1, 3, ln.MAX_POINTS + 5
+    x = torch.randn(B, C, M, device=dev, generator=torch.Generator("cuda").manual_seed(6))
+    w, b = torch.randn(C, device=dev), torch.randn(C, device=dev)
+    y, mean, rstd = ln.layer_norm_forward(x, w, b, channel_dim=1)
+    yr, mr, rr = ln.layer_norm_forward(x.transpose(1, 2).contiguous(), w, b)
+    assert y.is_contiguous() and torch.equal(y, yr.transpose(1, 2)) and torch.equal(mean, mr) and torch.equal(rstd, rr)
+    got = ln.layer_norm_backward(x, x, w, b, mean, rstd, channel_dim=1)
+    xr = x.transpose(1, 2).contiguous()
+    want = ln.layer_norm_backward(xr, xr, w, b, mean, rstd)
+    assert torch.equal(got[0], want[0].transpose(1, 2)) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
 def test_refusals(dev):
     x = torch.randn(4, 8, device=dev)
     w = torch.ones(8, device=dev)
