@@ -218,17 +218,18 @@ class _Linear8(torch.autograd.Function):
         with on_device(x.device):
             w = weight.detach().contiguous()
             y = _product(x.reshape(-1, C), C, w, False)
-            ctx.act = None
+            buf = ctx.kept = None
             if keep and ctx.needs_input_grad[1]:
-                ctx.act = act8_pack(x.detach())
-        ctx.save_for_backward(weight)
+                act = act8_pack(x.detach())
+                ctx.kept, buf = (act.rows, C, act.shape), act._buf
+        ctx.save_for_backward(weight, buf)        # (the buffer is given up behind this layer's backward pass)
         ctx.lead = x.shape[:-1]
         return y.view(x.shape[:-1] + (N,)) if x.dim() != 2 else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight, = ctx.saved_tensors
+        weight, buf = ctx.saved_tensors
         N, C = weight.shape
         dx = dw = None
         dy = dy.to(torch.bfloat16)
@@ -237,7 +238,7 @@ class _Linear8(torch.autograd.Function):
             if ctx.needs_input_grad[0]:
                 dx = _product(m, N, weight.detach().contiguous(), True).reshape(ctx.lead + (C,))
             if ctx.needs_input_grad[1]:
-                dw = linear8_weight_grad(m, ctx.act)
+                dw = linear8_weight_grad(m, Act8._in(buf, 0, *ctx.kept))
         return dx, dw, None
 
 

@@ -152,10 +152,11 @@ class Saved8(object):
     scales, mask, statistics; views of it are made when they are asked for."""
     __slots__ = ("act", "dtype", "relu", "_buf", "_mask", "_stat")
 
-    def __init__(self, rows, C, shape, dtype, relu, dev):
+    def __init__(self, rows, C, shape, dtype, relu, dev, buf=None):
+        """buf: an earlier one's buffer."""
         mask = (Act8._bytes(rows, C) + 3) & ~3
         stat = (mask + (rows * ((C + 7) // 8) if relu else 0) + 3) & ~3
-        self._buf = torch.empty(stat + 8 * rows, dtype=torch.uint8, device=dev)
+        self._buf = torch.empty(stat + 8 * rows, dtype=torch.uint8, device=dev) if buf is None else buf
         self._mask, self._stat, self.dtype, self.relu = mask, stat, dtype, relu
         self.act = Act8._in(self._buf, 0, rows, C, shape)
 
@@ -230,13 +231,18 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, channel_dim, relu, ckpt8):
         ctx.meta = (channel_dim, relu)
-        ctx.saved8 = None
+        ctx.kept = None
         if ckpt8:
             rows, v = _by_rows(x, channel_dim)
             _need(rows, "ckpt8 takes channels-last tensors (or a transposed view of one)")
             ctx.moved = v is not x
-            y, ctx.saved8 = layer_norm_forward8(v, weight, bias, eps, relu)
-            ctx.save_for_backward(weight)
+            if not any(ctx.needs_input_grad):
+                y = layer_norm_forward(v, weight, bias, eps, -1, relu)[0]
+            else:
+                # the buffer as a saved tensor: it is given up behind this layer's backward pass, not with the whole graph
+                y, saved = layer_norm_forward8(v, weight, bias, eps, relu)
+                ctx.kept = (saved.act.rows, saved.act.channels, saved.act.shape, saved.dtype, saved.relu)
+                ctx.save_for_backward(weight, saved._buf)
             return y.movedim(-1, 1) if ctx.moved else y
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps, channel_dim, relu)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
@@ -249,10 +255,10 @@ class _LayerNorm(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         if not (need_x or need_w or need_b):
             return (None,) * 7
-        if ctx.saved8 is not None:
-            weight, = ctx.saved_tensors
+        if ctx.kept is not None:
+            weight, buf = ctx.saved_tensors
             d = dy.movedim(1, -1) if ctx.moved else dy
-            dx, dw, db = layer_norm_backward8(d, ctx.saved8, weight, need_x, need_w or need_b)
+            dx, dw, db = layer_norm_backward8(d, Saved8(*ctx.kept, buf.device, buf), weight, need_x, need_w or need_b)
             if ctx.moved and need_x:
                 dx = dx.movedim(-1, 1)
         else:

@@ -178,6 +178,34 @@ def test_a_layer_and_its_training_pass(dev):
         assert float((a.double() - b).norm() / b.norm()) < 0.03      # bf16 activations (2^-8), steps of 1/64 - 1/128
 
 
+def test_kept_buffers_are_given_up_behind_the_backward_pass(dev):
+    """What a layer keeps goes when its backward pass is done, although the graph's output lives on; a graph that is retained
+    can be gone through again; without retaining it a second pass is refused."""
+    from pvn3d_amd.lib.layer_norm import layer_norm
+    x = torch.randn(4096, 256, device=dev).bfloat16()
+    w = torch.randn(256, 256, device=dev, requires_grad=True)
+    g = torch.ones(256, device=dev, requires_grad=True)
+    b = torch.zeros(256, device=dev, requires_grad=True)
+    calls = {"linear8": lambda: act8.linear8(x, w), "layer_norm": lambda: layer_norm(x, g, b, relu=True, ckpt8=True)}
+    for name, call in calls.items():
+        y = call()
+        dy = torch.ones_like(y)
+        leaves = [w] if name == "linear8" else [g, b]
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        again = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(first, again)), name
+        del first, again
+        before = torch.cuda.memory_allocated()
+        torch.autograd.grad(y, leaves, dy)
+        assert before - torch.cuda.memory_allocated() >= x.numel(), name
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaves, dy)
+    # nothing is kept where no gradient is asked for
+    before = torch.cuda.memory_allocated()
+    y = layer_norm(x, g.detach(), b.detach(), relu=True, ckpt8=True)
+    assert torch.cuda.memory_allocated() - before <= 2 * x.numel() and not y.requires_grad
+
+
 def test_captured(dev):
     g = torch.Generator().manual_seed(12)
     x = torch.randn(700, 99, generator=g).to(torch.bfloat16).to(dev)
@@ -198,6 +226,38 @@ def test_captured(dev):
     for i in range(4):
         x.copy_(torch.randn(700, 99, generator=g))
         dy.copy_(torch.randn(700, 130, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, step()))
+
+
+@pytest.mark.parametrize("dims", [(64, 96, 32), (33, 50, 7)])
+def test_a_training_pass_captured(dev, dims):
+    """The differentiable calls together, forward and backward in one captured graph, replayed with other inputs."""
+    g = torch.Generator().manual_seed(14)
+    rows = 1500
+    x = torch.zeros(rows, dims[0], dtype=torch.bfloat16, device=dev, requires_grad=True)
+    dy = torch.zeros(rows, dims[2], dtype=torch.bfloat16, device=dev)
+    ws = [(torch.randn(b, a, generator=g) / a ** 0.5).to(dev).requires_grad_() for a, b in zip(dims, dims[1:])]
+    norm = ln.LayerNorm(dims[1], relu=True, ckpt8=True).to(dev)
+    leaves = [x] + ws + [norm.weight, norm.bias]
+
+    def step():
+        out = act8.linear8(norm(act8.linear8(x, ws[0])), ws[1])
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=g))
+            dy.copy_(torch.randn(dy.shape, generator=g))
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, step()))

@@ -173,6 +173,21 @@ def test_network_with_layer_norm(dev):
     assert _rel(both[:1], one) < 1e-5
 
 
+def test_graphed_forward_with_layer_norm(dev):
+    """The captured eval forward of a network with layer norm replays the eager one."""
+    from pvn3d_amd.lib.pointnet2_msg import GraphedForward, Pointnet2MSG
+    torch.manual_seed(0)
+    net = Pointnet2MSG(norm="layer").to(dev).eval()
+    clouds = _clouds(3, 4096, dev)
+    pcs = [torch.cat([c, torch.rand(4096, 6, device=dev)], 1)[None].contiguous() for c in clouds]
+    graphed = GraphedForward(net, pcs[0])
+    for pc in pcs + pcs:
+        got = graphed(pc).clone()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert _rel(got, net(pc)) < 1e-5
+
+
 def test_unknown_norm_is_refused():
     from pvn3d_amd.lib.pointnet2_utils import pointnet2_modules as pm
     with pytest.raises(ValueError):
