@@ -646,6 +646,8 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
  *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C) names, 4-byte aligned, needed for dweight
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
+ * var + eps has to be a normal fp32 number (a smaller one counts as zero, and its points are not finite).  Outputs do not
+ * overlap inputs.
  * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^23 (or 0); mean, rstd (B, M). */
 int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
                      float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
@@ -664,12 +666,12 @@ int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const void* dy, c
 
 /* ---- Activations in 8 bits for the backward pass (csrc/act8.hip; no reference counterpart) --------------------
  * 32 consecutive channels of a row (the last group may be shorter) share 2^e: code = rint(x 2^-e) (int8), e >= -126 the
- * smallest with rint(absmax 2^-e) <= 127 (121 at most: codes stop at +-127 there); scales[row][c / 32] = e + 127.  A group with an infinity or a NaN: scale 255,
- * codes 0, read back as NaN.  codes [rows] of pitch `pitch` (a multiple of 16, base 16-byte aligned; the last row ends
- * with a whole 16-byte chunk too), scales [rows][ceil(C / 32)].  Codes behind C are not read as values.
+ * smallest with rint(absmax 2^-e) <= 127 (121 at most: codes stop at +-127 there); scales[row][c / 32] = e + 127.  A group
+ * with an infinity or a NaN: scale 255, codes 0, read back as NaN.  codes [rows] of pitch `pitch` (a multiple of 16, base
+ * 16-byte aligned; the last row ends with a whole 16-byte chunk too), scales [rows][ceil(C / 32)].  Codes behind C are not read as values.
  * pvn3d_act8_unpack writes the held values (exact in fp32 and bf16), zeros in columns C .. y_cols - 1.
  * pvn3d_act8_wgrad: dW [M][N] fp32 = dY^T X, dY bf16 [rows] of stride dys (M columns), X = the held values [rows][N], on
- * v_mfma_f32_32x32x16_bf16; fixed order of the sums; strides up to 2^20.  No rows: zeros. */
+ * v_mfma_f32_32x32x16_bf16; fixed order of the sums; strides up to 2^20.  workspace: 16-byte aligned.  No rows: zeros. */
 int pvn3d_act8_pack(int dtype, long long rows, int C, const void* x, long long xs, void* codes, long long pitch, void* scales,
                     void* stream);
 int pvn3d_act8_unpack(int dtype, long long rows, int C, const void* codes, long long pitch, const void* scales, void* y,

@@ -73,9 +73,10 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, i
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C, int tpr, const signed char* __restrict__ codes,
-                                                          int pitch, const unsigned char* __restrict__ scales,
-                                                          T* __restrict__ y, int ys, int ycols) {
+__global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C, int tpr,
+                                                          const signed char* __restrict__ codes, int pitch,
+                                                          const unsigned char* __restrict__ scales, T* __restrict__ y, int ys,
+                                                          int ycols) {
   constexpr int VEC = traits<T>::VEC;
   const int t = threadIdx.x & (tpr - 1), rg = threadIdx.x / tpr, rpb = 256 / tpr;
   const int G = (C + rv::GROUP - 1) / rv::GROUP;
@@ -126,14 +127,12 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C,
 
 // ------------------------------------------------------------------------------------------------ weight gradient
 // dW[m][n] = sum over rows r of dY[r][m] X[r][n].  Rows are the contraction and both operands hold them as their slow
-// dimension; a matrix instruction wants eight of them per lane.  A step of 32 or 64 rows is staged in LDS as it lies in memory (X
-// converted to bf16 on the way) and read back with ds_read_b64_tr_b16, which hands a group of 16 lanes a 4 x 16 block
+// dimension; a matrix instruction wants eight of them per lane.  A step of 32 or 64 rows is staged in LDS as it lies in memory
+// (X converted to bf16 on the way) and read back with ds_read_b64_tr_b16, which hands a group of 16 lanes a 4 x 16 block
 // transposed.  Row strides of 64 bytes times an odd number keep the four rows of such a block in different banks.
 // A workgroup owns a (32 MB WM) x (32 NB WN) tile of dW and steps s, s + S, ... of ROWS rows: WM WN waves share a step's
 // staging (a barrier per step), or, with WM = WN = 1, each of four waves stages its own steps.  S partial tiles go to the
 // workspace, summed in a fixed order by rowvec.h's fold (S = 1: straight to dW).
-
-
 __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride, int lane) {
   // lane l of a 16-lane group reads 8 bytes of row (l & 15) >> 2, columns 4 (l & 3) ..; it receives column l & 15, four rows
   const int g = lane >> 4;                                       // groups: (columns 0-15 | 16-31) x (rows 0-7 | 8-15)
@@ -169,10 +168,9 @@ __device__ __forceinline__ uint4 shift_down(const rv::u4_any& v, int skip) {
 // they are staged), columns behind the last repeat others and end in columns of the tile that are not stored -- and its
 // address is a base the workgroup shares plus a 32-bit offset.  RAGGED: M is no multiple of 8.
 template <int MB, int NB, int WM, int WN, int ROWS, bool RAGGED>
-__global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_kernel(long long rows, int M, int N, const bf16* __restrict__ dY, int dys,
-                                                         const signed char* __restrict__ codes, int pitch,
-                                                         const unsigned char* __restrict__ scales, float* __restrict__ out,
-                                                         int S, int tiles_n) {
+__global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_kernel(
+    long long rows, int M, int N, const bf16* __restrict__ dY, int dys, const signed char* __restrict__ codes, int pitch,
+    const unsigned char* __restrict__ scales, float* __restrict__ out, int S, int tiles_n) {
   constexpr bool SHARED = WM * WN > 1;                           // the waves share the staged step
   static_assert(SHARED || ROWS == 32, "a wave on its own takes 32 rows a step");
   constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN;
@@ -447,8 +445,8 @@ int run_pack(long long rows, int C, const void* x, long long xs, void* codes, lo
   return 0;
 }
 template <typename T>
-int run_unpack(long long rows, int C, const void* codes, long long pitch, const void* scales, void* y, long long ys, int ycols,
-               hipStream_t st) {
+int run_unpack(long long rows, int C, const void* codes, long long pitch, const void* scales, void* y, long long ys,
+               int ycols, hipStream_t st) {
   const int tpr = row_threads(C, traits<T>::VEC);
   hipLaunchKernelGGL((act8_unpack_kernel<T>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr,
                      (const signed char*)codes, (int)pitch, (const unsigned char*)scales, (T*)y, (int)ys, ycols);
@@ -506,19 +504,20 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
   if (!dY || !codes || !scales || rows > MAX_ROWS) return (int)hipErrorInvalidValue;
   const wg_plan p = wgrad_plan(rows, M, N);
   const size_t count = (size_t)M * N;
-  if (p.S > 1 && (!workspace || workspace_bytes < p.S * count * sizeof(float))) return (int)hipErrorInvalidValue;
+  if (p.S > 1 && (!workspace || ((size_t)workspace & 15) || workspace_bytes < p.S * count * sizeof(float)))
+    return (int)hipErrorInvalidValue;
   float* const out = p.S > 1 ? (float*)workspace : dW;
   const int tn = pvn3d_ceil_div(N, p.tn);
   const long long blocks = (long long)pvn3d_ceil_div(M, p.tm) * tn * p.S;
   if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidValue;
-#define A8_ONE(MB, NB, WM, WN, ROWS, RAG)                                                                                    \
-  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN, ROWS, RAG>), dim3((unsigned)blocks), dim3(WM * WN > 1 ? 64 * WM * WN : 256), 0, A8_ST, rows, M, N, \
-                     (const bf16*)dY, (int)dys, (const signed char*)codes, (int)pitch, (const unsigned char*)scales, out,  \
-                     p.S, tn)
-#define A8_CALL(MB, NB, WM, WN, ROWS)              \
-  do {                                           \
-    if (M & 7) A8_ONE(MB, NB, WM, WN, ROWS, true); \
-    else A8_ONE(MB, NB, WM, WN, ROWS, false);      \
+#define A8_ONE(MB, NB, WM, WN, ROWS, RAG)                                                                                   \
+  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN, ROWS, RAG>), dim3((unsigned)blocks),                                \
+                     dim3(WM * WN > 1 ? 64 * WM * WN : 256), 0, A8_ST, rows, M, N, (const bf16*)dY, (int)dys,               \
+                     (const signed char*)codes, (int)pitch, (const unsigned char*)scales, out, p.S, tn)
+#define A8_CALL(MB, NB, WM, WN, ROWS)                 \
+  do {                                                \
+    if (M & 7) A8_ONE(MB, NB, WM, WN, ROWS, true);    \
+    else A8_ONE(MB, NB, WM, WN, ROWS, false);         \
   } while (0)
   switch (p.kind) {
     case 0: A8_CALL(2, 2, 4, 2, 64); break;

@@ -9,9 +9,6 @@ using rv::fp16;
 using rv::traits;
 
 constexpr int MAX_C = 8192;
-// Workgroups of a backward launch, each with a partial dw and db: what the registers of one chunk a lane let stay on the
-// chip (bf16, 98304 x 1024, two chunks a lane: 111 us from the 8-bit input, 124 with 1024; the others within 2 %).
-constexpr int MAX_PARTS = 2048;
 // Row strides the kernels take: a workgroup addresses its rows (512 at most) as one base and 32-bit byte offsets -- the
 // 64-bit products of a row index cost more than the arithmetic on the row.
 constexpr long long MAX_STRIDE = 1 << 20;

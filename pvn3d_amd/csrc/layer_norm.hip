@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
       }
       if (ycols > C && live)
 #pragma unroll 1
-        for (int c = C + t; c < ycols; c += TPR) traits<T>::store1(rv::at32(yb, (__umul24(rl, ys) + c) * (unsigned)sizeof(T)), 0.f);
+        for (int c = C + t; c < ycols; c += TPR)
+          traits<T>::store1(rv::at32(yb, (__umul24(rl, ys) + c) * (unsigned)sizeof(T)), 0.f);
     }
   }
 }
@@ -142,15 +143,15 @@ int rows_forward(long long rows, int C, const void* x, long long xs, const float
                  void* mask, hipStream_t st) {
 #define LN_CALL(T, TPR, K, R)                                                                                           \
   do {                                                                                                                  \
-    const long long nb = ln::rows_blocks(rows, TPR, R);                                                                     \
-    const dim3 grid((unsigned)(nb < MAX_GRID ? nb : MAX_GRID));                                                               \
+    const long long nb = ln::rows_blocks(rows, TPR, R);                                                                 \
+    const dim3 grid((unsigned)(nb < MAX_GRID ? nb : MAX_GRID));                                                         \
     if (codes)                                                                                                          \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, b, \
-                         eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch, (unsigned char*)scales,   \
-                         (unsigned char*)mask);                                                                         \
+      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, \
+                         b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch,              \
+                         (unsigned char*)scales, (unsigned char*)mask);                                                 \
     else                                                                                                                \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, b, \
-                         eps, relu, (T*)y, (int)ys, ycols, mean, rstd, nullptr, 0, nullptr, nullptr);                      \
+      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs,  \
+                         w, b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, nullptr, 0, nullptr, nullptr);             \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
@@ -169,9 +170,7 @@ extern "C" int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x,
   if (codes && (!scales || (pitch & 15) || pitch < C)) return (int)hipErrorInvalidValue;
   if (rows <= 0) return 0;
   if (!x || !y || !mean || !rstd) return (int)hipErrorInvalidValue;
-  switch (dtype) {
-    case 0: return rows_forward<float>(rows, C, x, xs, weight, bias, eps, relu, y, ys, y_cols, mean, rstd, codes, pitch, scales, mask, (hipStream_t)stream);
-    case 1: return rows_forward<bf16>(rows, C, x, xs, weight, bias, eps, relu, y, ys, y_cols, mean, rstd, codes, pitch, scales, mask, (hipStream_t)stream);
-    default: return rows_forward<fp16>(rows, C, x, xs, weight, bias, eps, relu, y, ys, y_cols, mean, rstd, codes, pitch, scales, mask, (hipStream_t)stream);
-  }
+  const auto run = dtype == 0 ? rows_forward<float> : dtype == 1 ? rows_forward<bf16> : rows_forward<fp16>;
+  return run(rows, C, x, xs, weight, bias, eps, relu, y, ys, y_cols, mean, rstd, codes, pitch, scales, mask,
+             (hipStream_t)stream);
 }

@@ -1,8 +1,8 @@
 // layer_norm_chan.hip -- layer norm over the channels of (B, C, M) tensors, M contiguous: the layout in which the modules
 // hand features on.  The formulas are those of layer_norm.hip.
 //
-// A tile is 64 (32) consecutive points of one cloud: PX = 16 (8) lanes x 4 points across, blockDim.x / PX channel slots down.  A thread
-// holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
+// A tile is 64 (32) consecutive points of one cloud: PX = 16 (8) lanes x 4 points across, blockDim.x / PX channel slots
+// down.  A thread holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
 // is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
 // every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
 // exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more channels than the registers of 1024 threads hold
@@ -139,7 +139,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const p = x + at.b * cloud;
     T* const q = y + at.b * cloud;
-    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
+    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T);
+    const unsigned ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> r[KR];
     float s[PTS] = {0.f, 0.f, 0.f, 0.f}, mu[PTS], rs[PTS];
     if (KC > 0) {
@@ -202,8 +203,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
 template <typename T, int KC, int PX>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int runs, int per_cloud, int C, int M,
-                                                                   const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ w,
-                                                                   const float* __restrict__ b,
+                                                                   const T* __restrict__ dy, const T* __restrict__ x,
+                                                                   const float* __restrict__ w, const float* __restrict__ b,
                                                                    const float* __restrict__ mean,
                                                                    const float* __restrict__ rstd, int relu,
                                                                    T* __restrict__ dx, float* __restrict__ part_w,
@@ -237,7 +238,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     const T* const px_ = x + at.b * cloud;
     const T* const pd_ = dy + at.b * cloud;
     T* const po_ = dx + at.b * cloud;
-    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T), ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
+    const unsigned o = (unsigned)(cy * M + at.m0) * (unsigned)sizeof(T);
+    const unsigned ol = (unsigned)(clast * M + at.m0) * (unsigned)sizeof(T);
     raw4<T> rx[KR], rd[KR];
     float mu[PTS], rs[PTS], s[2 * PTS];
 #pragma unroll

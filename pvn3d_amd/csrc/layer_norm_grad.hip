@@ -12,7 +12,7 @@ using ln::row_sum;
 // As the forward; a thread's channels are the same for all its rows, so dw and db are summed in its registers over the
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
 // Bound by HBM: dy and x read, dx written, once each.  bf16 786432 x 128: 115 us = 5.2 TB/s; 393216 x 196 from 8 bits: 100 us
-// = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of 1024 to 2048 partials another 5 us.
+// = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of the partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
 __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
@@ -172,11 +172,18 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
   }
 }
 
-// workgroups of a rows backward launch = its partial sums; a call of a few passes' rows is one workgroup's, which writes dw
-// and db itself (no second launch)
-int rows_grad_parts(int dtype, long long rows, int C) {
-  const long long n = ln::rows_blocks(rows, ln::rows_threads(C, ln::vec_of(dtype)), 1);
-  return (int)(n <= 8 ? 1 : n < ln::MAX_PARTS ? n : ln::MAX_PARTS);
+// Workgroups of a rows backward launch = its partial sums: what the registers let stay on the chip (`resident` a CU), each
+// with four rows at least where it takes a row at a time.  bf16 16384 x 4096: 100 us,
+// 125 with twice as many, 137 with 2048; 46000 x 753: 45, 51, 57; 2000 x 1536: 19, 19, 36; 786432 x 128: 119, 122, 122.
+// A call of a few passes' rows is one workgroup's, which writes dw and db itself (no second launch).
+int rows_grad_parts(int dtype, long long rows, int C, bool from8) {
+  const int vec = ln::vec_of(dtype), tpr = ln::rows_threads(C, vec), k = (C + tpr * vec - 1) / (tpr * vec);
+  int resident;
+  if (vec == 8) resident = k == 1 ? 4 : k == 2 ? 3 : 1;
+  else resident = k == 1 ? 8 - from8 : k == 2 ? (tpr == 64 ? 5 : 5 - from8) : k <= 4 ? 2 : 1;
+  if (ln::rows_blocks(rows, tpr, 1) <= 8) return 1;
+  const long long n = tpr == 256 ? (rows + 3) / 4 : ln::rows_blocks(rows, tpr, k == 1 ? 2 : 1);
+  return (int)(n < 256 * resident ? n : 256 * resident);
 }
 
 template <typename T>
@@ -188,14 +195,14 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
   do {                                                                                                                   \
     if (codes)                                                                                                           \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, true>), dim3(parts), dim3(256), 0, st, rows, C,              \
-                         (const T*)dy, (int)dys, (const T*)nullptr, 0, (const signed char*)codes, (int)pitch,                    \
-                         (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, (int)dxs,  \
-                         dxcols, pw, pb, ps);                                                                               \
+                         (const T*)dy, (int)dys, (const T*)nullptr, 0, (const signed char*)codes, (int)pitch,            \
+                         (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx,       \
+                         (int)dxs, dxcols, pw, pb, ps);                                                                  \
     else                                                                                                                 \
       hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, false>), dim3(parts), dim3(256), 0, st, rows, C,             \
-                         (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)nullptr, 0,                           \
+                         (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)nullptr, 0,                   \
                          (const unsigned char*)nullptr, (const unsigned char*)nullptr, w, b, mean, rstd, relu, (T*)dx,   \
-                         (int)dxs, dxcols, pw, pb, ps);                                                                          \
+                         (int)dxs, dxcols, pw, pb, ps);                                                                  \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
@@ -207,7 +214,7 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
 
 extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C) {
   if (rows <= 0 || C <= 0 || C > ln::MAX_C || dtype < 0 || dtype > 2) return 0;
-  const int parts = rows_grad_parts(dtype, rows, C);
+  const int parts = rows_grad_parts(dtype, rows, C, false);            // (from 8 bits: as many or fewer)
   return parts > 1 ? (size_t)parts * 2 * C * sizeof(float) : 0;
 }
 extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x,
@@ -230,19 +237,16 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
     return 0;
   }
   if (!dy || (!x && !codes) || !mean || !rstd) return (int)hipErrorInvalidValue;
-  const int parts = rows_grad_parts(dtype, rows, C);
+  const int parts = rows_grad_parts(dtype, rows, C, codes != nullptr);
   if (dweight && parts > 1 && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
     return (int)hipErrorInvalidValue;
   float* const part = (float*)workspace;
   float* const pw = !dweight ? nullptr : parts > 1 ? part : dweight;
   float* const pb = !dweight ? nullptr : parts > 1 ? part + C : dbias;
   const size_t ps = parts > 1 ? 2 * (size_t)C : 0;
-  int rc;
-  switch (dtype) {
-    case 0: rc = rows_backward<float>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
-    case 1: rc = rows_backward<bf16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
-    default: rc = rows_backward<fp16>(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs, dx_cols, pw, pb, ps, (hipStream_t)stream); break;
-  }
+  const auto run = dtype == 0 ? rows_backward<float> : dtype == 1 ? rows_backward<bf16> : rows_backward<fp16>;
+  const int rc = run(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs,
+                     dx_cols, pw, pb, ps, (hipStream_t)stream);
   if (rc || !dweight || parts == 1) return rc;
   return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, (hipStream_t)stream);
 }

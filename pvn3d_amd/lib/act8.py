@@ -6,8 +6,9 @@ launch each, plus one that joins the row splits of a weight gradient (csrc/act8.
 
 The 8-bit form: 32 consecutive channels of a row (the last group of a row may be shorter) share a power of two 2^e and a
 value x is held as the int8 code rint(x 2^-e); e >= -126 is the smallest exponent at which the group's largest magnitude
-rounds to 127 at most, held as e + 127 in a byte (e <= 121: magnitudes from 127.5 2^121 on are held as 127 2^121).  A value is off by at most half a step, 1/128 of its group's largest
-magnitude; every held value is exact in bfloat16.  A group that holds an infinity or a NaN comes back as NaN.
+rounds to 127 at most, held as e + 127 in a byte (e <= 121: magnitudes from 127.5 2^121 on are held as 127 2^121).  A value
+is off by at most half a step, 1/128 of its group's largest magnitude (half of 2^-126 in a group smaller than that); every
+held value is exact in bfloat16.  A group that holds an infinity or a NaN comes back as NaN.
 
 Everything runs on the current stream of the tensors' device and reads only its arguments; calls may be captured."""
 import torch

@@ -561,7 +561,8 @@ def sa_level_train(module, xyz, new_xyz, features, idxs):
         layers = shared_mlp_layers(mlp)
         if layers is None or not isinstance(grouper, pointnet2_utils.QueryAndGroup) or idx is None:
             return None
-        if idx.size(2) > (MAX_NSAMPLE_LN if _is_ln(layers) else MAX_NSAMPLE) or max([c_feat + 3] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16:
+        if (idx.size(2) > (MAX_NSAMPLE_LN if _is_ln(layers) else MAX_NSAMPLE)
+                or max([c_feat + 3] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16):
             return None
         if features is None and not grouper.use_xyz:
             return None

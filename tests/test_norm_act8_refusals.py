@@ -64,7 +64,8 @@ def test_act8_entry_points_refuse():
         assert lib.pvn3d_act8_unpack(*a, None) != 0, a
     for a in ((4, -1, 8, P, 8, P, 16, P, P, None, 0), (4, 8, 8, P, -8, P, 16, P, P, None, 0), (4, 8, 8, P, 8, P, 8, P, P, None, 0),
               (4, 8, 8, None, 8, P, 16, P, P, None, 0), (4, 8, 8, P, 8, P, 16, P, None, None, 0),
-              (1 << 20, 8, 8, P, 8, P, 16, P, P, None, 0)):                   # row splits without their workspace
+              (1 << 20, 8, 8, P, 8, P, 16, P, P, None, 0),                    # row splits without their workspace
+              (1 << 20, 8, 8, P, 8, P, 16, P, P, P + 4, 1 << 40)):
         assert lib.pvn3d_act8_wgrad(*a, None) != 0, a
     assert lib.pvn3d_act8_pack(1, 0, 8, None, 8, None, 16, None, None) == 0
     assert lib.pvn3d_act8_wgrad(4, 0, 8, P, 0, P, 16, P, P, None, 0, None) == 0
