@@ -222,7 +222,8 @@ __global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t 
 #pragma unroll
       for (int j = 0; j < 8; ++j) get(i + j * SL, f[j]);
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] += ((f[0][j] + f[1][j]) + (f[2][j] + f[3][j])) + ((f[4][j] + f[5][j]) + (f[6][j] + f[7][j]));
+      for (int j = 0; j < W; ++j)
+        v[j] += ((f[0][j] + f[1][j]) + (f[2][j] + f[3][j])) + ((f[4][j] + f[5][j]) + (f[6][j] + f[7][j]));
     }
     for (; i < P; i += SL) {
       float f[W];
@@ -253,12 +254,14 @@ __global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t 
 }
 static inline int fold(int P, size_t count, size_t first, const float* part, float* a, float* b, hipStream_t st) {
   // slices: as many as leave a thread about eight partial sums (64 slices of 16 columns still read whole 64-byte lines);
-  // four columns a thread for few sums of many columns (16 of 512 x 1536: 50 MB)
+  // four columns a thread for many columns (256 sums of 256 x 128: 7.1 us with 32 slices, 10.0 with 16; 64 sums of
+  // 512 x 256 the other way round, 9.0 and 7.4)
 #define RV_FOLD(SL, W)                                                                                                    \
   hipLaunchKernelGGL((fold_kernel<SL, W>), dim3((unsigned)((count + W * 1024 / SL - 1) / (W * 1024 / SL))), dim3(1024), 0, \
                      st, P, count, first, part, a, b)
   const bool wide = count >= 32768 && (count & 3) == 0;
-  if (wide && P >= 64) RV_FOLD(16, 4);
+  if (wide && P >= 128) RV_FOLD(32, 4);
+  else if (wide && P >= 64) RV_FOLD(16, 4);
   else if (wide && P >= 16) RV_FOLD(4, 4);
   else if (wide) RV_FOLD(2, 4);
   else if (P >= 256) RV_FOLD(64, 1);

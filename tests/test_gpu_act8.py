@@ -231,6 +231,53 @@ def test_captured(dev):
         assert all(torch.equal(p, q) for p, q in zip(out, step()))
 
 
+def test_more_than_32_bits_of_elements(dev):
+    """Row offsets beyond 2^31 elements: pack, unpack and the weight gradient of a matrix that is zero but for a few rows."""
+    rows, C, M = (1 << 21) + 35, 1032, 24
+    x = torch.zeros((rows, C), dtype=torch.bfloat16, device=dev)
+    dy = torch.ones((rows, M), dtype=torch.bfloat16, device=dev)
+    pick = [0, 1, rows // 2, rows - 33, rows - 2, rows - 1]
+    g = torch.Generator().manual_seed(15)
+    x[pick] = torch.randn(len(pick), C, generator=g).to(torch.bfloat16).to(dev)
+    dy[pick] = torch.randn(len(pick), M, generator=g).to(torch.bfloat16).to(dev)
+    act = act8.act8_pack(x)
+    held = _held(x[pick])
+    out = act8.act8_unpack(act)
+    assert torch.equal(out[pick].double().cpu(), held) and int((out != 0).any(1).sum()) == len(pick)
+    dw = act8.linear8_weight_grad(dy, act).double().cpu()
+    a = dy[pick].double().cpu()
+    # six terms and zeros: a rounding of 2^-24 each of the terms' sizes
+    assert bool(((dw - a.t() @ held).abs() <= 8 * 2.0 ** -24 * (a.abs().t() @ held.abs())).all())
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Calls in flight together on two streams share nothing."""
+    g = torch.Generator().manual_seed(16)
+    sets = []
+    for rows, C, M in ((60000, 128, 96), (50001, 99, 70)):
+        x = torch.randn(rows, C, generator=g).to(torch.bfloat16).to(dev)
+        dy = torch.randn(rows, C, generator=g).to(torch.bfloat16).to(dev)
+        d2 = torch.randn(rows, M, generator=g).to(torch.bfloat16).to(dev)
+        w, b = torch.rand(C, generator=g).to(dev), torch.rand(C, generator=g).to(dev)
+        sets.append((x, dy, d2, w, b))
+
+    def step(x, dy, d2, w, b):
+        y, s = ln.layer_norm_forward8(x, w, b, relu=True)
+        return (y,) + ln.layer_norm_backward8(dy, s, w) + (act8.linear8_weight_grad(d2, s.act),)
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(p, q) for p, q in zip(r, want[i]))
+
+
 @pytest.mark.parametrize("dims", [(64, 96, 32), (33, 50, 7)])
 def test_a_training_pass_captured(dev, dims):
     """The differentiable calls together, forward and backward in one captured graph, replayed with other inputs."""
