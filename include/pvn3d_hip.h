@@ -648,7 +648,7 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
  * var + eps has to be a normal fp32 number (a smaller one counts as zero, and its points are not finite).  Outputs do not
  * overlap inputs.
- * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^23 (or 0); mean, rstd (B, M). */
+ * pvn3d_layer_norm_chan(_grad): the same for contiguous (B, C, M) tensors, 4 <= M <= 2^22 (or 0); mean, rstd (B, M). */
 int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x, long long xs, const float* weight, const float* bias,
                      float eps, int relu, void* y, long long ys, int y_cols, float* mean, float* rstd, void* codes,
                      long long pitch, void* scales, void* mask, void* stream);

@@ -1,8 +1,8 @@
 // layer_norm_chan.hip -- layer norm over the channels of (B, C, M) tensors, M contiguous: the layout in which the modules
 // hand features on.  The formulas are those of layer_norm.hip.
 //
-// A tile is 64 (32) consecutive points of one cloud: PX = 16 (8) lanes x 4 points across, blockDim.x / PX channel slots
-// down.  A thread holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
+// A tile is 64 (32, 16) consecutive points of one cloud: PX = 16 (8, 4) lanes x 4 points across, blockDim.x / PX channel
+// slots down.  A thread holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
 // is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
 // every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
 // exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more channels than the registers of 1024 threads hold
@@ -62,8 +62,8 @@ __device__ __forceinline__ void forget<float>(raw4<float>& a) {
 // where neighbouring tiles share memory lines each XCD walks a run of an eighth of the tiles with all its workgroups.
 struct tile_walk {
   int at, step, end;
-  __device__ __forceinline__ tile_walk(int tiles, int runs) {
-    const int g = gridDim.x, b = blockIdx.x;
+  __device__ __forceinline__ tile_walk(int tiles, int runs, int g) {
+    const int b = blockIdx.x;
     if (!runs) {
       at = b;
       step = g;
@@ -96,7 +96,8 @@ __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[PX * N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane & (PX - 1), waves = blockDim.x >> 6;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (PX == 8) s[i] += __uint_as_float(rv::turn8(__float_as_uint(s[i])));
+    if (PX <= 8) s[i] += __uint_as_float(rv::turn8(__float_as_uint(s[i])));
+    if (PX == 4) s[i] += __uint_as_float(rv::turn4(__float_as_uint(s[i])));
     s[i] = rv::add32(rv::add16(s[i]));
   }
   if (lane < PX) {
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
     bk[k] = KC > 0 && b && has[k] ? b[c] : 0.f;
   }
   const int clast = KC > 0 ? min(cy, C - 1 - (KR - 1) * CY) : 0;
-  const tile_walk walk(tiles, runs);
+  const tile_walk walk(tiles, runs, gridDim.x);
   for (int tile = walk.at; tile < walk.end; tile += walk.step) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const p = x + at.b * cloud;
@@ -201,14 +202,62 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
 
 // dw / db: a thread has the same channels for all its tiles: a register each, summed over the 16 lanes at the end (KC = 0:
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
-template <typename T, int KC, int PX>
+// CHANNELS: the call has channel workgroups (an instance of its own: they take registers).
+template <typename T, int KC, int PX, bool CHANNELS>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int runs, int per_cloud, int C, int M,
                                                                    const T* __restrict__ dy, const T* __restrict__ x,
                                                                    const float* __restrict__ w, const float* __restrict__ b,
                                                                    const float* __restrict__ mean,
                                                                    const float* __restrict__ rstd, int relu,
                                                                    T* __restrict__ dx, float* __restrict__ part_w,
-                                                                   float* __restrict__ part_b, size_t part_stride) {
+                                                                   float* __restrict__ part_b, size_t part_stride,
+                                                                   int tile_blocks) {
+  if (CHANNELS && (int)blockIdx.x >= tile_blocks) {       // a channel workgroup: a wave for dw and db of a channel
+    const int lane = threadIdx.x & 63, c = ((blockIdx.x - tile_blocks) * blockDim.x + threadIdx.x) >> 6;
+    if (c >= C) return;
+    const float g = w ? w[c] : 1.f, be = b ? b[c] : 0.f;
+    const int per = (M + PTS - 1) / PTS, clouds = tiles / per_cloud, chunks = clouds * per;
+    float w1 = 0.f, b1 = 0.f;
+    for (int base = lane; base < chunks; base += 2 * 64) {
+      raw4<T> rx[2], rd[2];
+      rv::u4_any mu_[2], rs_[2];
+      int skip[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int q = min(base + r * 64, chunks - 1), cl = q / per, m = (q - cl * per) * PTS, m0 = min(m, M - PTS);
+        const size_t at = ((size_t)cl * C + c) * M + m0, point = (size_t)cl * M + m0;
+        skip[r] = base + r * 64 < chunks ? m - m0 : PTS;
+        rx[r] = *reinterpret_cast<const raw4<T>*>(x + at);
+        rd[r] = *reinterpret_cast<const raw4<T>*>(dy + at);
+        mu_[r] = *reinterpret_cast<const rv::u4_any*>(mean + point);
+        rs_[r] = *reinterpret_cast<const rv::u4_any*>(rstd + point);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v[PTS], d[PTS], mu[PTS], rs[PTS];
+        open<T>(rx[r], v);
+        open<T>(rd[r], d);
+        traits<float>::unpack(mu_[r], mu);
+        traits<float>::unpack(rs_[r], rs);
+#pragma unroll
+        for (int i = 0; i < PTS; ++i) {
+          const float xh = (v[i] - mu[i]) * rs[i];
+          const bool off_ = relu && fmaf(xh, g, be) <= 0.f;
+          const float dz = i >= skip[r] && !off_ ? d[i] : 0.f;
+          w1 = fmaf(dz, xh, w1);
+          b1 += dz;
+        }
+      }
+    }
+    w1 = rv::lanes_sum<64>(w1);
+    b1 = rv::lanes_sum<64>(b1);
+    if (lane == 0) {
+      part_w[c] = w1;
+      part_b[c] = b1;
+    }
+    return;
+  }
   constexpr int KR = KC > 0 ? KC : 1;
   __shared__ float buf[2][MAX_THREADS / 64][PX * 2 * PTS];
   extern __shared__ float lacc[];
@@ -232,7 +281,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     __syncthreads();
   }
   int turn = 0;
-  const tile_walk walk(tiles, runs);
+  const tile_walk walk(tiles, runs, tile_blocks);
   for (int tile = walk.at; tile < walk.end; tile += walk.step, turn ^= 1) {
     const tile_at<PX> at(tile, per_cloud, M);
     const T* const px_ = x + at.b * cloud;
@@ -347,7 +396,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
       }
     }
   }
-  if (!part_w) return;
+  if (CHANNELS || !part_w) return;
   float* const pw = part_w + blockIdx.x * part_stride;
   float* const pb = part_b + blockIdx.x * part_stride;
   if (KC > 0) {
@@ -370,19 +419,22 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
   }
 }
 
+constexpr int MAX_HELD = 2048;             // channels that the registers of a workgroup hold
 // lanes across, threads and channels per thread: 16 lanes and 16 channel slots up to 128 channels, then eight channels a
 // slot (8 x 196 x 16384 in bf16, backward: 39.5 us; with six channels a slot and more slots 51.4, with four 52.9); from 257
-// channels 8 lanes, so that two workgroups of them still share a CU; beyond 1024 channels x is read again for every pass
+// channels 8 lanes, so that two workgroups of them still share a CU, from 1025 4 (8 x 1536 x 2048 in bf16: forward 25 us,
+// backward 63; 42 and 65 with x read again for every pass, which is left for more than 2048)
 struct chan_plan { int px, threads, kc; };
 chan_plan chan_shape(int C) {
   chan_plan p;
-  p.px = C > 256 && C <= 1024 ? 8 : 16;
+  p.px = C > MAX_HELD ? 16 : C > 1024 ? 4 : C > 256 ? 8 : 16;
   int cy = 16;
-  if (p.px == 8) cy = (C + 63) / 64 * 8;
-  else if (C > 1024) cy = 64;
+  if (p.px == 4) cy = (C + 127) / 128 * 16;
+  else if (p.px == 8) cy = (C + 63) / 64 * 8;
+  else if (C > MAX_HELD) cy = 64;
   else if (C > 128) cy = (C + 31) / 32 * 4;
   p.threads = cy * p.px;
-  p.kc = C > 1024 ? 0 : (C + cy - 1) / cy;
+  p.kc = C > MAX_HELD ? 0 : (C + cy - 1) / cy;
   return p;
 }
 int cloud_tiles(int C, int M) { return (int)(((long long)M + chan_shape(C).px * PTS - 1) / (chan_shape(C).px * PTS)); }
@@ -396,21 +448,31 @@ bool chan_runs(int elem, int C, int M, int line, long long grid) {
 }
 // workgroups of a backward launch: what is on the chip at once (every one starts with the parameters and ends with its
 // partial sums): by its registers 32 waves a CU with two or three channels a thread, 16 with more (one: 16 are
-// the faster, 24 x 16 x 65536 fp32 61 us against 72).  A few tiles are one workgroup's, which writes dw and db itself.
+// the faster, 24 x 16 x 65536 fp32 61 us against 72).
 int chan_grad_parts(int B, int C, int M) {
   const chan_plan p = chan_shape(C);
   const long long n = chan_tiles(B, C, M), most = 256 * (long long)((p.kc == 2 || p.kc == 3 ? 2048 : 1024) / p.threads);
-  return (int)(n <= 4 ? 1 : n < 8 ? n : n < most ? (n + 7) / 8 * 8 : most);
+  return (int)(n < 8 ? n : n < most ? (n + 7) / 8 * 8 : most);
 }
-constexpr int MAX_POINTS = 1 << 23;        // per cloud: 128 channel slots (chan_shape) of them are within 32-bit byte offsets
+// Channel workgroups of a backward call: as for rows (layer_norm_grad.hip), a call of few points is one launch, with a wave
+// for every channel that goes through its points again for dw and db (4 x 64 x 500: 15 us a call, 19 with two launches;
+// 1 x 256 x 8192: 15.5, 19; 1 x 512 x 8192: 19, 19; 1 x 64 x 16384: 24, 19).
+int chan_grad_channels(int B, int C, int M) {
+  const long long points = (long long)B * M;
+  const int waves = chan_shape(C).threads / 64;
+  return points <= 8192 && points * C <= 1 << 21 ? (C + waves - 1) / waves : 0;
+}
+constexpr int MAX_POINTS = 1 << 22;        // per cloud: 256 channel slots (chan_shape) of them are within 32-bit byte offsets
 bool chan_ok(int dtype, int B, int C, int M) {
   return dtype >= 0 && dtype <= 2 && C > 0 && C <= ln::MAX_C && B >= 0 && (M == 0 || (M >= PTS && M <= MAX_POINTS)) &&
          chan_tiles(B, C, M) < 0x7fffffffLL - 16384;
 }
 
-// (8 lanes: seven or eight channels a slot come of 257 to 1024 channels)
+// (8 lanes: seven or eight channels a slot come of 257 to 1024 channels; 4 lanes: eight)
 #define LN_CHAN_PICK(CALL)                          \
-  if (p.px == 8) {                                  \
+  if (p.px == 4) {                                  \
+    CALL(8, 4);                                     \
+  } else if (p.px == 8) {                           \
     if (p.kc <= 7) CALL(7, 8);                      \
     else CALL(8, 8);                                \
   } else {                                          \
@@ -444,20 +506,27 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
 }
 
 template <typename T>
-int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x, const float* w, const float* b,
+int chan_backward(int parts, int channels, int B, int C, int M, const void* dy, const void* x, const float* w, const float* b,
                   const float* mean, const float* rstd, int relu, void* dx, float* pw, float* pb, size_t ps, hipStream_t st) {
   const chan_plan p = chan_shape(C);
   const int lds = p.kc ? 0 : (int)(2 * C * sizeof(float));
   if (!p.kc) {
-    const int rc = pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16>);
+    const int rc = channels ? pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, true>)
+                            : pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, false>);
     if (rc) return rc;
   }
-#define LN_CALL(KC, PX)                                                                                                     \
-  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX>), dim3(parts), dim3(p.threads), lds, st, (int)chan_tiles(B, C, M),     \
-                     (int)chan_runs(sizeof(T), C, M, 128, parts),                                                           \
-                     cloud_tiles(C, M), C, M, (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, pw, pb, ps)
+#define LN_ONE(KC, PX, CHANNELS)                                                                                            \
+  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX, CHANNELS>), dim3(parts + channels), dim3(p.threads), lds, st,          \
+                     (int)chan_tiles(B, C, M), (int)chan_runs(sizeof(T), C, M, 128, parts), cloud_tiles(C, M), C, M,        \
+                     (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, pw, pb, ps, parts)
+#define LN_CALL(KC, PX)                  \
+  do {                                   \
+    if (channels) LN_ONE(KC, PX, true);  \
+    else LN_ONE(KC, PX, false);          \
+  } while (0)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
+#undef LN_ONE
   PVN3D_LAUNCH_CHECK();
   return 0;
 }
@@ -466,8 +535,7 @@ int chan_backward(int parts, int B, int C, int M, const void* dy, const void* x,
 
 extern "C" size_t pvn3d_layer_norm_chan_grad_workspace_bytes(int dtype, int B, int C, int M) {
   if (!chan_ok(dtype, B, C, M) || B == 0 || M == 0) return 0;
-  const int parts = chan_grad_parts(B, C, M);
-  return parts > 1 ? (size_t)parts * 2 * C * sizeof(float) : 0;
+  return chan_grad_channels(B, C, M) ? 0 : (size_t)chan_grad_parts(B, C, M) * 2 * C * sizeof(float);
 }
 
 extern "C" int pvn3d_layer_norm_chan(int dtype, int B, int C, int M, const void* x, const float* weight, const float* bias,
@@ -499,19 +567,15 @@ extern "C" int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const 
     return 0;
   }
   if (!dy || !x || !mean || !rstd) return (int)hipErrorInvalidValue;
-  const int parts = chan_grad_parts(B, C, M);
-  if (dweight && parts > 1 && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
+  const int channels = dweight ? chan_grad_channels(B, C, M) : 0;
+  const int parts = dx || !channels ? chan_grad_parts(B, C, M) : 0;
+  if (dweight && !channels && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
     return (int)hipErrorInvalidValue;
   float* const part = (float*)workspace;
-  float* const pw = !dweight ? nullptr : parts > 1 ? part : dweight;
-  float* const pb = !dweight ? nullptr : parts > 1 ? part + C : dbias;
-  const size_t ps = parts > 1 ? 2 * (size_t)C : 0;
-  int rc;
-  switch (dtype) {
-    case 0: rc = chan_backward<float>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
-    case 1: rc = chan_backward<bf16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
-    default: rc = chan_backward<fp16>(parts, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, ps, st); break;
-  }
-  if (rc || !dweight || parts == 1) return rc;
+  float* const pw = dweight && !channels ? part : dweight;
+  float* const pb = dweight && !channels ? part + C : dbias;
+  const auto run = dtype == 0 ? chan_backward<float> : dtype == 1 ? chan_backward<bf16> : chan_backward<fp16>;
+  const int rc = run(parts, channels, B, C, M, dy, x, weight, bias, mean, rstd, relu, dx, pw, pb, 2 * (size_t)C, st);
+  if (rc || !dweight || channels) return rc;
   return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, st);
 }

@@ -8,6 +8,8 @@ using rv::fp16;
 using rv::traits;
 using ln::row_sum;
 
+constexpr int ACROSS = 2;                            // chunks across of a column workgroup
+
 // ------------------------------------------------------------------------------------------------ rows, backward
 // As the forward; a thread's channels are the same for all its rows, so dw and db are summed in its registers over the
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
@@ -15,7 +17,7 @@ using ln::row_sum;
 // = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of the partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
-__global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
+__global__ __launch_bounds__(256, traits<T>::VEC == 8 && K == 2 ? 3 : 1) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
                                                            const T* __restrict__ x, int xs,
                                                            const signed char* __restrict__ codes, int pitch,
                                                            const unsigned char* __restrict__ scales,
@@ -24,15 +26,115 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                            int relu, T* __restrict__ dx, int dxs, int dxcols,
                                                            float* __restrict__ part_w, float* __restrict__ part_b,
-                                                           size_t part_stride) {
+                                                           size_t part_stride, int row_blocks) {
   constexpr int VEC = traits<T>::VEC;
   constexpr int RPB = 256 / TPR;
   constexpr int COLS = TPR * K * VEC;
   __shared__ float red[4];
-  __shared__ float fold[TPR > 64 ? 1 : 4 * COLS];
+  constexpr int OWN = TPR > 64 ? 0 : 4 * COLS, COLUMN = 8 * ACROSS * VEC;        // of a row, a column workgroup
+  __shared__ float fold[OWN > COLUMN ? OWN : COLUMN];
   const int t = threadIdx.x % TPR, rg = threadIdx.x / TPR;
   const int G = (C + rv::GROUP - 1) / rv::GROUP, MB = (C + 7) / 8;
   const bool ragged = (C & (VEC - 1)) != 0;
+  // one chunk's dy and x (or codes, scales, ReLU bits) -> xh and dz
+  auto terms = [&](const rv::u4_any& rd, const rv::u4_any& rx, const unsigned (&cw)[VEC / 4], const unsigned char (&sc)[2],
+                   const unsigned char (&mk)[2], int at, int skip, float mu, float rs, bool live, const float (&g)[VEC],
+                   const float (&be)[VEC], float (&xh)[VEC], float (&dz)[VEC]) {
+    traits<T>::unpack(rd, dz);
+    if (!FROM8) traits<T>::unpack(rx, xh);
+    const float a = FROM8 ? rv::group_step(sc[0]) : 0.f, a0 = FROM8 && ragged ? rv::group_step(sc[1]) : a;
+    unsigned bits = 0xffffffffu;
+    if (FROM8 && mask) bits = ((unsigned)mk[0] | (ragged ? (unsigned)mk[1] << 8 : 0u)) >> (at & 7);
+    if (FROM8 && !live) bits = 0u;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float xm = FROM8 ? fmaf(rv::code_at(cw, i), i < skip ? a0 : a, -mu) : xh[i] - mu;
+      xh[i] = xm * rs;
+      if (FROM8) {
+        // bit i as a mask of the whole word
+        const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)bits, i, 1);
+        dz[i] = __uint_as_float(__float_as_uint(dz[i]) & on);
+      } else {
+        const bool off_ = relu && fmaf(xh[i], g[i], be[i]) <= 0.f;          // (a NaN passes, as in the forward)
+        dz[i] = live && !off_ ? dz[i] : 0.f;
+      }
+    }
+  };
+  if ((int)blockIdx.x >= row_blocks) {                 // a column workgroup: dw and db of ACROSS chunks of columns
+    constexpr int SLOTS = 256 / ACROSS, FLY = 2;
+    const int slot = threadIdx.x / ACROSS;
+    const ln::lane_cols<T, TPR, 1> col((blockIdx.x - row_blocks) * ACROSS + threadIdx.x % ACROSS, C);
+    float g[1][VEC], be[1][VEC], aw[VEC], ab[VEC];
+    col.params(w, 1.f, C, g);
+    col.params(b, 0.f, C, be);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { aw[i] = 0.f; ab[i] = 0.f; }
+    for (int base = slot; base < rows; base += SLOTS * FLY) {
+      rv::u4_any rx[FLY], rd[FLY];
+      float mu[FLY], rs[FLY];
+      unsigned cw[FLY][VEC / 4];
+      unsigned char sc[FLY][2], mk[FLY][2];
+#pragma unroll
+      for (int r = 0; r < FLY; ++r) {
+        const long long row = min(base + r * SLOTS, (int)rows - 1);
+        mu[r] = mean[row];
+        rs[r] = rstd[row];
+        rd[r] = col.load(dy + row * dys, 0, 0, C);
+        if (FROM8) {
+          const int c = min(col.c[0], (C - 1) & ~(VEC - 1)), at = col.at[0];
+          rv::load_codes(codes + row * pitch + at, cw[r]);
+          sc[r][0] = scales[row * G + c / rv::GROUP];
+          if (ragged) sc[r][1] = scales[row * G + at / rv::GROUP];
+          if (mask) mk[r][0] = mask[row * MB + at / 8];
+          if (mask && ragged) mk[r][1] = mask[row * MB + min(at / 8 + 1, MB - 1)];
+        } else {
+          rx[r] = col.load(x + row * xs, 0, 0, C);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < FLY; ++r) {
+        float xh[VEC], dz[VEC];
+        terms(rd[r], rx[r], cw[r], sc[r], mk[r], col.at[0], col.skip[0], mu[r], rs[r], base + r * SLOTS < rows, g[0], be[0], xh,
+              dz);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          aw[i] = fmaf(dz[i], xh[i], aw[i]);
+          ab[i] += dz[i];
+        }
+      }
+    }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+      for (int o = ACROSS; o < 64; o <<= 1) {
+        aw[i] += __shfl_xor(aw[i], o, 64);
+        ab[i] += __shfl_xor(ab[i], o, 64);
+      }
+      if (lane < ACROSS) {
+        fold[((2 * wave) * ACROSS + lane) * VEC + i] = aw[i];
+        fold[((2 * wave + 1) * ACROSS + lane) * VEC + i] = ab[i];
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < ACROSS && col.c[0] < C) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (col.own[0][i] != 0.f) {
+          float s[2];
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            const float* const f = fold + (which * ACROSS + threadIdx.x) * VEC + i;
+            constexpr int W = 2 * ACROSS * VEC;
+            s[which] = (f[0] + f[W]) + (f[2 * W] + f[3 * W]);
+          }
+          part_w[col.at[0] + i] = s[0];
+          part_b[col.at[0] + i] = s[1];
+        }
+    }
+    return;
+  }
   const ln::lane_cols<T, TPR, K> col(t, C);
   float g[K][VEC], be[K][VEC], aw[K][VEC], ab[K][VEC];
   col.params(w, 1.f, C, g);
@@ -45,7 +147,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       ab[k][i] = 0.f;
     }
   const float rc = 1.f / (float)C;
-  for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)gridDim.x * (RPB * R)) {
+  for (long long base = (long long)blockIdx.x * (RPB * R); base < rows; base += (long long)row_blocks * (RPB * R)) {
     const int last = (int)(rows - 1 - base < RPB * R - 1 ? rows - 1 - base : RPB * R - 1);
     const T* const db = dy + base * dys;
     const T* const xb = x + base * xs;
@@ -87,32 +189,17 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       float v[K][VEC], d[K][VEC], s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        traits<T>::unpack(rd[r][k], d[k]);
-        if (!FROM8) traits<T>::unpack(rx[r][k], v[k]);
-        const float a = FROM8 ? rv::group_step(sc[r][k][0]) : 0.f, a0 = FROM8 && ragged ? rv::group_step(sc[r][k][1]) : a;
-        unsigned bits = 0xffffffffu;
-        if (FROM8 && mask) bits = ((unsigned)mk[r][k][0] | (ragged ? (unsigned)mk[r][k][1] << 8 : 0u)) >> (col.at[k] & 7);
-        if (FROM8 && !live) bits = 0u;
+        terms(rd[r][k], rx[r][k], cw[r][k], sc[r][k], mk[r][k], col.at[k], col.skip[k], mu[r], rs[r], live, g[k], be[k], v[k],
+              d[k]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float xm = FROM8 ? fmaf(rv::code_at(cw[r][k], i), i < col.skip[k] ? a0 : a, -mu[r]) : v[k][i] - mu[r];
-          const float xh = xm * rs[r];
-          float dz;
-          if (FROM8) {
-            // bit i as a mask of the whole word
-            const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)bits, i, 1);
-            dz = __uint_as_float(__float_as_uint(d[k][i]) & on);
-          } else {
-            const bool off_ = relu && fmaf(xh, g[k][i], be[k][i]) <= 0.f;          // (a NaN passes, as in the forward)
-            dz = live && !off_ ? d[k][i] : 0.f;
-          }
+          const float xh = v[k][i], dz = d[k][i];
           aw[k][i] = fmaf(dz, xh, aw[k][i]);
           ab[k][i] += dz;
           const float u = dz * g[k][i], um = u * col.own[k][i];
           s1 += um;
           s2 = fmaf(um, xh, s2);
           d[k][i] = u;
-          v[k][i] = xh;
         }
       }
       if (dx) {
@@ -132,7 +219,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       }
     }
   }
-  if (!part_w) return;
+  if (!part_w || (int)gridDim.x > row_blocks) return;
   float* const pw = part_w + blockIdx.x * part_stride;
   float* const pb = part_b + blockIdx.x * part_stride;
   if (TPR > 64) {
@@ -172,40 +259,44 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
   }
 }
 
+// Column workgroups of a call.  A call of few rows is one launch: workgroups for dx, and one for every ACROSS chunks of
+// columns that goes through all the rows again (by then they are in a cache) for dw and db -- no partial sums, no second
+// launch, which costs the host 4 us.  512 x 512: 14 us a call, 18 with two launches; 2048 x 512: 14, 18; 4096 x 256: 19, 18;
+// 2048 x 1536: 24, 18.
+int rows_grad_columns(int dtype, long long rows, int C) {
+  const int wide = ACROSS * ln::vec_of(dtype);
+  return rows <= 2048 && rows * C <= 3 << 19 ? (C + wide - 1) / wide : 0;
+}
+
 // Workgroups of a rows backward launch = its partial sums: what the registers let stay on the chip (`resident` a CU), each
 // with four rows at least where it takes a row at a time.  bf16 16384 x 4096: 100 us,
 // 125 with twice as many, 137 with 2048; 46000 x 753: 45, 51, 57; 2000 x 1536: 19, 19, 36; 786432 x 128: 119, 122, 122.
-// A call of a few passes' rows is one workgroup's, which writes dw and db itself (no second launch).
 int rows_grad_parts(int dtype, long long rows, int C, bool from8) {
   const int vec = ln::vec_of(dtype), tpr = ln::rows_threads(C, vec), k = (C + tpr * vec - 1) / (tpr * vec);
   int resident;
   if (vec == 8) resident = k == 1 ? 4 : k == 2 ? 3 : 1;
   else resident = k == 1 ? 8 - from8 : k == 2 ? (tpr == 64 ? 5 : 5 - from8) : k <= 4 ? 2 : 1;
-  if (ln::rows_blocks(rows, tpr, 1) <= 8) return 1;
   const long long n = tpr == 256 ? (rows + 3) / 4 : ln::rows_blocks(rows, tpr, k == 1 ? 2 : 1);
   return (int)(n < 256 * resident ? n : 256 * resident);
 }
-
 template <typename T>
-int rows_backward(int parts, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
+int rows_backward(int parts, int columns, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
                   const void* codes, long long pitch, const void* scales, const void* mask, const float* w, const float* b,
                   const float* mean, const float* rstd, int relu, void* dx, long long dxs, int dxcols, float* pw, float* pb,
                   size_t ps, hipStream_t st) {
-#define LN_CALL(T, TPR, K, R)                                                                                            \
-  do {                                                                                                                   \
-    if (codes)                                                                                                           \
-      hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, true>), dim3(parts), dim3(256), 0, st, rows, C,              \
-                         (const T*)dy, (int)dys, (const T*)nullptr, 0, (const signed char*)codes, (int)pitch,            \
-                         (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx,       \
-                         (int)dxs, dxcols, pw, pb, ps);                                                                  \
-    else                                                                                                                 \
-      hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, false>), dim3(parts), dim3(256), 0, st, rows, C,             \
-                         (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)nullptr, 0,                   \
-                         (const unsigned char*)nullptr, (const unsigned char*)nullptr, w, b, mean, rstd, relu, (T*)dx,   \
-                         (int)dxs, dxcols, pw, pb, ps);                                                                  \
+#define LN_ONE(T, TPR, K, R, FROM8)                                                                                       \
+  hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, FROM8>), dim3(parts + columns), dim3(256), 0, st, rows, C,        \
+                     (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)codes, (int)pitch,                 \
+                     (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, (int)dxs,  \
+                     dxcols, pw, pb, ps, parts)
+#define LN_CALL(T, TPR, K, R)                   \
+  do {                                          \
+    if (codes) LN_ONE(T, TPR, K, R, true);      \
+    else LN_ONE(T, TPR, K, R, false);           \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
+#undef LN_ONE
   PVN3D_LAUNCH_CHECK();
   return 0;
 }
@@ -214,8 +305,8 @@ int rows_backward(int parts, long long rows, int C, const void* dy, long long dy
 
 extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C) {
   if (rows <= 0 || C <= 0 || C > ln::MAX_C || dtype < 0 || dtype > 2) return 0;
-  const int parts = rows_grad_parts(dtype, rows, C, false);            // (from 8 bits: as many or fewer)
-  return parts > 1 ? (size_t)parts * 2 * C * sizeof(float) : 0;
+  if (rows_grad_columns(dtype, rows, C)) return 0;
+  return (size_t)rows_grad_parts(dtype, rows, C, false) * 2 * C * sizeof(float);        // (from 8 bits: as many or fewer)
 }
 extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x,
                                      long long xs, const void* codes, long long pitch, const void* scales,
@@ -227,6 +318,7 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
     return (int)hipErrorInvalidValue;
   if (dx && (dx_cols < C || dx_cols > C + 15 || dxs < dx_cols)) return (int)hipErrorInvalidValue;
   if ((dweight == nullptr) != (dbias == nullptr) || (!dx && !dweight)) return (int)hipErrorInvalidValue;
+  if (!codes) scales = mask = nullptr;
   if (codes && (!scales || (pitch & 15) || pitch < C || (relu != 0) != (mask != nullptr))) return (int)hipErrorInvalidValue;
   if (rows <= 0) {
     if (dweight) {
@@ -237,16 +329,16 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
     return 0;
   }
   if (!dy || (!x && !codes) || !mean || !rstd) return (int)hipErrorInvalidValue;
-  const int parts = rows_grad_parts(dtype, rows, C, codes != nullptr);
-  if (dweight && parts > 1 && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
+  const int columns = dweight ? rows_grad_columns(dtype, rows, C) : 0;
+  const int parts = dx || !columns ? rows_grad_parts(dtype, rows, C, codes != nullptr) : 0;
+  if (dweight && !columns && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
     return (int)hipErrorInvalidValue;
   float* const part = (float*)workspace;
-  float* const pw = !dweight ? nullptr : parts > 1 ? part : dweight;
-  float* const pb = !dweight ? nullptr : parts > 1 ? part + C : dbias;
-  const size_t ps = parts > 1 ? 2 * (size_t)C : 0;
+  float* const pw = dweight && !columns ? part : dweight;
+  float* const pb = dweight && !columns ? part + C : dbias;
   const auto run = dtype == 0 ? rows_backward<float> : dtype == 1 ? rows_backward<bf16> : rows_backward<fp16>;
-  const int rc = run(parts, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx, dxs,
-                     dx_cols, pw, pb, ps, (hipStream_t)stream);
-  if (rc || !dweight || parts == 1) return rc;
+  const int rc = run(parts, columns, rows, C, dy, dys, x, xs, codes, pitch, scales, mask, weight, bias, mean, rstd, relu, dx,
+                     dxs, dx_cols, pw, pb, 2 * (size_t)C, (hipStream_t)stream);
+  if (rc || !dweight || columns) return rc;
   return rv::fold(parts, 2 * (size_t)C, C, part, dweight, dbias, (hipStream_t)stream);
 }

@@ -167,6 +167,8 @@ __device__ __forceinline__ unsigned dpp(unsigned v, int step) {
 }
 // lane ^ 8: a turn by eight within rows of 16 (row_ror:8)
 __device__ __forceinline__ unsigned turn8(unsigned v) { return __builtin_amdgcn_update_dpp(0u, v, 0x128, 0xf, 0xf, true); }
+// once lanes 8 apart hold the same: a turn by four makes lane ^ 4 of it
+__device__ __forceinline__ unsigned turn4(unsigned v) { return __builtin_amdgcn_update_dpp(0u, v, 0x124, 0xf, 0xf, true); }
 __device__ __forceinline__ float add16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);

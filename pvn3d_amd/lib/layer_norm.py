@@ -22,7 +22,7 @@ from .._lib import lib, check, on_device
 from .act8 import Act8, DTYPES, _like, _need, _rows, _stream
 
 MAX_CHANNELS = 8192
-MAX_POINTS = 1 << 23         # per cloud, of the channel-major kernels
+MAX_POINTS = 1 << 22         # per cloud, of the channel-major kernels
 
 
 def _param(p, C, x, name):

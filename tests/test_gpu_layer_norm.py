@@ -152,6 +152,70 @@ def test_many_rows_join_their_partial_sums(dev, C):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows,C", [(2048, 1), (2048, 99), (2047, 768), (2049, 1), (2050, 3), (2051, 7), (2060, 8), (2061, 17),
+                                    (2061, 33), (4500, 65), (9000, 100), (3001, 259), (2062, 513), (2100, 1000), (2200, 1030),
+                                    (1030, 2050), (520, 4100), (300, 8192)])
+def test_both_ways_to_the_parameters_gradients(dev, rows, C, dt):
+    """Around the border between one launch and partial sums: dx, dweight, dbias from x and from its 8-bit form, in rows of
+    a stride of their own."""
+    relu = rows % 2 == 1
+    x, dy, w, b = _make((rows, C + 3), C + 3, dt, dev, rows + C)
+    x, dy, w, b = x[:, :C], dy[:, 2:C + 2], w[:C].contiguous(), b[:C].contiguous()
+    wy, wm, wr, xh = _ref(x, w, b, False)
+    amp = _amp(x, wr)
+    zscale = xh.abs().max() * w.abs().max().double() + b.abs().max().double() + 1e-30
+    on = (wy > 0).double() if relu else torch.ones_like(wy)
+    if relu:
+        dy = torch.where(wy.abs() < 1e-4 * zscale * amp[..., None], torch.zeros_like(dy), dy)
+    y, mean, rstd = ln.layer_norm_forward(x, w, b, EPS, relu=relu)
+    got = ln.layer_norm_backward(dy, x, w, b, mean, rstd, relu=relu)
+    u = float(dy.abs().max()) * float(w.abs().max())
+    wdx, wdw, wdb = _ref_grad(dy, xh, wr, w, on)
+    _close(got[0], wdx, dt, scale=(wr * amp)[..., None] * u * (1 + xh.abs().max() ** 2))
+    _close(got[1], wdw, torch.float32, rows ** 0.5, dy.double().abs().max() * xh.abs().max() * amp.max())
+    _close(got[2], wdb, torch.float32, rows ** 0.5, dy.double().abs().max())
+    again = ln.layer_norm_backward(dy, x, w, b, mean, rstd, relu=relu)
+    only = ln.layer_norm_backward(dy, x, w, b, mean, rstd, relu=relu, need_dx=False)
+    assert all(torch.equal(p, q) for p, q in zip(got, again)) and torch.equal(only[1], got[1]) and torch.equal(only[2], got[2])
+    _, s = ln.layer_norm_forward8(x, w, b, EPS, relu=relu)
+    held = act8.act8_unpack(s.act, torch.float32).double()
+    xh8 = (held - mean.double()[:, None]) * rstd.double()[:, None]
+    got = ln.layer_norm_backward8(dy, s, w)
+    if relu:
+        on = (((s.mask[:, :, None].int() >> torch.arange(8, device=dev)) & 1).reshape(rows, -1)[:, :C]).double()
+    wdx, wdw, wdb = _ref_grad(dy, xh8, rstd.double(), w, on)
+    _close(got[0], wdx, dt, scale=rstd.double().max() * u * (1 + xh8.abs().max() ** 2))
+    _close(got[1], wdw, torch.float32, rows ** 0.5, dy.double().abs().max() * xh8.abs().max())
+    _close(got[2], wdb, torch.float32, rows ** 0.5, dy.double().abs().max())
+    only = ln.layer_norm_backward8(dy, s, w, need_dx=False)
+    assert torch.equal(only[1], got[1]) and torch.equal(only[2], got[2])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("B,C,M", [(2, 99, 4095), (1, 3, 8192), (3, 1, 2731), (5, 16, 1700), (1, 40, 8201), (11, 129, 770), (2, 256, 4101),
+                                   (2, 300, 4100), (1, 513, 4097), (2, 1024, 1100), (1, 1025, 2100), (3, 2048, 500),
+                                   (1, 2049, 1300), (40, 64, 5)])
+def test_both_ways_to_the_parameters_gradients_of_channels(dev, B, C, M, dt):
+    x, dy, w, b = _make((B, M, C), C, dt, dev, C + M)
+    xc, dyc = x.transpose(1, 2).contiguous(), dy.transpose(1, 2).contiguous()
+    y, mean, rstd = ln.layer_norm_forward(xc, w, b, EPS, channel_dim=1)
+    wy, wm, wr, xh = _ref(x, w, b, False)
+    amp = _amp(x, wr)
+    zscale = xh.abs().max() * w.abs().max().double() + b.abs().max().double() + 1e-30
+    _close(y.transpose(1, 2), wy, dt, scale=zscale * amp[..., None])
+    got = ln.layer_norm_backward(dyc, xc, w, b, mean, rstd, channel_dim=1)
+    wdx, wdw, wdb = _ref_grad(dy, xh, wr, w, 1.0)
+    u = float(dy.abs().max()) * float(w.abs().max())
+    _close(got[0].transpose(1, 2), wdx, dt, scale=(wr * amp)[..., None] * u * (1 + xh.abs().max() ** 2))
+    n = (B * M) ** 0.5
+    _close(got[1], wdw, torch.float32, n, dy.double().abs().max() * xh.abs().max() * amp.max())
+    _close(got[2], wdb, torch.float32, n, dy.double().abs().max())
+    again = ln.layer_norm_backward(dyc, xc, w, b, mean, rstd, channel_dim=1)
+    only = ln.layer_norm_backward(dyc, xc, w, b, mean, rstd, channel_dim=1, need_dx=False)
+    assert all(torch.equal(p, q) for p, q in zip(got, again)) and torch.equal(only[1], got[1]) and torch.equal(only[2], got[2])
+
+
+@pytest.mark.parametrize("dt", TYPES)
 def test_strides_and_views(dev, dt):
     g = torch.Generator().manual_seed(1)
     big = torch.randn(40, 3, 70, generator=g).to(dt).to(dev)

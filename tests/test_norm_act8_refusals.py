@@ -43,9 +43,9 @@ def test_layer_norm_entry_points_refuse():
         assert lib.pvn3d_layer_norm_chan(a["dtype"], a["B"], a["C"], a["M"], P, None, None, 1e-5, 0, P, P, P, None) != 0
         assert lib.pvn3d_layer_norm_chan_grad(a["dtype"], a["B"], a["C"], a["M"], P, P, None, None, P, P, 0, P, P, P, P,
                                               1 << 20, None) != 0
-    # more points a cloud than 128 channel slots of them have 32-bit offsets for
-    assert lib.pvn3d_layer_norm_chan(0, 1, 1024, (1 << 23) + 1, P, None, None, 1e-5, 0, P, P, P, None) != 0
-    assert lib.pvn3d_layer_norm_chan_grad(0, 1, 1024, (1 << 23) + 1, P, P, None, None, P, P, 0, P, P, P, P, 1 << 40, None) != 0
+    # more points a cloud than the channel slots of them have 32-bit offsets for
+    assert lib.pvn3d_layer_norm_chan(0, 1, 2048, (1 << 22) + 1, P, None, None, 1e-5, 0, P, P, P, None) != 0
+    assert lib.pvn3d_layer_norm_chan_grad(0, 1, 2048, (1 << 22) + 1, P, P, None, None, P, P, 0, P, P, P, P, 1 << 40, None) != 0
     assert lib.pvn3d_layer_norm_chan_grad(0, 200, 8, 400, P, P, None, None, P, P, 0, P, P, P, None, 0, None) != 0
     assert lib.pvn3d_layer_norm_chan(0, 0, 8, 4, P, None, None, 1e-5, 0, P, P, P, None) == 0
     # the workspace holds a partial dweight and dbias per workgroup
