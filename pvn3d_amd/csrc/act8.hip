@@ -147,10 +147,10 @@ __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride
 }
 
 // What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 46 us and 5 us for the sum of 768 partial tiles, 5.0 TB/s).
-// For wide ones LDS: a 256 x 128 tile's step of 64 rows reads and writes 176 KB of it (1400 cycles at 128 bytes a cycle) for
-// 1024 cycles of matrix instructions on every SIMD, and the two waves there overlap in part: 12288 rows, 512 x 1536 take
-// 34 us with the sum of the 33 MB of partial tiles, 556 TFLOP/s; 98304 rows, 512 x 512 76 us, 675 TFLOP/s (the library's
-// bf16 product: 81 and 311 us; its rate for a large square one: 1257 TFLOP/s).
+// For wide ones how much the two waves of a SIMD overlap: a step of 64 rows of the 256 x 128 tile keeps the matrix pipes busy
+// for 45 % of its cycles, LDS (176 KB) for 45 %, the vector units for 22 %.  12288 rows, 512 x 1536 take 34 us with the sum
+// of the 33 MB of partial tiles, 556 TFLOP/s; 98304 rows, 512 x 512 76 us, 675 TFLOP/s (the library's bf16 product: 81 and
+// 311 us; its rate for a large square one: 1257 TFLOP/s).
 constexpr int odd64(int cols) {                                  // row stride in elements: 32 times an odd number
   return ((cols / 32) & 1) ? cols : cols + 32;
 }
