@@ -146,14 +146,18 @@ def check(rc, what):
 import contextlib as _contextlib
 
 _NO_SWITCH = _contextlib.nullcontext()
+_torch = None
 
 
 def on_device(dev):
     """Context for a library call on `dev`: torch.cuda.device(dev) only when `dev` is not already the
     current device (entering / leaving that context costs two driver calls, ~10 us of host time per
     operator -- more than the short kernels of the small pyramid levels take)."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
     idx = dev.index
-    if idx is None or idx == torch.cuda.current_device():
+    if idx is None or idx == _torch._C._cuda_getDevice():      # (cuda.current_device() costs twice that)
         return _NO_SWITCH
-    return torch.cuda.device(dev)
+    return _torch.cuda.device(dev)

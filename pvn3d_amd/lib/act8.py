@@ -152,7 +152,7 @@ def act8_unpack(act, dtype=torch.bfloat16):
     _need(t is not None, "dtype must be float32, bfloat16 or float16")
     dev = act.device
     with on_device(dev):
-        out = torch.empty(act.shape, dtype=dtype, device=dev)
+        out = torch.empty(*act.shape, dtype=dtype, device=dev)
         codes, scales = act._ptrs()
         check(lib.pvn3d_act8_unpack(t, act.rows, act.channels, codes, act.pitch, scales, out.data_ptr(), act.channels,
                                     act.channels, _stream(out)), "act8_unpack")

@@ -22,15 +22,17 @@ from .._lib import lib, check, on_device
 from .act8 import Act8, DTYPES, _like, _need, _rows, _stream
 
 MAX_CHANNELS = 8192
+_F32, _U8 = torch.float32, torch.uint8
 MAX_POINTS = 1 << 22         # per cloud, of the channel-major kernels
 
 
 def _param(p, C, x, name):
     if p is None:
         return None
-    _need(p.dtype is torch.float32 and p.dim() == 1 and p.numel() == C,
-          "%s must be a float32 tensor of the channels' length", name)
-    _need(p.get_device() == x.get_device(), "%s must be on x's device", name)
+    if p.dtype is not _F32 or p.dim() != 1 or p.numel() != C:
+        raise RuntimeError("%s must be a float32 tensor of the channels' length" % name)
+    if p.get_device() != x.get_device():
+        raise RuntimeError("%s must be on x's device" % name)
     return p if p.is_contiguous() else p.contiguous()
 
 
@@ -79,7 +81,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
     with on_device(x.device):
         n = v.numel() // C
         y = _like(v)
-        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device).unbind()
+        mean, rstd = torch.empty(2, n, dtype=_F32, device=x.device).unbind()
         if rows:
             m, xs = _rows(v)
             check(lib.pvn3d_layer_norm(t, n, C, m.data_ptr(), xs, _ptr(w), _ptr(b), eps, 1 if relu else 0, y.data_ptr(), C, C,
@@ -95,8 +97,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu
 
 def _grad_buffers(C, wsb, dev):
     """dweight, dbias and the workspace of their partial sums."""
-    dw, db = torch.empty(2, C, dtype=torch.float32, device=dev).unbind()
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    dw, db = torch.empty(2, C, dtype=_F32, device=dev).unbind()
+    ws = torch.empty(wsb, dtype=_U8, device=dev) if wsb else None
     return dw, db, ws, dw.data_ptr(), db.data_ptr(), _ptr(ws)
 
 
