@@ -27,9 +27,18 @@ def _stream(t):
     return _raw_stream(t.get_device())
 
 
-def _need(ok, what, *args):
+def _need(ok, what):
     if not ok:
-        raise RuntimeError(what % args if args else what)
+        raise RuntimeError(what)
+
+
+def _dtype(t, name):
+    """The kernels' number of t's type; refuses CPU tensors and other types."""
+    _need(t.is_cuda, "CPU not supported")
+    d = DTYPES.get(t.dtype)
+    if d is None:
+        raise RuntimeError("%s must be a float32, bfloat16 or float16 tensor" % name)
+    return d
 
 
 MAX_STRIDE = 1 << 20        # row strides (in elements) that the kernels take; wider ones are copied
@@ -62,29 +71,30 @@ class Act8(object):
     __slots__ = ("_codes", "_scales", "_buf", "_at", "rows", "channels", "pitch", "shape", "device")
 
     def __init__(self, codes, scales, shape=None):
-        _need(codes.dim() == 2 and codes.dtype == torch.int8, "codes must be an int8 matrix")
-        rows, C = codes.shape
+        _need(codes.dtype is torch.int8 and codes.dim() == 2, "codes must be an int8 matrix")
+        rows, C = size = codes.shape
         _need(C > 0, "codes must have at least one channel")
-        _need(scales.dtype == torch.uint8 and scales.shape == (rows, (C + GROUP - 1) // GROUP)
+        _need(scales.dtype is torch.uint8 and scales.shape == (rows, (C + GROUP - 1) // GROUP)
               and scales.is_contiguous(), "scales must be a contiguous uint8 (rows, ceil(channels / 32)) matrix")
         _need(codes.is_cuda and scales.is_cuda, "CPU not supported")
-        _need(scales.device == codes.device, "scales must be on the codes' device")
+        _need(scales.get_device() == codes.get_device(), "scales must be on the codes' device")
+        pitch = _align16(C)
         if rows > 0:
-            _need((codes.stride(1) == 1 or C == 1) and codes.data_ptr() % 16 == 0, "codes must have 16-byte aligned rows")
-            if rows > 1:
-                _need(codes.stride(0) % 16 == 0 and C <= codes.stride(0) <= MAX_STRIDE, "codes must have 16-byte aligned rows")
-            last = codes.storage_offset() + (rows - 1) * codes.stride(0) + _align16(C)
+            step, inner = codes.stride()
+            _need((inner == 1 or C == 1) and codes.data_ptr() % 16 == 0
+                  and (rows == 1 or (step % 16 == 0 and C <= step <= MAX_STRIDE)), "codes must have 16-byte aligned rows")
+            last = codes.storage_offset() + (rows - 1) * step + pitch
             _need(codes.untyped_storage().nbytes() >= last, "codes must end with a whole 16-byte chunk")
+            if rows > 1:
+                pitch = step
         if shape is not None:
             n = 1
             for v in shape[:-1]:
                 n *= v
             _need(len(shape) > 0 and shape[-1] == C and n == rows, "shape does not fit the codes")
+            size = torch.Size(shape)
         self._codes, self._scales, self._buf, self._at = codes, scales, None, 0
-        self.rows, self.channels = rows, C
-        self.pitch = codes.stride(0) if rows > 1 else _align16(C)
-        self.shape = torch.Size(shape) if shape is not None else codes.shape
-        self.device = codes.device
+        self.rows, self.channels, self.pitch, self.shape, self.device = rows, C, pitch, size, codes.device
 
     @staticmethod
     def _in(buf, at, rows, C, shape):
@@ -130,15 +140,14 @@ class Act8(object):
 
 def act8_pack(x):
     """x (..., C) float32 / bfloat16 / float16 -> Act8."""
-    _need(x.is_cuda, "CPU not supported")
-    t = DTYPES.get(x.dtype)
-    _need(t is not None, "x must be a float32, bfloat16 or float16 tensor")
-    _need(x.dim() >= 1 and x.size(-1) > 0, "x must have at least one channel")
-    with on_device(x.device):
+    t = _dtype(x, "x")
+    C = x.size(-1) if x.dim() else 0
+    _need(C > 0, "x must have at least one channel")
+    dev = x.device
+    with on_device(dev):
         m, xs = _rows(x)
-        C = x.size(-1)
         rows = x.numel() // C
-        act = Act8._in(torch.empty(Act8._bytes(rows, C), dtype=torch.uint8, device=x.device), 0, rows, C, x.shape)
+        act = Act8._in(torch.empty(Act8._bytes(rows, C), dtype=torch.uint8, device=dev), 0, rows, C, x.shape)
         codes, scales = act._ptrs()
         check(lib.pvn3d_act8_pack(t, rows, C, m.data_ptr(), xs, codes, act.pitch, scales, _stream(x)), "act8_pack")
     return act
@@ -163,17 +172,18 @@ def linear8_weight_grad(dy, act):
     """dW (M, N) float32 = dy^T X: dy (..., M) bfloat16, X the rows of `act` (..., N).  Exact operands, fp32 sums in a fixed
     order (the same bits on every call); no rows: zeros."""
     _need(dy.is_cuda, "CPU not supported")
-    _need(dy.dtype == torch.bfloat16, "dy must be a bfloat16 tensor")
+    _need(dy.dtype is torch.bfloat16, "dy must be a bfloat16 tensor")
     _need(isinstance(act, Act8), "act must be an Act8")
-    _need(act.device == dy.device, "act must be on dy's device")
-    _need(dy.dim() >= 1 and dy.size(-1) > 0, "dy must have at least one channel")
-    rows, N, M = act.rows, act.channels, dy.size(-1)
+    dev = dy.device
+    _need(act.device == dev, "act must be on dy's device")
+    rows, N, M = act.rows, act.channels, dy.size(-1) if dy.dim() else 0
+    _need(M > 0, "dy must have at least one channel")
     _need(dy.numel() == rows * M, "dy and act must have the same number of rows")
-    with on_device(dy.device):
+    with on_device(dev):
         m, ds = _rows(dy)
-        dw = torch.empty(M, N, dtype=torch.float32, device=dy.device)
+        dw = torch.empty(M, N, dtype=torch.float32, device=dev)
         wsb = lib.pvn3d_act8_wgrad_workspace_bytes(rows, M, N)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         codes, scales = act._ptrs()
         check(lib.pvn3d_act8_wgrad(rows, M, N, m.data_ptr(), ds, codes, act.pitch, scales, dw.data_ptr(),
                                    ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_wgrad")

@@ -19,9 +19,10 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .._lib import lib, check, on_device
-from .act8 import Act8, DTYPES, _like, _need, _rows, _stream
+from .act8 import Act8, _dtype, _like, _need, _rows, _stream
 
 MAX_CHANNELS = 8192
+_CHANNELS = "layer norm takes 1 to %d channels" % MAX_CHANNELS
 _F32, _U8 = torch.float32, torch.uint8
 MAX_POINTS = 1 << 22         # per cloud, of the channel-major kernels
 
@@ -40,13 +41,6 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _check_x(x, name="x"):
-    _need(x.is_cuda, "CPU not supported")
-    t = DTYPES.get(x.dtype)
-    _need(t is not None, "%s must be a float32, bfloat16 or float16 tensor", name)
-    return t
-
-
 def _by_rows(x, channel_dim):
     """-> (True, x with the channels last) or (False, contiguous (B, C, ...)); refuses what is neither."""
     n = x.dim()
@@ -62,7 +56,7 @@ def _by_rows(x, channel_dim):
         M = x.numel() // max(1, x.size(0) * C)
         rows = not 4 <= M <= MAX_POINTS or (x.movedim(1, -1).is_contiguous() and not x.is_contiguous())
         x = x.movedim(1, -1) if rows else x.contiguous()
-    _need(1 <= C <= MAX_CHANNELS, "layer norm takes 1 to %d channels", MAX_CHANNELS)
+    _need(1 <= C <= MAX_CHANNELS, _CHANNELS)
     return rows, x
 
 
@@ -74,7 +68,7 @@ def _second(y, x):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False):
     """-> (y like x, mean, rstd): the statistics are float32, one value per point in the points' order."""
-    t = _check_x(x)
+    t = _dtype(x, "x")
     rows, v = _by_rows(x, channel_dim)
     C = v.size(-1) if rows else v.size(1)
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
@@ -103,15 +97,16 @@ def _grad_buffers(C, wsb, dev):
 
 
 def _check_stats(mean, rstd, n, x):
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == x.get_device(),
-              "%s must be a contiguous float32 tensor with one value per point", name)
+    dev = x.get_device()
+    for t in (mean, rstd):
+        _need(t.dtype is _F32 and t.numel() == n and t.is_contiguous() and t.get_device() == dev,
+              "mean and rstd must be contiguous float32 tensors with one value per point")
 
 
 def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=False, need_dx=True, need_dparams=True):
     """-> (dx like x or None, dweight (C,), dbias (C,) float32 or None, None).  mean, rstd: the forward's; relu: the
     derivative is taken where weight xh + bias > 0."""
-    t = _check_x(x)
+    t = _dtype(x, "x")
     _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.get_device() == x.get_device(), "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
     rows, v = _by_rows(x, channel_dim)
@@ -188,8 +183,8 @@ class Saved8(object):
 
 def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
     """x (..., C) -> (y like x, Saved8).  y is layer_norm_forward's, bit for bit."""
-    t = _check_x(x)
-    _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, "layer norm takes 1 to %d channels", MAX_CHANNELS)
+    t = _dtype(x, "x")
+    _need(x.dim() >= 1 and 1 <= x.size(-1) <= MAX_CHANNELS, _CHANNELS)
     C = x.size(-1)
     w, b = _param(weight, C, x, "weight"), _param(bias, C, x, "bias")
     dev = x.device
@@ -207,7 +202,7 @@ def layer_norm_forward8(x, weight=None, bias=None, eps=1e-5, relu=False):
 def layer_norm_backward8(dy, saved, weight=None, need_dx=True, need_dparams=True):
     """layer_norm_backward with xh = (held x - mean) rstd from the 8-bit form and the ReLU from its bits."""
     _need(isinstance(saved, Saved8), "saved must be what layer_norm_forward8 returned")
-    t = _check_x(dy, "dy")
+    t = _dtype(dy, "dy")
     act = saved.act
     _need(dy.shape == act.shape and dy.dtype == saved.dtype and dy.device == act.device, "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
@@ -273,7 +268,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=-1, relu=False, ckpt8=False):
     """Differentiable layer norm (see the top of this file).  ckpt8: keep x for the backward pass in 8 bits instead of
     holding on to it (channels last only); the output is the same, the gradients take xh from the 8-bit form."""
-    _check_x(x)
+    _dtype(x, "x")
     return _LayerNorm.apply(x, weight, bias, eps, channel_dim, bool(relu), bool(ckpt8) and torch.is_grad_enabled())
 
 
