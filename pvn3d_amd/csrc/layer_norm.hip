@@ -137,16 +137,19 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
 // 98304 x 1024 with the input saved: 100 us against 114 with one per four rows).
 constexpr long long MAX_GRID = 8192;
 
+// R8: two rows in flight where the input is saved and a row is two chunks a lane (bf16 46000 x 753: 49 us, 52 with one;
+// without saving 150000 x 600 73 us, 70 with one)
 template <typename T>
 int rows_forward(long long rows, int C, const void* x, long long xs, const float* w, const float* b, float eps, int relu,
                  void* y, long long ys, int ycols, float* mean, float* rstd, void* codes, long long pitch, void* scales,
                  void* mask, hipStream_t st) {
 #define LN_CALL(T, TPR, K, R)                                                                                           \
   do {                                                                                                                  \
-    const long long nb = ln::rows_blocks(rows, TPR, R);                                                                 \
+    constexpr int R8 = K == 2 ? 2 : R;                                                                                  \
+    const long long nb = ln::rows_blocks(rows, TPR, codes ? R8 : R);                                                    \
     const dim3 grid((unsigned)(nb < MAX_GRID ? nb : MAX_GRID));                                                         \
     if (codes)                                                                                                          \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w, \
+      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R8, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w,\
                          b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch,              \
                          (unsigned char*)scales, (unsigned char*)mask);                                                 \
     else                                                                                                                \
