@@ -446,12 +446,15 @@ bool chan_runs(int elem, int C, int M, int line, long long grid) {
   const long long tile = (long long)chan_shape(C).px * PTS * elem;
   return (grid & 7) == 0 && (tile % line != 0 || (long long)M * elem % line != 0);
 }
-// workgroups of a backward launch: what is on the chip at once (every one starts with the parameters and ends with its
-// partial sums): by its registers 32 waves a CU with two or three channels a thread, 16 with more (one: 16 are
-// the faster, 24 x 16 x 65536 fp32 61 us against 72).
-int chan_grad_parts(int B, int C, int M) {
+// Workgroups of a backward launch (every one starts with the parameters and ends with its partial sums): `per` a CU, the
+// fewer the more a thread holds.  Backward, a CU: bf16 24 x 128 x 12288: 1 81 us, 2 53, 4 56, 8 59; 24 x 160 x 6000: 2 38,
+// 3 61; 24 x 64 x 65536: 2 147, 4 135, 8 151; 24 x 32 x 65536: 4 86, 8 70; fp32 24 x 128 x 12288: 2 102, 4 105, 8 108;
+// 24 x 32 x 65536: 2 123, 4 127, 8 136; 24 x 8 x 100000: 4 81, 8 58.
+int chan_grad_parts(int dtype, int B, int C, int M) {
   const chan_plan p = chan_shape(C);
-  const long long n = chan_tiles(B, C, M), most = 256 * (long long)((p.kc == 2 || p.kc == 3 ? 2048 : 1024) / p.threads);
+  const int few = (dtype == 0 ? 8 : 16) / (p.kc ? p.kc : 1);
+  const int per = p.threads > 512 ? 1 : few < 2 ? 2 : few > 8 ? 8 : few;
+  const long long n = chan_tiles(B, C, M), most = 256 * per;
   return (int)(n < 8 ? n : n < most ? (n + 7) / 8 * 8 : most);
 }
 // Channel workgroups of a backward call: as for rows (layer_norm_grad.hip), a call of few points is one launch, with a wave
@@ -535,7 +538,7 @@ int chan_backward(int parts, int channels, int B, int C, int M, const void* dy, 
 
 extern "C" size_t pvn3d_layer_norm_chan_grad_workspace_bytes(int dtype, int B, int C, int M) {
   if (!chan_ok(dtype, B, C, M) || B == 0 || M == 0) return 0;
-  return chan_grad_channels(B, C, M) ? 0 : (size_t)chan_grad_parts(B, C, M) * 2 * C * sizeof(float);
+  return chan_grad_channels(B, C, M) ? 0 : (size_t)chan_grad_parts(dtype, B, C, M) * 2 * C * sizeof(float);
 }
 
 extern "C" int pvn3d_layer_norm_chan(int dtype, int B, int C, int M, const void* x, const float* weight, const float* bias,
@@ -568,7 +571,7 @@ extern "C" int pvn3d_layer_norm_chan_grad(int dtype, int B, int C, int M, const 
   }
   if (!dy || !x || !mean || !rstd) return (int)hipErrorInvalidValue;
   const int channels = dweight ? chan_grad_channels(B, C, M) : 0;
-  const int parts = dx || !channels ? chan_grad_parts(B, C, M) : 0;
+  const int parts = dx || !channels ? chan_grad_parts(dtype, B, C, M) : 0;
   if (dweight && !channels && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
     return (int)hipErrorInvalidValue;
   float* const part = (float*)workspace;

@@ -17,7 +17,7 @@ constexpr int ACROSS = 2;                            // chunks across of a colum
 // = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of the partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8>
-__global__ __launch_bounds__(256, traits<T>::VEC == 8 && K == 2 ? 3 : 1) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
+__global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
                                                            const T* __restrict__ x, int xs,
                                                            const signed char* __restrict__ codes, int pitch,
                                                            const unsigned char* __restrict__ scales,
@@ -196,6 +196,7 @@ __global__ __launch_bounds__(256, traits<T>::VEC == 8 && K == 2 ? 3 : 1) void ln
           const float xh = v[k][i], dz = d[k][i];
           aw[k][i] = fmaf(dz, xh, aw[k][i]);
           ab[k][i] += dz;
+          asm volatile("" : "+v"(aw[k][i]), "+v"(ab[k][i]));     // summed here: put off behind the row's sums, the terms stay alive
           const float u = dz * g[k][i], um = u * col.own[k][i];
           s1 += um;
           s2 = fmaf(um, xh, s2);
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(256, traits<T>::VEC == 8 && K == 2 ? 3 : 1) void ln
         for (int k = 0; k < K; ++k) {
           float o[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] = rs[r] * (d[k][i] - s1 - v[k][i] * s2);
+          for (int i = 0; i < VEC; ++i) o[i] = rs[r] * fmaf(-s2, v[k][i], d[k][i] - s1);
           if (live) col.store(ob, __umul24(rl, dxs), k, C, o);
         }
         if (dxcols > C && live)
@@ -268,17 +269,19 @@ int rows_grad_columns(int dtype, long long rows, int C) {
   return rows <= 2048 && rows * C <= 3 << 19 ? (C + wide - 1) / wide : 0;
 }
 
-// Workgroups of a rows backward launch = its partial sums: what the registers let stay on the chip (`resident` a CU), each
-// with four rows at least where it takes a row at a time.  bf16 16384 x 4096: 100 us,
-// 125 with twice as many, 137 with 2048; 46000 x 753: 45, 51, 57; 2000 x 1536: 19, 19, 36; 786432 x 128: 119, 122, 122.
-int rows_grad_parts(int dtype, long long rows, int C, bool from8) {
+// Workgroups of a rows backward launch = its partial sums: `per` a CU, as many as keep memory busy and no more, each with
+// four rows at least where it takes a row at a time.  A CU (dx, dweight, dbias from x / from 8 bits, us):
+//   one chunk a lane   bf16 786432 x 128: 3 118 / 112, 4 120 / 108, 6 131 / 112;  fp32 393216 x 128: 3 115 / 95, 4 115 / 92, 8 124 / 101
+//   two, a wave a row  bf16 46000 x 753: 2 48 / 51, 3 45 / 48, 4 57 / 57;  fp32 98304 x 512: 2 116 / 91, 3 118 / 92, 5 124 / 95
+//   two, a workgroup   bf16 16384 x 4000: 2 90 / 92, 3 98 / 90, 4 124 / 109;  fp32 10000 x 1501: 2 43 / 43, 3 41 / 38, 5 46 / 41
+//   four, eight        fp32 8192 x 4096: 1 93 / 80, 2 87 / 70, 4 97 / 81;  bf16 4096 x 8192: 1 67 / 65, 2 81 / 80
+int rows_grad_parts(int dtype, long long rows, int C) {
   const int vec = ln::vec_of(dtype), tpr = ln::rows_threads(C, vec), k = (C + tpr * vec - 1) / (tpr * vec);
-  int resident;
-  if (vec == 8) resident = k == 1 ? 4 : k == 2 ? 3 : 1;
-  else resident = k == 1 ? 8 - from8 : k == 2 ? (tpr == 64 ? 5 : 5 - from8) : k <= 4 ? 2 : 1;
+  const int per = k == 1 ? 4 : k == 2 ? ((vec == 8) == (tpr == 64) ? 3 : 2) : vec == 4 && k <= 4 ? 2 : 1;
   const long long n = tpr == 256 ? (rows + 3) / 4 : ln::rows_blocks(rows, tpr, k == 1 ? 2 : 1);
-  return (int)(n < 256 * resident ? n : 256 * resident);
+  return (int)(n < 256 * per ? n : 256 * per);
 }
+
 template <typename T>
 int rows_backward(int parts, int columns, long long rows, int C, const void* dy, long long dys, const void* x, long long xs,
                   const void* codes, long long pitch, const void* scales, const void* mask, const float* w, const float* b,
@@ -306,7 +309,7 @@ int rows_backward(int parts, int columns, long long rows, int C, const void* dy,
 extern "C" size_t pvn3d_layer_norm_grad_workspace_bytes(int dtype, long long rows, int C) {
   if (rows <= 0 || C <= 0 || C > ln::MAX_C || dtype < 0 || dtype > 2) return 0;
   if (rows_grad_columns(dtype, rows, C)) return 0;
-  return (size_t)rows_grad_parts(dtype, rows, C, false) * 2 * C * sizeof(float);        // (from 8 bits: as many or fewer)
+  return (size_t)rows_grad_parts(dtype, rows, C) * 2 * C * sizeof(float);
 }
 extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const void* dy, long long dys, const void* x,
                                      long long xs, const void* codes, long long pitch, const void* scales,
@@ -330,7 +333,7 @@ extern "C" int pvn3d_layer_norm_grad(int dtype, long long rows, int C, const voi
   }
   if (!dy || (!x && !codes) || !mean || !rstd) return (int)hipErrorInvalidValue;
   const int columns = dweight ? rows_grad_columns(dtype, rows, C) : 0;
-  const int parts = dx || !columns ? rows_grad_parts(dtype, rows, C, codes != nullptr) : 0;
+  const int parts = dx || !columns ? rows_grad_parts(dtype, rows, C) : 0;
   if (dweight && !columns && (!workspace || workspace_bytes < (size_t)parts * 2 * C * sizeof(float)))
     return (int)hipErrorInvalidValue;
   float* const part = (float*)workspace;
