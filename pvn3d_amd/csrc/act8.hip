@@ -146,7 +146,7 @@ __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 46 us and 5 us for the sum of 768 partial tiles, 5.0 TB/s).
+// What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 49 us with the sum of 512 partial tiles, 5.2 TB/s).
 // For wide ones how much the two waves of a SIMD overlap: a step of 64 rows of the 256 x 128 tile keeps the matrix pipes busy
 // for 45 % of its cycles, LDS (176 KB) for 45 %, the vector units for 22 %.  12288 rows, 512 x 1536 take 34 us with the sum
 // of the 33 MB of partial tiles, 556 TFLOP/s; 98304 rows, 512 x 512 76 us, 675 TFLOP/s (the library's bf16 product: 81 and
@@ -389,18 +389,18 @@ __global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_k
 
 // Tile, rows of a step and number of row splits of a call.  Every split leaves a partial tile that is written and read
 // again, so there are no more workgroups than keep the chip busy: one of eight waves per CU for the 256 x 128 tile (33 MB of
-// partial sums at most; 98304 x 512 x 512: 81 us, 93 us with two per CU), two of four waves for 128 x 128 (91 us; 101 us with
-// three), three for the narrow tiles, whose waves work for themselves.  The 256 x 128 tile converts each code for twice the
+// partial sums at most; 98304 x 512 x 512: 81 us, 93 us with two per CU), two of four waves for the others (786432 x 96 x 64:
+// 43 us, 55 with one, 54 with three; 1572864 x 32 x 16: 27, 37, 28).  The 256 x 128 tile converts each code for twice the
 // output; up to 128 output channels half of it would be empty (393216 x 128 x 128: 128 x 128).
 struct wg_plan { int kind, tm, tn, S; };
 
 wg_plan wgrad_plan(long long rows, int M, int N) {
   wg_plan p;
-  int step = 32, wgs = 768, per = 16;                            // per: steps a workgroup should have at least
+  int step = 32, wgs = 512, per = 16;                            // per: steps a workgroup should have at least
   if (M > 128 && N > 64) { p.kind = 0; p.tm = 256; p.tn = 128; step = 64; wgs = 256; per = 4; }
-  else if (M > 64 && N > 64) { p.kind = 1; p.tm = 128; p.tn = 128; step = 64; wgs = 512; per = 4; }
-  else if (M > 32 && N > 64) { p.kind = 2; p.tm = 64; p.tn = 128; step = 64; wgs = 512; per = 4; }
-  else if (M > 64 && N > 32) { p.kind = 3; p.tm = 128; p.tn = 64; step = 64; wgs = 512; per = 4; }
+  else if (M > 64 && N > 64) { p.kind = 1; p.tm = 128; p.tn = 128; step = 64; per = 4; }
+  else if (M > 32 && N > 64) { p.kind = 2; p.tm = 64; p.tn = 128; step = 64; per = 4; }
+  else if (M > 64 && N > 32) { p.kind = 3; p.tm = 128; p.tn = 64; step = 64; per = 4; }
   else if (M > 32 && N > 32) { p.kind = 4; p.tm = 64; p.tn = 64; }
   else if (M > 32) { p.kind = 5; p.tm = 64; p.tn = 32; }
   else if (N > 32) { p.kind = 6; p.tm = 32; p.tn = 64; }
