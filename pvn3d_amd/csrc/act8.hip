@@ -425,8 +425,8 @@ int row_threads(int C, int vec) {                                // threads acro
 }
 unsigned row_grid(long long rows, int tpr) {
   const int per = 256 / tpr * FLY;
-  const long long n = (rows + per - 1) / per;
-  return (unsigned)(n < 16384 ? n : 16384);
+  // packed and unpacked: bf16 786432 x 96 77.0 us (4096: 83, 8192: 79, 24576: 80), fp32 1000000 x 33 56 (57, 56, 59)
+  return rv::even_grid((rows + per - 1) / per, 12288);
 }
 
 template <typename T>

@@ -21,7 +21,7 @@ using rv::fp16;
 using rv::traits;
 using ln::row_sum;
 
-// Bound by HBM: x read once, y written once.  bf16 1572864 x 64: 75 us = 5.4 TB/s (a large copy on this card: 4.9);
+// Bound by HBM: x read once, y written once.  bf16 1572864 x 64: 74 us = 5.5 TB/s (a large copy on this card: 4.9);
 // 393216 x 196 with x put away in 8 bits and ReLU bits, 84 us = 4.8 TB/s (lanes behind the row's end and the codes'
 // arithmetic cost the rest).  128 x 512, a call whose cost is its launch: 3.6 us.  What it took: the parameters loaded in
 // vectors (with a load per value 98304 x 1024 took 237 us, now 74), the loads of both rows ahead of any wait, addresses as a
@@ -132,10 +132,11 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
   }
 }
 
-// Workgroups of a forward launch: enough to keep every CU at its eight and to end evenly, few enough that loading the
-// parameters is spread over several rows (bf16, 786432 x 128: 75.7 us; 1024 workgroups 77.3, one per 32 rows 74.8 -- and
-// 98304 x 1024 with the input saved: 100 us against 114 with one per four rows).
-constexpr long long MAX_GRID = 8192;
+// Workgroups of a forward launch: enough to keep every CU busy, few enough that loading the parameters is spread over several
+// rows, and all with as many passes.  bf16 786432 x 128 with the input saved: 96 us with two passes each, 99 with three; where
+// a workgroup takes four rows or two at a time 46000 x 753 29 us with two or three passes each, 34 with one, 31 with two in
+// some and one in others; 150000 x 600 70 us with five, 73 with ten.
+constexpr long long most_blocks(int tpr, int k) { return tpr <= 64 && k == 1 ? 12288 : 8192; }
 
 // R8: two rows in flight where the input is saved and a row is two chunks a lane (bf16 46000 x 753: 49 us, 52 with one;
 // without saving 150000 x 600 73 us, 70 with one)
@@ -147,7 +148,7 @@ int rows_forward(long long rows, int C, const void* x, long long xs, const float
   do {                                                                                                                  \
     constexpr int R8 = K == 2 ? 2 : R;                                                                                  \
     const long long nb = ln::rows_blocks(rows, TPR, codes ? R8 : R);                                                    \
-    const dim3 grid((unsigned)(nb < MAX_GRID ? nb : MAX_GRID));                                                         \
+    const dim3 grid(rv::even_grid(nb, most_blocks(TPR, K)));                                                            \
     if (codes)                                                                                                          \
       hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R8, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w,\
                          b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch,              \

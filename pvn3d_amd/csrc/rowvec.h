@@ -195,6 +195,12 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v) {
   return v;
 }
 
+// workgroups for n > 0 passes, `most` at most, all with the same number of passes (but the last few)
+static inline unsigned even_grid(long long n, long long most) {
+  const long long passes = (n + most - 1) / most;
+  return (unsigned)((n + passes - 1) / passes);
+}
+
 // ---------------------------------------------------------------------------------------------- partial sums
 // out[e] = sum over p of part[p][count], e < count, in a fixed order: SL slices of p a workgroup, 1024 / SL threads across,
 // W (1 or 4) columns each, eight loads in flight per thread.  e < first goes to a, the rest to b.
