@@ -120,6 +120,12 @@ def test_weight_gradient(dev, rows, M, N):
     assert torch.equal(dw, act8.linear8_weight_grad(wide[:, 5:5 + M], act8.Act8(other[:, :N], act.scales)))
 
 
+@pytest.mark.parametrize("rows,M,N", [(100003, 20, 130), (70000, 130, 20), (50001, 200, 300), (33000, 100, 100), (90001, 40, 70)])
+def test_weight_gradient_of_many_splits(dev, rows, M, N):
+    """Split counts of every tile shape at their largest."""
+    test_weight_gradient(dev, rows, M, N)
+
+
 def test_weight_gradient_of_nothing_and_of_bad_rows(dev):
     dw = act8.linear8_weight_grad(torch.zeros(0, 5, dtype=torch.bfloat16, device=dev),
                                   act8.act8_pack(torch.zeros(0, 7, dtype=torch.bfloat16, device=dev)))
