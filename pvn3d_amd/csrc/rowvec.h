@@ -208,9 +208,10 @@ template <int SL, int W>
 __global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t first, const float* __restrict__ part,
                                                     float* __restrict__ a, float* __restrict__ b) {
   constexpr int TX = 1024 / SL;
-  __shared__ float s[SL][TX * W];
+  constexpr int NP = TX < 64 ? 16 : SL;                    // sums of a column that meet in LDS: a wave's or a slice's
+  __shared__ float s[NP][TX * W];
   const int tx = threadIdx.x % TX, sl = threadIdx.x / TX;
-  const size_t e = ((size_t)blockIdx.x * TX + tx) * W;
+  const size_t base = (size_t)blockIdx.x * TX * W, e = base + (size_t)tx * W;
   float v[W];
 #pragma unroll
   for (int j = 0; j < W; ++j) v[j] = 0.f;
@@ -240,24 +241,22 @@ __global__ __launch_bounds__(1024) void fold_kernel(int P, size_t count, size_t 
       for (int j = 0; j < W; ++j) v[j] += f[j];
     }
   }
-  if (SL > 1) {
+  // slices of a wave in registers, the rest through LDS once
 #pragma unroll
-    for (int j = 0; j < W; ++j) s[sl][tx * W + j] = v[j];
-    __syncthreads();
-#pragma unroll
-    for (int o = SL / 2; o >= 1; o >>= 1) {
-      if (sl < o) {
-#pragma unroll
-        for (int j = 0; j < W; ++j) s[sl][tx * W + j] += s[sl + o][tx * W + j];
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = s[sl][tx * W + j];
+  for (int j = 0; j < W; ++j) {
+    if (TX == 16) v[j] = add16(v[j]);
+    if (TX <= 32) v[j] = add32(v[j]);
   }
-  if (sl == 0 && e < count) {
+  if (TX >= 64 || (threadIdx.x & 63) < TX) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) (e + j < first ? a[e + j] : b[e + j - first]) = v[j];
+    for (int j = 0; j < W; ++j) s[TX < 64 ? threadIdx.x >> 6 : sl][tx * W + j] = v[j];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < TX * W && base + c < count; c += 1024) {
+    float t = s[0][c];
+#pragma unroll
+    for (int g = 1; g < NP; ++g) t += s[g][c];
+    (base + c < first ? a[base + c] : b[base + c - first]) = t;
   }
 }
 static inline int fold(int P, size_t count, size_t first, const float* part, float* a, float* b, hipStream_t st) {
