@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(long long rows, int C, i
   }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C, int tpr,
                                                           const signed char* __restrict__ codes, int pitch,
                                                           const unsigned char* __restrict__ scales, T* __restrict__ y, int ys,
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(long long rows, int C,
         if (rl <= last) {
           T* const p = rv::at32(yb, (__umul24(rl, ys) + at) * (unsigned)sizeof(T));
           if (C >= VEC) {
-            rv::store_vec<T>(p, v);
+            rv::store_vec<T, STREAM>(p, v);
           } else {
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
@@ -452,8 +452,12 @@ template <typename T>
 int run_unpack(long long rows, int C, const void* codes, long long pitch, const void* scales, void* y, long long ys,
                int ycols, hipStream_t st) {
   const int tpr = row_threads(C, traits<T>::VEC);
-  hipLaunchKernelGGL((act8_unpack_kernel<T>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr,
-                     (const signed char*)codes, (int)pitch, (const unsigned char*)scales, (T*)y, (int)ys, ycols);
+#define A8_UNPACK(STREAM)                                                                                                  \
+  hipLaunchKernelGGL((act8_unpack_kernel<T, STREAM>), dim3(row_grid(rows, tpr)), dim3(256), 0, st, rows, C, tpr,           \
+                     (const signed char*)codes, (int)pitch, (const unsigned char*)scales, (T*)y, (int)ys, ycols)
+  if (rows * C * (long long)sizeof(T) >= rv::STREAM_BYTES) A8_UNPACK(true);
+  else A8_UNPACK(false);
+#undef A8_UNPACK
   PVN3D_LAUNCH_CHECK();
   return 0;
 }

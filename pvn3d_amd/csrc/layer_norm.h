@@ -66,18 +66,24 @@ struct lane_cols {
       }
   }
   // the chunk as loaded; row: its place behind base, in elements
+  template <bool STREAM>
   __device__ __forceinline__ rv::u4_any load(const T* __restrict__ base, unsigned row, int k, int C) const {
     const T* const p = rv::at32(base, (row + at[k]) * (unsigned)sizeof(T));
-    if (TPR > 1) return *reinterpret_cast<const rv::u4_any*>(p);
+    rv::u4_any r;
+    if (TPR > 1) {
+      rv::get<STREAM>(p, r);
+      return r;
+    }
     float v[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = i < C ? traits<T>::load1(p + i) : 0.f;
     return traits<T>::pack(v);                         // (exact: the values are of type T)
   }
+  template <bool STREAM>
   __device__ __forceinline__ void store(T* __restrict__ base, unsigned row, int k, int C, const float (&v)[VEC]) const {
     T* const p = rv::at32(base, (row + at[k]) * (unsigned)sizeof(T));
     if (TPR > 1) {
-      if (c[k] < C) rv::store_vec<T>(p, v);
+      if (c[k] < C) rv::store_vec<T, STREAM>(p, v);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)

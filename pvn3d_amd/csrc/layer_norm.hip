@@ -21,7 +21,7 @@ using rv::fp16;
 using rv::traits;
 using ln::row_sum;
 
-// Bound by HBM: x read once, y written once.  bf16 1572864 x 64: 74 us = 5.5 TB/s (a large copy on this card: 4.9);
+// Bound by HBM: x read once, y written once.  bf16 1572864 x 64: 68 us = 5.9 TB/s (a large copy on this card: 4.9);
 // 393216 x 196 with x put away in 8 bits and ReLU bits, 84 us = 4.8 TB/s (lanes behind the row's end and the codes'
 // arithmetic cost the rest).  128 x 512, a call whose cost is its launch: 3.6 us.  What it took: the parameters loaded in
 // vectors (with a load per value 98304 x 1024 took 237 us, now 74), the loads of both rows ahead of any wait, addresses as a
@@ -29,7 +29,7 @@ using ln::row_sum;
 // ------------------------------------------------------------------------------------------------ rows, forward
 // TPR threads share a row, chunk k of thread t = the VEC channels from (k TPR + t) VEC on (16 bytes): K chunks cover the
 // row, R rows per thread are in flight at once.
-template <typename T, int TPR, int K, int R, bool SAVE8>
+template <typename T, int TPR, int K, int R, bool SAVE8, bool STREAM>
 __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, const T* __restrict__ x, int xs,
                                                       const float* __restrict__ w, const float* __restrict__ b, float eps,
                                                       int relu, T* __restrict__ y, int ys, int ycols,
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
     for (int r = 0; r < R; ++r) {
       const unsigned row = __umul24(min(rg + r * RPB, last), xs);
 #pragma unroll
-      for (int k = 0; k < K; ++k) raw[r][k] = col.load(xb, row, k, C);
+      for (int k = 0; k < K; ++k) raw[r][k] = col.template load<STREAM>(xb, row, k, C);
     }
     __builtin_amdgcn_sched_barrier(0);       // all loads on their way before anything waits for one
 #pragma unroll
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
 #pragma unroll
         for (int i = 0; i < VEC; ++i)       // (maximum: a NaN stays one, which max(z, 0) would make 0)
           z[i] = __builtin_elementwise_maximum(fmaf((v[k][i] - mu) * rs, g[k][i], be[k][i]), low);
-        if (live) col.store(yb, __umul24(rl, ys), k, C, z);
+        if (live) col.template store<STREAM>(yb, __umul24(rl, ys), k, C, z);
         if (SAVE8) {
           constexpr int LPG = rv::GROUP / VEC < TPR ? rv::GROUP / VEC : TPR;       // lanes per group
           unsigned big = 0, wd[VEC / 4];
@@ -144,21 +144,24 @@ template <typename T>
 int rows_forward(long long rows, int C, const void* x, long long xs, const float* w, const float* b, float eps, int relu,
                  void* y, long long ys, int ycols, float* mean, float* rstd, void* codes, long long pitch, void* scales,
                  void* mask, hipStream_t st) {
+  const bool stream = rows * C * (long long)sizeof(T) >= rv::STREAM_BYTES;
+#define LN_ONE(T, TPR, K, R, SAVE8, STREAM)                                                                              \
+  hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, SAVE8, STREAM>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, \
+                     w, b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch,               \
+                     (unsigned char*)scales, (unsigned char*)mask)
 #define LN_CALL(T, TPR, K, R)                                                                                           \
   do {                                                                                                                  \
     constexpr int R8 = K == 2 ? 2 : R;                                                                                  \
     const long long nb = ln::rows_blocks(rows, TPR, codes ? R8 : R);                                                    \
     const dim3 grid(rv::even_grid(nb, most_blocks(TPR, K)));                                                            \
-    if (codes)                                                                                                          \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R8, true>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs, w,\
-                         b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, (signed char*)codes, (int)pitch,              \
-                         (unsigned char*)scales, (unsigned char*)mask);                                                 \
-    else                                                                                                                \
-      hipLaunchKernelGGL((ln_rows_kernel<T, TPR, K, R, false>), grid, dim3(256), 0, st, rows, C, (const T*)x, (int)xs,  \
-                         w, b, eps, relu, (T*)y, (int)ys, ycols, mean, rstd, nullptr, 0, nullptr, nullptr);             \
+    if (codes && stream) LN_ONE(T, TPR, K, R8, true, true);                                                             \
+    else if (codes) LN_ONE(T, TPR, K, R8, true, false);                                                                 \
+    else if (stream) LN_ONE(T, TPR, K, R, false, true);                                                                 \
+    else LN_ONE(T, TPR, K, R, false, false);                                                                            \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL
+#undef LN_ONE
   PVN3D_LAUNCH_CHECK();
   return 0;
 }

@@ -112,7 +112,7 @@ __device__ __forceinline__ void slot_sum(float (&s)[N], float (*buf)[PX * N]) {
     for (int i = 0; i < N; ++i) s[i] += buf[wv][px * N + i];
 }
 
-template <typename T, int KC, int PX>
+template <typename T, int KC, int PX, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int runs, int per_cloud, int C, int M,
                                                               const T* __restrict__ x,
                                                               const float* __restrict__ w, const float* __restrict__ b,
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
     float s[PTS] = {0.f, 0.f, 0.f, 0.f}, mu[PTS], rs[PTS];
     if (KC > 0) {
 #pragma unroll
-      for (int k = 0; k < KR; ++k) r[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(p + k * slots, k < KR - 1 ? o : ol));
+      for (int k = 0; k < KR; ++k) rv::get<STREAM>(rv::at32(p + k * slots, k < KR - 1 ? o : ol), r[k].r);
       __builtin_amdgcn_sched_barrier(0);     // all loads on their way before anything waits for one
     }
     // f(k, channel's base, channel, values) for each of the thread's channels
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
 #pragma unroll
       for (int i = 0; i < PTS; ++i)                      // (maximum: a NaN stays one)
         z[i] = __builtin_elementwise_maximum(fmaf((v[i] - mu[i]) * rs[i], g, be), low);
-      if (at.live) *reinterpret_cast<raw4<T>*>(rv::at32(q + at_c, o)) = shut<T>(z);
+      if (at.live) rv::put<STREAM>(rv::at32(q + at_c, o), shut<T>(z).r);
     });
   }
 }
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_kernel(int tiles, int run
 // dw / db: a thread has the same channels for all its tiles: a register each, summed over the 16 lanes at the end (KC = 0:
 // in LDS, summed over the lanes per tile; dynamic LDS, 2 C floats).
 // CHANNELS: the call has channel workgroups (an instance of its own: they take registers).
-template <typename T, int KC, int PX, bool CHANNELS>
+template <typename T, int KC, int PX, bool CHANNELS, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, int runs, int per_cloud, int C, int M,
                                                                    const T* __restrict__ dy, const T* __restrict__ x,
                                                                    const float* __restrict__ w, const float* __restrict__ b,
@@ -301,8 +301,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     if (KC > 0) {
 #pragma unroll
       for (int k = 0; k < KR; ++k) {
-        rx[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(px_ + k * slots, k < KR - 1 ? o : ol));
-        rd[k] = *reinterpret_cast<const raw4<T>*>(rv::at32(pd_ + k * slots, k < KR - 1 ? o : ol));
+        rv::get<STREAM>(rv::at32(px_ + k * slots, k < KR - 1 ? o : ol), rx[k].r);
+        rv::get<STREAM>(rv::at32(pd_ + k * slots, k < KR - 1 ? o : ol), rd[k].r);
       }
       __builtin_amdgcn_sched_barrier(0);     // all loads on their way before anything waits for one
     }
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
       float e[PTS];
 #pragma unroll
       for (int i = 0; i < PTS; ++i) e[i] = fmaf(rs[i], dz[i] * g, fmaf(v[i] - mu[i], s[PTS + i], s[i]));
-      if (at.live) *reinterpret_cast<raw4<T>*>(rv::at32(po_ + at_c, o)) = shut<T>(e);
+      if (at.live) rv::put<STREAM>(rv::at32(po_ + at_c, o), shut<T>(e).r);
     };
     float v[PTS], d[PTS];
     if (KC > 0) {
@@ -499,12 +499,19 @@ int chan_forward(int B, int C, int M, const void* x, const float* w, const float
   const long long tiles = chan_tiles(B, C, M);
   // (bf16 24 x 64 x 65536: 84 us, 91 with 8192, 106 with 512; 24 x 32 x 65536: 42, 40, 88, and 45 with one per tile)
   const dim3 grid((unsigned)(tiles < 8 ? tiles : tiles < 16384 ? (tiles + 7) / 8 * 8 : 16384));
-#define LN_CALL(KC, PX)                                                                                                     \
-  hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX>), grid, dim3(p.threads), 0, st, (int)tiles,                                 \
+  const bool stream = (long long)B * C * M * (long long)sizeof(T) >= rv::STREAM_BYTES;
+#define LN_ONE(KC, PX, STREAM)                                                                                              \
+  hipLaunchKernelGGL((ln_chan_kernel<T, KC, PX, STREAM>), grid, dim3(p.threads), 0, st, (int)tiles,                         \
                      (int)chan_runs(sizeof(T), C, M, 256, grid.x), cloud_tiles(C, M), C, M,                                 \
                      (const T*)x, w, b, eps, relu, (T*)y, mean, rstd)
+#define LN_CALL(KC, PX)                \
+  do {                                 \
+    if (stream) LN_ONE(KC, PX, true);  \
+    else LN_ONE(KC, PX, false);        \
+  } while (0)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL
+#undef LN_ONE
   PVN3D_LAUNCH_CHECK();
   return 0;
 }
@@ -513,20 +520,23 @@ template <typename T>
 int chan_backward(int parts, int channels, int B, int C, int M, const void* dy, const void* x, const float* w, const float* b,
                   const float* mean, const float* rstd, int relu, void* dx, float* pw, float* pb, size_t ps, hipStream_t st) {
   const chan_plan p = chan_shape(C);
+  const bool stream = (long long)B * C * M * (long long)sizeof(T) >= rv::STREAM_BYTES;
   const int lds = p.kc ? 0 : (int)(2 * C * sizeof(float));
   if (!p.kc) {
-    const int rc = channels ? pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, true>)
-                            : pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, false>);
+    const int rc = channels ? pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, true, false>)
+                   : stream ? pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, false, true>)
+                            : pvn3d_allow_big_lds(ln_chan_grad_kernel<T, 0, 16, false, false>);
     if (rc) return rc;
   }
-#define LN_ONE(KC, PX, CHANNELS)                                                                                            \
-  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX, CHANNELS>), dim3(parts + channels), dim3(p.threads), lds, st,          \
+#define LN_ONE(KC, PX, CHANNELS, STREAM)                                                                                    \
+  hipLaunchKernelGGL((ln_chan_grad_kernel<T, KC, PX, CHANNELS, STREAM>), dim3(parts + channels), dim3(p.threads), lds, st,  \
                      (int)chan_tiles(B, C, M), (int)chan_runs(sizeof(T), C, M, 128, parts), cloud_tiles(C, M), C, M,        \
                      (const T*)dy, (const T*)x, w, b, mean, rstd, relu, (T*)dx, pw, pb, ps, parts)
-#define LN_CALL(KC, PX)                  \
-  do {                                   \
-    if (channels) LN_ONE(KC, PX, true);  \
-    else LN_ONE(KC, PX, false);          \
+#define LN_CALL(KC, PX)                             \
+  do {                                              \
+    if (channels) LN_ONE(KC, PX, true, false);      \
+    else if (stream) LN_ONE(KC, PX, false, true);   \
+    else LN_ONE(KC, PX, false, false);              \
   } while (0)
   LN_CHAN_PICK(LN_CALL)
 #undef LN_CALL

@@ -16,7 +16,7 @@ constexpr int ACROSS = 2;                            // chunks across of a colum
 // Bound by HBM: dy and x read, dx written, once each.  bf16 786432 x 128: 115 us = 5.2 TB/s; 393216 x 196 from 8 bits: 100 us
 // = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of the partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
-template <typename T, int TPR, int K, int R, bool FROM8>
+template <typename T, int TPR, int K, int R, bool FROM8, bool STREAM>
 __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
                                                            const T* __restrict__ x, int xs,
                                                            const signed char* __restrict__ codes, int pitch,
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
         const long long row = min(base + r * SLOTS, (int)rows - 1);
         mu[r] = mean[row];
         rs[r] = rstd[row];
-        rd[r] = col.load(dy + row * dys, 0, 0, C);
+        rd[r] = col.template load<false>(dy + row * dys, 0, 0, C);
         if (FROM8) {
           const int c = min(col.c[0], (C - 1) & ~(VEC - 1)), at = col.at[0];
           rv::load_codes(codes + row * pitch + at, cw[r]);
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
           if (mask) mk[r][0] = mask[row * MB + at / 8];
           if (mask && ragged) mk[r][1] = mask[row * MB + min(at / 8 + 1, MB - 1)];
         } else {
-          rx[r] = col.load(x + row * xs, 0, 0, C);
+          rx[r] = col.template load<false>(x + row * xs, 0, 0, C);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
       rs[r] = *rv::at32(rstd + base, rl * 4u);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        rd[r][k] = col.load(db, __umul24(rl, dys), k, C);
+        rd[r][k] = col.template load<STREAM>(db, __umul24(rl, dys), k, C);
         if (FROM8) {
           // a window that repeats values of its neighbour may start in the group before its own
           const int c = min(col.c[k], (C - 1) & ~(VEC - 1)), at = col.at[k];
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
           if (mask) mk[r][k][0] = *rv::at32(mb, mrow + at / 8);
           if (mask && ragged) mk[r][k][1] = *rv::at32(mb, mrow + min(at / 8 + 1, MB - 1));
         } else {
-          rx[r][k] = col.load(xb, __umul24(rl, xs), k, C);
+          rx[r][k] = col.template load<STREAM>(xb, __umul24(rl, xs), k, C);
         }
       }
     }
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
           float o[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) o[i] = rs[r] * fmaf(-s2, v[k][i], d[k][i] - s1);
-          if (live) col.store(ob, __umul24(rl, dxs), k, C, o);
+          if (live) col.template store<STREAM>(ob, __umul24(rl, dxs), k, C, o);
         }
         if (dxcols > C && live)
 #pragma unroll 1
@@ -287,15 +287,18 @@ int rows_backward(int parts, int columns, long long rows, int C, const void* dy,
                   const void* codes, long long pitch, const void* scales, const void* mask, const float* w, const float* b,
                   const float* mean, const float* rstd, int relu, void* dx, long long dxs, int dxcols, float* pw, float* pb,
                   size_t ps, hipStream_t st) {
-#define LN_ONE(T, TPR, K, R, FROM8)                                                                                       \
-  hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, FROM8>), dim3(parts + columns), dim3(256), 0, st, rows, C,        \
-                     (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)codes, (int)pitch,                 \
+  const bool stream = rows * C * (long long)sizeof(T) >= rv::STREAM_BYTES;
+#define LN_ONE(T, TPR, K, R, FROM8, STREAM)                                                                               \
+  hipLaunchKernelGGL((ln_rows_grad_kernel<T, TPR, K, R, FROM8, STREAM>), dim3(parts + columns), dim3(256), 0, st, rows,   \
+                     C, (const T*)dy, (int)dys, (const T*)x, (int)xs, (const signed char*)codes, (int)pitch,              \
                      (const unsigned char*)scales, (const unsigned char*)mask, w, b, mean, rstd, relu, (T*)dx, (int)dxs,  \
                      dxcols, pw, pb, ps, parts)
-#define LN_CALL(T, TPR, K, R)                   \
-  do {                                          \
-    if (codes) LN_ONE(T, TPR, K, R, true);      \
-    else LN_ONE(T, TPR, K, R, false);           \
+#define LN_CALL(T, TPR, K, R)                                \
+  do {                                                       \
+    if (codes && stream) LN_ONE(T, TPR, K, R, true, true);   \
+    else if (codes) LN_ONE(T, TPR, K, R, true, false);       \
+    else if (stream) LN_ONE(T, TPR, K, R, false, true);      \
+    else LN_ONE(T, TPR, K, R, false, false);                 \
   } while (0)
   LN_ROWS_PICK(T, C, LN_CALL);
 #undef LN_CALL

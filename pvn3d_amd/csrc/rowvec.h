@@ -71,13 +71,50 @@ template <> struct traits<fp16> {
   }
 };
 
+// Tensors that no cache holds until their next use are read and written past the caches (non-temporal): from STREAM_BYTES
+// on, as instances of their own (a choice at run time cost more than it gave).  bf16: forward 1572864 x 64 73.7 us, so 68.4;
+// backward 786432 x 128 117.5, 106; forward and backward with 8 bits kept, 393216 x 196 186, 165.5; pack and unpack
+// 786432 x 96 77.7, 71.  The next kernel counts too: forward of 524288 x 128 (134 MB) and an addition to its result 88 us
+// either way, a product, its backward and an addition 170, 160; of 131072 x 128 24.4 us, 27.4, and 44.4, 46.7.
+constexpr long long STREAM_BYTES = 1ll << 27;
+typedef unsigned v4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned v2_any __attribute__((ext_vector_type(2), aligned(2)));
+template <bool STREAM>
+__device__ __forceinline__ void put(void* p, const u4_any& r) {
+  if (STREAM) __builtin_nontemporal_store(v4_any{r.x, r.y, r.z, r.w}, reinterpret_cast<v4_any*>(p));
+  else *reinterpret_cast<u4_any*>(p) = r;
+}
+template <bool STREAM>
+__device__ __forceinline__ void put(void* p, const u2_any& r) {
+  if (STREAM) __builtin_nontemporal_store(v2_any{r.x, r.y}, reinterpret_cast<v2_any*>(p));
+  else *reinterpret_cast<u2_any*>(p) = r;
+}
+template <bool STREAM>
+__device__ __forceinline__ void get(const void* p, u4_any& r) {
+  if (STREAM) {
+    const v4_any v = __builtin_nontemporal_load(reinterpret_cast<const v4_any*>(p));
+    r = u4_any{v[0], v[1], v[2], v[3]};
+  } else {
+    r = *reinterpret_cast<const u4_any*>(p);
+  }
+}
+template <bool STREAM>
+__device__ __forceinline__ void get(const void* p, u2_any& r) {
+  if (STREAM) {
+    const v2_any v = __builtin_nontemporal_load(reinterpret_cast<const v2_any*>(p));
+    r = u2_any{v[0], v[1]};
+  } else {
+    r = *reinterpret_cast<const u2_any*>(p);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[traits<T>::VEC]) {
   traits<T>::unpack(*reinterpret_cast<const u4_any*>(p), v);
 }
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[traits<T>::VEC]) {
-  *reinterpret_cast<u4_any*>(p) = traits<T>::pack(v);
+  put<STREAM>(p, traits<T>::pack(v));
 }
 
 // base + offset in bytes, base the same for the whole wave: one 32-bit register per lane for the address

@@ -466,6 +466,46 @@ def test_clouds_of_many_points(dev):
     assert torch.equal(got[0], want[0].transpose(1, 2)) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
 
 
+@pytest.mark.parametrize("dt,rows,C", [(torch.bfloat16, 690001, 99), (torch.float32, 1050003, 33), (torch.float16, 130007, 601),
+                                       (torch.bfloat16, 17000001, 5), (torch.bfloat16, 33001, 2050)])
+def test_tensors_larger_than_the_caches(dev, dt, rows, C):
+    """Rows of large tensors, which are read and written past the caches, are those of a small one bit for bit."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = torch.randn(rows, C, device=dev, generator=g).to(dt)
+    dy = torch.randn(rows, C, device=dev, generator=g).to(dt)
+    w, b = torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    y, mean, rstd = ln.layer_norm_forward(x, w, b, relu=True)
+    dx = ln.layer_norm_backward(dy, x, w, b, mean, rstd, relu=True, need_dparams=False)[0]
+    y8, s = ln.layer_norm_forward8(x, w, b, relu=True)
+    dx8 = ln.layer_norm_backward8(dy, s, w, need_dparams=False)[0]
+    held = act8.act8_unpack(s.act, dt)
+    for i in (0, rows // 2, rows - 1000):
+        k = slice(i, i + 1000)
+        ys, ms, rs = ln.layer_norm_forward(x[k], w, b, relu=True)
+        y8s, ss = ln.layer_norm_forward8(x[k], w, b, relu=True)
+        assert torch.equal(y[k], ys) and torch.equal(mean[k], ms) and torch.equal(rstd[k], rs) and torch.equal(y8[k], y8s)
+        assert torch.equal(dx[k], ln.layer_norm_backward(dy[k], x[k], w, b, ms, rs, relu=True, need_dparams=False)[0])
+        assert torch.equal(dx8[k], ln.layer_norm_backward8(dy[k], ss, w, need_dparams=False)[0])
+        assert torch.equal(s.act.codes[k], ss.act.codes) and torch.equal(held[k], act8.act8_unpack(ss.act, dt))
+
+
+@pytest.mark.parametrize("dt,B,C,M", [(torch.bfloat16, 3, 99, 240001), (torch.float32, 2, 300, 60002), (torch.bfloat16, 2, 1100, 31003),
+                                      (torch.float16, 1, 2100, 33001)])
+def test_channel_tensors_larger_than_the_caches(dev, dt, B, C, M):
+    g = torch.Generator("cuda").manual_seed(M)
+    x = torch.randn(B, C, M, device=dev, generator=g).to(dt)
+    dy = torch.randn(B, C, M, device=dev, generator=g).to(dt)
+    w, b = torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    y, mean, rstd = ln.layer_norm_forward(x, w, b, channel_dim=1, relu=True)
+    dx = ln.layer_norm_backward(dy, x, w, b, mean, rstd, channel_dim=1, relu=True, need_dparams=False)[0]
+    for c, i in ((0, 0), (B - 1, M // 3), (B - 1, M - 1000)):
+        k = slice(i, i + 1000)
+        xs, ds = x[c:c + 1, :, k].contiguous(), dy[c:c + 1, :, k].contiguous()
+        ys, ms, rs = ln.layer_norm_forward(xs, w, b, channel_dim=1, relu=True)
+        assert torch.equal(y[c, :, k], ys[0]) and torch.equal(mean.view(B, M)[c, k], ms)
+        assert torch.equal(dx[c, :, k], ln.layer_norm_backward(ds, xs, w, b, ms, rs, channel_dim=1, relu=True, need_dparams=False)[0][0])
+
+
 def test_refusals(dev):
     x = torch.randn(4, 8, device=dev)
     w = torch.ones(8, device=dev)
