@@ -146,7 +146,7 @@ __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 49 us with the sum of 512 partial tiles, 5.2 TB/s).
+// What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 45 us with the sum of 512 partial tiles, 5.6 TB/s).
 // For wide ones how much the two waves of a SIMD overlap: a step of 64 rows of the 256 x 128 tile keeps the matrix pipes busy
 // for 45 % of its cycles, LDS (176 KB) for 45 %, the vector units for 22 %.  12288 rows, 512 x 1536 take 34 us with the sum
 // of the 33 MB of partial tiles, 556 TFLOP/s; 98304 rows, 512 x 512 76 us, 675 TFLOP/s (the library's bf16 product: 81 and
@@ -167,7 +167,7 @@ __device__ __forceinline__ uint4 shift_down(const rv::u4_any& v, int skip) {
 // Every load is whole and unconditional -- rows behind the last repeat it (their dY is zeroed and their scale set to 1 when
 // they are staged), columns behind the last repeat others and end in columns of the tile that are not stored -- and its
 // address is a base the workgroup shares plus a 32-bit offset.  RAGGED: M is no multiple of 8.
-template <int MB, int NB, int WM, int WN, int ROWS, bool RAGGED>
+template <int MB, int NB, int WM, int WN, int ROWS, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_kernel(
     long long rows, int M, int N, const bf16* __restrict__ dY, int dys, const signed char* __restrict__ codes, int pitch,
     const unsigned char* __restrict__ scales, float* __restrict__ out, int S, int tiles_n) {
@@ -232,13 +232,15 @@ __global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_k
         for (int e = 0; e < 8; ++e) v[e] = p[min(e, M - 1)].u;
         h.a[i] = rv::u4_any{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
       } else {
-        h.a[i] = *reinterpret_cast<const rv::u4_any*>(p);
+        rv::get<STREAM>(p, h.a[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
       const int r = last_step ? min(br[i], rest - 1) : br[i];
-      h.b[i] = *reinterpret_cast<const uint4*>(rv::at32(pb, __umul24(r, pitch) + bc[i]));
+      rv::u4_any b;
+      rv::get<STREAM>(rv::at32(pb, __umul24(r, pitch) + bc[i]), b);
+      h.b[i] = make_uint4(b.x, b.y, b.z, b.w);
       h.s[i] = *rv::at32(ps, __umul24(r, G) + bc[i] / rv::GROUP);
     }
   };
@@ -518,27 +520,37 @@ extern "C" int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, lo
   const int tn = pvn3d_ceil_div(N, p.tn);
   const long long blocks = (long long)pvn3d_ceil_div(M, p.tm) * tn * p.S;
   if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidValue;
-#define A8_ONE(MB, NB, WM, WN, ROWS, RAG)                                                                                   \
-  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN, ROWS, RAG>), dim3((unsigned)blocks),                                \
+  // a single tile reads its rows once (1572864 x 64 x 32: 45.3 us past the caches, 48.0; tiles that waves share are the slower
+  // for it, 800000 x 100 x 100 60, 57)
+  const bool once = p.kind >= 4 && blocks == p.S && rows * (2 * M + (long long)N) >= rv::STREAM_BYTES;
+#define A8_ONE(MB, NB, WM, WN, ROWS, RAG, STREAM)                                                                           \
+  hipLaunchKernelGGL((act8_wgrad_kernel<MB, NB, WM, WN, ROWS, RAG, STREAM>), dim3((unsigned)blocks),                                \
                      dim3(WM * WN > 1 ? 64 * WM * WN : 256), 0, A8_ST, rows, M, N, (const bf16*)dY, (int)dys,               \
                      (const signed char*)codes, (int)pitch, (const unsigned char*)scales, out, p.S, tn)
-#define A8_CALL(MB, NB, WM, WN, ROWS)                 \
-  do {                                                \
-    if (M & 7) A8_ONE(MB, NB, WM, WN, ROWS, true);    \
-    else A8_ONE(MB, NB, WM, WN, ROWS, false);         \
+#define A8_CALL(MB, NB, WM, WN, ROWS)                        \
+  do {                                                       \
+    if (M & 7) A8_ONE(MB, NB, WM, WN, ROWS, true, false);    \
+    else A8_ONE(MB, NB, WM, WN, ROWS, false, false);         \
+  } while (0)
+#define A8_NARROW(MB, NB)                                    \
+  do {                                                       \
+    if (!once) A8_CALL(MB, NB, 1, 1, 32);                    \
+    else if (M & 7) A8_ONE(MB, NB, 1, 1, 32, true, true);    \
+    else A8_ONE(MB, NB, 1, 1, 32, false, true);              \
   } while (0)
   switch (p.kind) {
     case 0: A8_CALL(2, 2, 4, 2, 64); break;
     case 1: A8_CALL(2, 2, 2, 2, 64); break;
     case 2: A8_CALL(1, 2, 2, 2, 64); break;
     case 3: A8_CALL(2, 1, 2, 2, 64); break;
-    case 4: A8_CALL(2, 2, 1, 1, 32); break;
-    case 5: A8_CALL(2, 1, 1, 1, 32); break;
-    case 6: A8_CALL(1, 2, 1, 1, 32); break;
-    default: A8_CALL(1, 1, 1, 1, 32); break;
+    case 4: A8_NARROW(2, 2); break;
+    case 5: A8_NARROW(2, 1); break;
+    case 6: A8_NARROW(1, 2); break;
+    default: A8_NARROW(1, 1); break;
   }
 #undef A8_ONE
 #undef A8_CALL
+#undef A8_NARROW
   PVN3D_LAUNCH_CHECK();
   return p.S > 1 ? rv::fold(p.S, count, count, (const float*)workspace, dW, nullptr, A8_ST) : 0;
 }

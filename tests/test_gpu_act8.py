@@ -120,7 +120,8 @@ def test_weight_gradient(dev, rows, M, N):
     assert torch.equal(dw, act8.linear8_weight_grad(wide[:, 5:5 + M], act8.Act8(other[:, :N], act.scales)))
 
 
-@pytest.mark.parametrize("rows,M,N", [(100003, 20, 130), (70000, 130, 20), (50001, 200, 300), (33000, 100, 100), (90001, 40, 70)])
+@pytest.mark.parametrize("rows,M,N", [(100003, 20, 130), (70000, 130, 20), (50001, 200, 300), (33000, 100, 100), (90001, 40, 70),
+                                      (1500001, 41, 30), (1400003, 64, 32), (2200000, 20, 50), (2000011, 32, 32)])
 def test_weight_gradient_of_many_splits(dev, rows, M, N):
     """Split counts of every tile shape at their largest."""
     test_weight_gradient(dev, rows, M, N)
