@@ -19,7 +19,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // tpr threads across a row (a power of two that covers the row, or whole groups of it), 256 / tpr rows a pass and two passes
 // in flight.  Chunks are windows (rowvec.h), addresses a base the workgroup shares plus a 32-bit offset; a row shorter than a
 // chunk is read value by value.  LPG: lanes per group, fewer than a whole group's if the row is shorter.
-// Bound by HBM: bf16 786432 x 96 packed in 43 us (5.4 TB/s), unpacked in 36 us (6.4 TB/s, partly from the cache behind L2).
+// Bound by HBM: bf16 786432 x 96 packed in 38 us (6.0 TB/s), unpacked in 34 us (6.8 TB/s, partly from the cache behind L2).
 constexpr int FLY = 2;
 
 template <typename T, int LPG>

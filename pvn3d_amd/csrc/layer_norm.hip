@@ -22,7 +22,7 @@ using rv::traits;
 using ln::row_sum;
 
 // Bound by HBM: x read once, y written once.  bf16 1572864 x 64: 68 us = 5.9 TB/s (a large copy on this card: 4.9);
-// 393216 x 196 with x put away in 8 bits and ReLU bits, 84 us = 4.8 TB/s (lanes behind the row's end and the codes'
+// 393216 x 196 with x put away in 8 bits and ReLU bits, 78 us = 5.1 TB/s (lanes behind the row's end and the codes'
 // arithmetic cost the rest).  128 x 512, a call whose cost is its launch: 3.6 us.  What it took: the parameters loaded in
 // vectors (with a load per value 98304 x 1024 took 237 us, now 74), the loads of both rows ahead of any wait, addresses as a
 // shared base plus 32-bit offsets instead of a 64-bit product per row and tensor, sums over lanes in registers.

@@ -2,12 +2,12 @@
 // hand features on.  The formulas are those of layer_norm.hip.
 //
 // A tile is 64 (32, 16) consecutive points of one cloud: PX = 16 (8, 4) lanes x 4 points across, blockDim.x / PX channel
-// slots down.  A thread holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at each use), so memory
-// is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
+// slots down.  A thread holds channels cy, cy + CY, ... (KC of them) of its four points in registers, as loaded (unpacked at
+// each use), so memory is read once.  All addresses are a base that the workgroup shares plus one 32-bit offset per lane (64-bit addresses for
 // every channel were half of the registers).  The sums over the channels go through two lane exchanges and one LDS
 // exchange; two LDS buffers in turn, one barrier per sum.  KC = 0: more channels than the registers of 1024 threads hold
 // -- x is read again for every pass.
-// Bound by HBM.  fp32 24 x 128 x 12288 forward 61 us = 5.0 TB/s; bf16 8 x 196 x 16384 backward 38 us = 4.0 TB/s (two
+// Bound by HBM.  fp32 24 x 128 x 12288 forward 56 us = 5.4 TB/s; bf16 8 x 196 x 16384 backward 38 us = 4.0 TB/s (two
 // workgroups a CU load, add up and store in turn).
 #include "layer_norm.h"
 

@@ -13,8 +13,8 @@ constexpr int ACROSS = 2;                            // chunks across of a colum
 // ------------------------------------------------------------------------------------------------ rows, backward
 // As the forward; a thread's channels are the same for all its rows, so dw and db are summed in its registers over the
 // rows of the workgroup, then over the workgroup's row slots (shuffles, LDS) into part[workgroup][2][C].
-// Bound by HBM: dy and x read, dx written, once each.  bf16 786432 x 128: 115 us = 5.2 TB/s; 393216 x 196 from 8 bits: 100 us
-// = 4.0 TB/s (25 of 32 lanes have a chunk; 8 small loads a row); the sum of the partials another 5 us.
+// Bound by HBM: dy and x read, dx written, once each.  bf16 786432 x 128: 104 us = 5.8 TB/s; 393216 x 196 from 8 bits: 88 us
+// = 4.5 TB/s (25 of 32 lanes have a chunk); the sum of the partials another 5 us.
 // FROM8: code 2^e - mean is one fma (code 2^e is exact), with the rounding that x - mean has.
 template <typename T, int TPR, int K, int R, bool FROM8, bool STREAM>
 __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C, const T* __restrict__ dy, int dys,
@@ -196,7 +196,8 @@ __global__ __launch_bounds__(256) void ln_rows_grad_kernel(long long rows, int C
           const float xh = v[k][i], dz = d[k][i];
           aw[k][i] = fmaf(dz, xh, aw[k][i]);
           ab[k][i] += dz;
-          asm volatile("" : "+v"(aw[k][i]), "+v"(ab[k][i]));     // summed here: put off behind the row's sums, the terms stay alive
+          // summed here: put off behind the row's sums, the terms stay alive
+          asm volatile("" : "+v"(aw[k][i]), "+v"(ab[k][i]));
           const float u = dz * g[k][i], um = u * col.own[k][i];
           s1 += um;
           s2 = fmaf(um, xh, s2);
@@ -270,10 +271,11 @@ int rows_grad_columns(int dtype, long long rows, int C) {
 }
 
 // Workgroups of a rows backward launch = its partial sums: `per` a CU, as many as keep memory busy and no more, each with
-// four rows at least where it takes a row at a time.  A CU (dx, dweight, dbias from x / from 8 bits, us):
-//   one chunk a lane   bf16 786432 x 128: 3 118 / 112, 4 120 / 108, 6 131 / 112;  fp32 393216 x 128: 3 115 / 95, 4 115 / 92, 8 124 / 101
-//   two, a wave a row  bf16 46000 x 753: 2 48 / 51, 3 45 / 48, 4 57 / 57;  fp32 98304 x 512: 2 116 / 91, 3 118 / 92, 5 124 / 95
-//   two, a workgroup   bf16 16384 x 4000: 2 90 / 92, 3 98 / 90, 4 124 / 109;  fp32 10000 x 1501: 2 43 / 43, 3 41 / 38, 5 46 / 41
+// four rows at least where it takes a row at a time.  A CU (dx, dweight, dbias from x / from 8 bits, us; all cached):
+//   one chunk a lane   bf16 786432 x 128: 3 118 / 112, 4 120 / 108, 6 131 / 112
+//                      fp32 393216 x 128: 3 115 / 95, 4 115 / 92, 8 124 / 101
+//   two, a wave a row  bf16 46000 x 753: 2 48 / 51, 3 45 / 48, 4 57 / 57;  fp32 98304 x 512: 2 116 / 91, 3 118 / 92
+//   two, a workgroup   bf16 16384 x 4000: 2 90 / 92, 3 98 / 90, 4 124 / 109;  fp32 10000 x 1501: 2 43 / 43, 3 41 / 38
 //   four, eight        fp32 8192 x 4096: 1 93 / 80, 2 87 / 70, 4 97 / 81;  bf16 4096 x 8192: 1 67 / 65, 2 81 / 80
 int rows_grad_parts(int dtype, long long rows, int C) {
   const int vec = ln::vec_of(dtype), tpr = ln::rows_threads(C, vec), k = (C + tpr * vec - 1) / (tpr * vec);
