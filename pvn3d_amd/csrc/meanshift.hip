@@ -241,8 +241,8 @@ struct MsAcc {
 
 // A staged point record is (x', y', -|a'|^2, z'): the register pairs (x', y') and (-|a'|^2, z').
 //
-// Operand placement of the packed path is hand-written, for a measured reason (round 5, tools/sg_fault_repro.hip
-// variant 20, tools/ms_beside_mfma.py, profiles/r05_pk_opsel_fault.txt): on gfx950 a packed-fp32 instruction whose
+// Operand placement of the packed path is hand-written, for a measured reason (tools/ms_beside_mfma.py,
+// profiles/r05_pk_opsel_fault.txt): on gfx950 a packed-fp32 instruction whose
 // LOW half selects the HIGH register of a VGPR pair in its src1 or src2 position (op_sel bit 1 / bit 2) returns that
 // operand as +0 in lanes 48-63 now and then WHILE the other wave of its SIMD runs an MFMA / LDS K loop -- i.e. while a
 // kernel of the MLP stream shares the SIMD.  (The compiler's own code for ms_splat(a.y) was exactly that form, and a

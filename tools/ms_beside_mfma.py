@@ -1,7 +1,7 @@
 #!/usr/bin/env python
 """Do kernels keep their bits when kernels of the other island run on the same SIMDs?
 
-tools/sg_fault_repro.hip pinned the round-4 split-GEMM epilogue fault to a packed-fp32 VALU instruction whose low half
+profiles/r05_pk_opsel_fault.txt pins a wrong split-GEMM epilogue to a packed-fp32 VALU instruction whose low half
 selects the HIGH register of a source pair (`v_pk_mul_f32 ... op_sel:[0,1]`): it returned +0 in lanes 48-63 now and then
 -- but only while the second wave of its SIMD was inside an MFMA / LDS K loop.  The MeanShift iteration kernel is built
 from packed-fp32 instructions with such selectors (csrc/meanshift.hip), and in bench.py's pipelined step it runs beside

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Lint the gfx950 ISA of every translation unit for the packed-fp32 operand form that goes wrong on MI355X.
 
-Measured (round 5; tools/sg_fault_repro.hip variant 20, tools/ms_beside_mfma.py; profiles/r05_pk_opsel_fault.txt): a
+Measured (profiles/r05_pk_opsel_fault.txt, tools/ms_beside_mfma.py): a
 VOP3P packed-fp32 instruction (v_pk_mul_f32 / v_pk_add_f32 / v_pk_fma_f32) whose LOW result half takes the HIGH register
 of a VGPR pair in its src1 or src2 position -- op_sel:[_,1] / op_sel:[_,_,1] -- reads that operand as +0 in lanes 48-63
 now and then while the other wave of its SIMD is inside an MFMA / LDS K loop.  Never observed for: the src0 position,
