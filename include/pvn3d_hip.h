@@ -679,6 +679,11 @@ int pvn3d_act8_unpack(int dtype, long long rows, int C, const void* codes, long 
 size_t pvn3d_act8_wgrad_workspace_bytes(long long rows, int M, int N);
 int pvn3d_act8_wgrad(long long rows, int M, int N, const void* dY, long long dys, const void* codes, long long pitch,
                      const void* scales, float* dW, void* workspace, size_t workspace_bytes, void* stream);
+/* dW [M][K] fp32 = dY^T X for K <= 8 bf16 columns X [rows] of stride xs (elements, any alignment) that are kept as they are
+ * beside codes; otherwise as pvn3d_act8_wgrad. */
+size_t pvn3d_act8_columns_workspace_bytes(long long rows, int M, int K);
+int pvn3d_act8_columns_wgrad(long long rows, int M, int K, const void* dY, long long dys, const void* X, long long xs,
+                             float* dW, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -120,6 +120,8 @@ SIGNATURES = {
     "pvn3d_act8_unpack": (_i, [_i, _ll, _i, _p, _ll, _p, _p, _ll, _i, _p]),
     "pvn3d_act8_wgrad_workspace_bytes": (_sz, [_ll, _i, _i]),
     "pvn3d_act8_wgrad": (_i, [_ll, _i, _i, _p, _ll, _p, _ll, _p, _p, _p, _sz, _p]),
+    "pvn3d_act8_columns_workspace_bytes": (_sz, [_ll, _i, _i]),
+    "pvn3d_act8_columns_wgrad": (_i, [_ll, _i, _i, _p, _ll, _p, _ll, _p, _p, _sz, _p]),
 }
 
 if not os.path.exists(LIB_PATH):

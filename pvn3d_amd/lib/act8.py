@@ -9,6 +9,8 @@ value x is held as the int8 code rint(x 2^-e); e >= -126 is the smallest exponen
 rounds to 127 at most, held as e + 127 in a byte (e <= 121: magnitudes from 127.5 2^121 on are held as 127 2^121).  A value
 is off by at most half a step, 1/128 of its group's largest magnitude (half of 2^-126 in a group smaller than that); every
 held value is exact in bfloat16.  A group that holds an infinity or a NaN comes back as NaN.
+The error is relative to the group: channels much smaller than others of their 32 (coordinates beside features) are held
+coarsely or as zeros, and a weight's gradient is lost with its input.  Such columns do not belong in this form.
 
 Everything runs on the current stream of the tensors' device and reads only its arguments; calls may be captured."""
 import torch
@@ -187,6 +189,27 @@ def linear8_weight_grad(dy, act):
         codes, scales = act._ptrs()
         check(lib.pvn3d_act8_wgrad(rows, M, N, m.data_ptr(), ds, codes, act.pitch, scales, dw.data_ptr(),
                                    ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_wgrad")
+    return dw
+
+
+MAX_COLUMNS = 8             # of _columns_weight_grad
+
+
+def _columns_weight_grad(dy, x):
+    """dW (M, K) float32 = dy^T x for a few columns that are kept in bfloat16 beside the codes: dy (rows, M), x (rows, K),
+    K <= 8, both bfloat16.  fp32 sums in a fixed order, like linear8_weight_grad."""
+    _need(dy.is_cuda and x.device == dy.device, "x must be on dy's device")
+    _need(dy.dtype is torch.bfloat16 and x.dtype is torch.bfloat16, "dy and x must be bfloat16 tensors")
+    _need(dy.dim() == 2 and x.dim() == 2 and dy.size(0) == x.size(0), "dy and x must have the same number of rows")
+    rows, M, K, dev = dy.size(0), dy.size(1), x.size(1), dy.device
+    _need(M > 0 and 0 < K <= MAX_COLUMNS, "dy must have at least one channel, x 1 to %d" % MAX_COLUMNS)
+    with on_device(dev):
+        (m, ds), (v, xs) = _rows(dy), _rows(x)
+        dw = torch.empty(M, K, dtype=torch.float32, device=dev)
+        wsb = lib.pvn3d_act8_columns_workspace_bytes(rows, M, K)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        check(lib.pvn3d_act8_columns_wgrad(rows, M, K, m.data_ptr(), ds, v.data_ptr(), xs, dw.data_ptr(),
+                                           ws.data_ptr() if wsb else None, wsb, _stream(dy)), "act8_columns_wgrad")
     return dw
 
 

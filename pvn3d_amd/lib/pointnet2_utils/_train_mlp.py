@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 
 from ..._lib import lib, check, on_device
-from ..act8 import Act8, act8_pack, linear8_weight_grad
+from ..act8 import MAX_COLUMNS, Act8, _columns_weight_grad, act8_pack, linear8_weight_grad
 from ..layer_norm import LayerNorm, Saved8
 from . import _ext
 
@@ -34,6 +34,8 @@ TRAIN_FUSED = "auto"
 #   True: their 8-bit form (lib/act8.py) -- 33/32 bytes per value instead of 2, the weight gradients are taken from it (a
 #         value is off by at most 1/128 of the largest of its 32 channels); layers with a LayerNorm keep the norm's input
 #         that way too, with one bit per value for the ReLU.  Outputs, and with BatchNorm the input gradients, do not change.
+#         What enters a chain beside features of a layer stays bf16, because it has a scale of its own: the neighbours'
+#         relative coordinates, and features that take no gradient (colours and normals of the cloud).
 ACT_CKPT8 = False
 
 
@@ -109,22 +111,46 @@ def _is_ln(layers):
     return isinstance(layers[0][1], LayerNorm)
 
 
+def _pieces(*parts):
+    """parts: (channels, whether they are features of a layer) of a chain's input in their order -> [(first, end, learned)]
+    with neighbours of a kind joined, or None where the input is kept as it is: no learned channels, or more exact ones in a
+    piece than their weight gradient takes."""
+    out, at = [], 0
+    for n, learned in parts:
+        if n > 0:
+            if out and out[-1][2] == bool(learned):
+                out[-1] = (out[-1][0], at + n, bool(learned))
+            else:
+                out.append((at, at + n, bool(learned)))
+            at += n
+    if not any(p[2] for p in out) or any(not p[2] and p[1] - p[0] > MAX_COLUMNS for p in out):
+        return None
+    return out
+
+
 class _Chain(object):
     """Forward / backward of one [GEMM -> BatchNorm(batch stats) -> ReLU] x L chain on a point-major bf16 input
-    X0 (rows, ld0).  Holds what the backward needs."""
+    X0 (rows, ld0).  Holds what the backward needs.  pieces: which channels of X0 may be kept in 8 bits (_pieces)."""
 
-    def __init__(self, x0, c_in, weights, gammas, betas, bns):
+    def __init__(self, x0, c_in, weights, gammas, betas, bns, pieces):
         self.dev = x0.device
         self.rows = x0.size(0)
         self.x0 = x0                     # the forward's input; given up once it is kept in `inputs`
         self.c = [int(c_in)] + [int(w.size(0)) for w in weights]
         self.weights, self.gammas, self.betas, self.bns = weights, gammas, betas, bns
         self.ckpt8 = bool(ACT_CKPT8)
-        self.inputs = []                 # per layer, for its weight gradient: the bf16 matrix or its Act8
+        self.pieces = pieces
+        self.inputs = []                 # per layer, for its weight gradient: the bf16 matrix, its Act8 or a list of pieces
         self.y, self.mean = [], []
 
     def _keep_input(self, li, prev):
-        self.inputs.append(act8_pack(prev[:, :self.c[li]]) if self.ckpt8 else prev)
+        if not self.ckpt8 or (li == 0 and self.pieces is None):
+            self.inputs.append(prev)
+        elif li == 0 and len(self.pieces) > 1:
+            self.inputs.append([act8_pack(prev[:, a:b]) if learned else prev[:, a:b].contiguous()
+                                for a, b, learned in self.pieces])
+        else:
+            self.inputs.append(act8_pack(prev[:, :self.c[li]]))
 
     def _product(self, li, prev, y, ps, st):
         """y = prev . W_li^T; ps: partial column sums for BatchNorm, or None."""
@@ -190,6 +216,9 @@ class _Chain(object):
         prev = self.inputs[li]
         if isinstance(prev, Act8):
             return linear8_weight_grad(dy[:, :cout], prev)
+        if isinstance(prev, list):
+            return torch.cat([linear8_weight_grad(dy[:, :cout], p) if isinstance(p, Act8) else
+                              _columns_weight_grad(dy[:, :cout], p) for p in prev], 1)
         dw = torch.zeros((cout, cin), dtype=torch.float32, device=dev)
         if WGRAD_TN and lib.pvn3d_mt_wgrad_tn_ok(cout, cin):
             # straight from the row-major matrices (no transposed copies)
@@ -351,8 +380,8 @@ class _LNChain(_Chain):
         return dh, dws, dgs, dbs
 
 
-def _chain(x0, c_in, weights, gammas, betas, layers):
-    return (_LNChain if _is_ln(layers) else _Chain)(x0, c_in, weights, gammas, betas, [norm for _, norm in layers])
+def _chain(x0, c_in, weights, gammas, betas, layers, pieces):
+    return (_LNChain if _is_ln(layers) else _Chain)(x0, c_in, weights, gammas, betas, [norm for _, norm in layers], pieces)
 
 
 # Backward of the layer-0 gathers through inverted index lists (csrc/mlp_train.hip mt_csr_build / mt_inv_gather)
@@ -418,7 +447,7 @@ class SALevelTrain(torch.autograd.Function):
                 check(lib.pvn3d_mt_gather_sa(B, N, m, ns, C, 1 if use_xyz else 0, xyz.data_ptr(), new_xyz.data_ptr(), fp,
                                              fsb, fsc, fsn, idx.data_ptr(), x0.data_ptr(), _ld(c0), _stream(xyz)),
                       "mt_gather_sa")
-                ch = _chain(x0, c0, ws, gs, bs, layers)
+                ch = _chain(x0, c0, ws, gs, bs, layers, _pieces((nx, False), (C, C > 0 and features.requires_grad)))
                 del x0
                 arg = torch.empty((B * m, _ld(width)), dtype=torch.uint8, device=dev)
                 ch.forward(pool=(B * m, ns, out.data_ptr() + 4 * off, total, arg))
@@ -493,7 +522,8 @@ class FPTrain(torch.autograd.Function):
             up, usb, usc, usn = _strides3(uf) if uf is not None else (None, 0, 0, 0)
             check(lib.pvn3d_mt_gather_fp(B, n, mk, C2, C1, kp, ksb, ksc, ksn, up, usb, usc, usn, idx.data_ptr(),
                                          weight.data_ptr(), x0.data_ptr(), _ld(c0), st), "mt_gather_fp")
-            ch = _chain(x0, c0, ws, gs, bs, layers)
+            ch = _chain(x0, c0, ws, gs, bs, layers, _pieces((C2, known_feats.requires_grad),
+                                                            (C1, C1 > 0 and unknow_feats.requires_grad)))
             del x0
             h = ch.forward()
             cout = ch.c[-1]
