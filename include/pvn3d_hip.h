@@ -640,10 +640,11 @@ int pvn3d_mt_bn_bwd_apply(long long rows, int ld, const void* dH, const void* Y,
  * strides (and pitch) of 2^20 elements at most.
  * pvn3d_layer_norm: rows [rows][C] of stride xs (elements, any alignment) -> y [rows] of stride ys; columns C .. y_cols - 1
  *   (y_cols <= C + 15) are written as zeros.  codes != NULL: x also goes to codes / scales in the 8-bit form of
- *   pvn3d_act8_pack, and mask (may be NULL) gets bit c & 7 of byte [row][c / 8], row length ceil(C / 8), = z > 0.
+ *   pvn3d_act8_pack, and mask (may be NULL; with relu only) gets bit c & 7 of byte [row][c / 8], row length ceil(C / 8), = y
+ *   is not 0: z > 0, or NaN (which the ReLU passes on).
  * pvn3d_layer_norm_grad: dx (NULL: not wanted; columns up to dx_cols written, zeros from C on), dweight and dbias (both or
  *   neither).  The normalised input comes from x, or, if codes != NULL, from codes / scales (relu != 0: and the ReLU from
- *   mask, which must then be given; from x it is taken from weight xh + bias > 0).  workspace: the bytes that
+ *   mask, which must then be given; from x it is off where weight xh + bias <= 0).  workspace: the bytes that
  *   pvn3d_layer_norm_grad_workspace_bytes(dtype, rows, C) names, 4-byte aligned, needed for dweight
  *   only.  Sums in a fixed order: the same bits on every call.  No rows: dweight and dbias are zeroed.
  * var + eps has to be a normal fp32 number (a smaller one counts as zero, and its points are not finite).  Outputs do not

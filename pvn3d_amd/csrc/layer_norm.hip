@@ -111,10 +111,11 @@ __global__ __launch_bounds__(256) void ln_rows_kernel(long long rows, int C, con
             rv::store_codes(rv::at32(cb, __umul24(rl, pitch) + c), col.skip[k], wd);
             if ((c & (rv::GROUP - 1)) == 0) *rv::at32(sb, __umul24(rl, G) + c / rv::GROUP) = (unsigned char)sc;
           }
-          if (mask) {                                          // y is 0 or positive here: minus its bits, the sign bit
+          if (mask) {           // y is +0, positive or a NaN of either sign: any bit of it carries into the sign, and stays there
             unsigned bits = 0;
 #pragma unroll
-            for (int i = VEC - 1; i >= 0; --i) bits = __builtin_amdgcn_alignbit(bits, 0u - __float_as_uint(z[i]), 31);
+            for (int i = VEC - 1; i >= 0; --i)
+              bits = __builtin_amdgcn_alignbit(bits, __builtin_elementwise_add_sat(__float_as_uint(z[i]), 0x7fffffffu), 31);
             bits >>= col.skip[k];
             if (VEC == 4 && TPR > 1) {                         // two lanes share a byte
               const unsigned other = rv::dpp(bits, 1);
@@ -174,7 +175,7 @@ extern "C" int pvn3d_layer_norm(int dtype, long long rows, int C, const void* x,
   if (dtype < 0 || dtype > 2 || C <= 0 || C > ln::MAX_C || y_cols < C || y_cols > C + 15 || ys < y_cols || xs < 0)
     return (int)hipErrorInvalidValue;
   if (xs > ln::MAX_STRIDE || ys > ln::MAX_STRIDE || pitch > ln::MAX_STRIDE) return (int)hipErrorInvalidValue;
-  if (codes && (!scales || (pitch & 15) || pitch < C)) return (int)hipErrorInvalidValue;
+  if (codes && (!scales || (pitch & 15) || pitch < C || (mask && !relu))) return (int)hipErrorInvalidValue;
   if (rows <= 0) return 0;
   if (!x || !y || !mean || !rstd) return (int)hipErrorInvalidValue;
   const auto run = dtype == 0 ? rows_forward<float> : dtype == 1 ? rows_forward<bf16> : rows_forward<fp16>;

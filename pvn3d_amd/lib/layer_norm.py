@@ -3,7 +3,7 @@ SharedMLP layers of the reference use (pvn3d/lib/utils/etw_pytorch_utils/pytorch
 point's own, so a rank that trains on one frame computes what one that trains on 24 does.
 
     mean = sum_c x / C    var = sum_c (x - mean)^2 / C    rstd = 1 / sqrt(var + eps)    xh = (x - mean) rstd
-    y = weight xh + bias, with relu: max(y, 0)
+    y = weight xh + bias, with relu: max(y, 0), NaN where y is
 
 x is float32, bfloat16 or float16; statistics, sums and gradients of the parameters are float32 in a fixed order (the same
 bits on every call).  ``channel_dim`` -1: channels last, (..., C), rows of any stride; ``channel_dim`` 1: (B, C, ...), a
@@ -105,7 +105,7 @@ def _check_stats(mean, rstd, n, x):
 
 def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=False, need_dx=True, need_dparams=True):
     """-> (dx like x or None, dweight (C,), dbias (C,) float32 or None, None).  mean, rstd: the forward's; relu: the
-    derivative is taken where weight xh + bias > 0."""
+    derivative is 0 where weight xh + bias <= 0 (a NaN passes, as in the forward)."""
     t = _dtype(x, "x")
     _need(dy.shape == x.shape and dy.dtype == x.dtype and dy.get_device() == x.get_device(), "dy must be like x")
     _need(need_dx or need_dparams, "nothing to compute")
@@ -146,7 +146,7 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, channel_dim=-1, relu=Fa
 
 class Saved8(object):
     """What layer_norm_forward8 keeps for the backward pass: x in 8 bits (`act`), the statistics `mean` and `rstd`, and with
-    a ReLU one bit per value, `mask` (rows, ceil(C / 8)) uint8: bit i of byte j: channel 8 j + i is on.  One buffer: codes,
+    a ReLU one bit per value, `mask` (rows, ceil(C / 8)) uint8: bit i of byte j: channel 8 j + i is on (or NaN).  One buffer: codes,
     scales, mask, statistics; views of it are made when they are asked for."""
     __slots__ = ("act", "dtype", "relu", "_buf", "_mask", "_stat")
 
