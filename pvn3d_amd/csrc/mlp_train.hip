@@ -816,8 +816,8 @@ __global__ void mt_pool_max_kernel(long long G, int ns, int ld, int C, const bf1
     float h[8];
     unpack8(*reinterpret_cast<const uint4*>(H + (g * ns + s) * ld + c0), h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (h[i] > best[i]) { best[i] = h[i]; bi[i] = s; }       // first maximum wins (as ATen's max_pool2d)
+    for (int i = 0; i < 8; ++i)                                // first maximum wins, the last NaN before any (as max_pool2d)
+      if (h[i] > best[i] || h[i] != h[i]) { best[i] = h[i]; bi[i] = s; }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

@@ -39,3 +39,75 @@ def test_a_nan_of_either_sign_passes_the_kept_relu(dev, dt, C):
     got = ln.layer_norm_backward8(dy, s, w)
     for p, q in zip(got, want):
         assert torch.equal(torch.isnan(p), torch.isnan(q))
+
+
+def test_pool_takes_a_nan(dev):
+    """mt_pool_max against max_pool2d, values and indices: one NaN, several, all of a group, infinities, none."""
+    G, ns, C, ld = 9, 7, 21, 32
+    h = torch.randn(G, ns, ld, generator=torch.Generator().manual_seed(0)).clamp_min(0)
+    nan = float("nan")
+    h[1, 3, 2] = nan
+    h[2, 0, :9] = nan
+    h[3, 2, 4] = h[3, 5, 4] = nan
+    h[4] = nan
+    h[5, 6] = nan
+    h[6, 1, 3], h[6, 2, 3] = float("inf"), nan
+    h[7, 1, 3] = float("inf")
+    h[8, :, 5] = -float("inf")
+    h = h.to(torch.bfloat16).to(dev)
+    out = torch.zeros(G, C, device=dev)
+    arg = torch.zeros(G, ld, dtype=torch.uint8, device=dev)
+    check(lib.pvn3d_mt_pool_max(G, ns, ld, C, h.data_ptr(), out.data_ptr(), C, arg.data_ptr(),
+                                torch.cuda.current_stream().cuda_stream), "mt_pool_max")
+    ref = h.float().cpu().permute(0, 2, 1)[:, :C, None]                       # (G, C, 1, ns)
+    want, at = F.max_pool2d(ref, kernel_size=[1, ns], return_indices=True)
+    want, at, out = want[:, :, 0, 0], at[:, :, 0, 0], out.cpu()
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.nan_to_num(out), torch.nan_to_num(want))
+    some = ~torch.isinf(want) | (want > 0)                                    # (a group of -inf has no first maximum above it)
+    assert torch.equal(arg.cpu()[:, :C].long()[some], at[some])
+
+
+def _level(dev, norm):
+    from pvn3d_amd import synth
+    from pvn3d_amd.lib.pointnet2_utils import pointnet2_modules as pm
+    torch.manual_seed(3)
+    mod = pm.PointnetSAModuleMSG(npoint=128, radii=[0.05, 0.1], nsamples=[16, 32], mlps=[[10, 16, 32], [10, 32, 64]],
+                                 norm=norm).to(dev).train()
+    xyz = torch.from_numpy(np.stack([synth.synth_cloud(np.random.default_rng(i), 1024)[0] for i in range(2)], 0)).to(dev)
+    f = torch.randn(2, 10, 1024, device=dev, generator=torch.Generator("cuda").manual_seed(1))
+    return mod, xyz, f
+
+
+def _pass(mod, xyz, f, fused, ckpt8=False):
+    from pvn3d_amd.lib.pointnet2_utils import _train_mlp
+    mod = copy.deepcopy(mod)
+    f = f.clone().requires_grad_()
+    _train_mlp.TRAIN_FUSED, _train_mlp.ACT_CKPT8 = fused, ckpt8
+    try:
+        out = mod(xyz, f)[1]
+        out.sum().backward()
+    finally:
+        _train_mlp.TRAIN_FUSED, _train_mlp.ACT_CKPT8 = "auto", False
+    return out.detach(), {k: v.grad.detach() for k, v in mod.named_parameters()}
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_layer_norm_chain_passes_bad_points_on(dev, bad, ckpt8):
+    """One point that is not finite, and a whole cloud of them: the centres that have it as a neighbour are NaN and no
+    others, and the parameters' gradients show it."""
+    mod, xyz, f = _level(dev, "layer")
+    for where in ("point", "cloud"):
+        g = f.clone()
+        if where == "point":
+            g[0, 4, 17] = bad
+        else:
+            g[1] = bad
+        want, plain = _pass(mod, xyz, g, False)
+        got, grads = _pass(mod, xyz, g, True, ckpt8)
+        assert bool(torch.isnan(want).any()) and torch.equal(torch.isnan(got), torch.isnan(want))
+        assert bool(torch.isfinite(got[~torch.isnan(got)]).all())
+        # (the last layer's dbias is a sum of the output's gradients alone: finite)
+        for k, v in grads.items():
+            assert bool(torch.isnan(v).any()) == bool(torch.isnan(plain[k]).any()), k
+            assert bool(torch.isnan(v).any()) or k.endswith("layer1.normlayer.ln.bias"), k
