@@ -54,8 +54,10 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // H > 0 without reading H: H = bf16(relu(a y + b)) (mt_bn_relu_apply), so the mask is recomputed from y -- the
 // backward passes stream two matrices instead of three
 // (a positive fp32 a y + b rounds to a positive bf16 unless it is a subnormal below 2^-134, where the derivative of
-// the ReLU is 1 anyway)
-__device__ __forceinline__ bool relu_on(float a, float y, float b) { return fmaf(a, y, b) > 0.f; }
+// the ReLU is 1 anyway).  A NaN passes the ReLU, forward and backward, as torch's does: with batch statistics one bad
+// point is every point's.
+__device__ __forceinline__ bool relu_on(float a, float y, float b) { return !(fmaf(a, y, b) <= 0.f); }
+__device__ __forceinline__ float relu(float z) { return __builtin_elementwise_maximum(z, 0.f); }
 // thread index -> (row, 8-channel chunk) and row -> (group, sample) in 32-bit arithmetic (the entry points refuse
 // launches beyond 2^31 chunks; a 64-bit division costs more than the rest of these kernels)
 __device__ __forceinline__ void split_idx(long long t, int cpr, long long& row, int& c0) {
@@ -796,7 +798,7 @@ __global__ void mt_bn_relu_apply_kernel(long long rows, int ld, const bf16_t* __
   const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
   const float bv[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fmaxf(fmaf(av[i], y[i], bv[i]), 0.f);
+  for (int i = 0; i < 8; ++i) y[i] = relu(fmaf(av[i], y[i], bv[i]));
   *reinterpret_cast<uint4*>(H + t * 8) = pack8(y);
 }
 
@@ -1056,8 +1058,8 @@ __global__ void mt_bn_relu_pool_kernel(long long G, int ns, int ld, int C, const
     unpack8(*reinterpret_cast<const uint4*>(Y + (g * ns + s) * ld + c0), y);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float h = bf2f(f2bf(fmaxf(fmaf(aa[i], y[i], bb[i]), 0.f)));
-      if (h > best[i]) { best[i] = h; bi[i] = s; }             // first maximum wins (as ATen's max_pool2d)
+      const float h = bf2f(f2bf(relu(fmaf(aa[i], y[i], bb[i]))));
+      if (h > best[i] || h != h) { best[i] = h; bi[i] = s; }   // first maximum wins, the last NaN before any (as max_pool2d)
     }
   }
 #pragma unroll

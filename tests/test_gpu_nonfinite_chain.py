@@ -111,3 +111,17 @@ def test_layer_norm_chain_passes_bad_points_on(dev, bad, ckpt8):
         for k, v in grads.items():
             assert bool(torch.isnan(v).any()) == bool(torch.isnan(plain[k]).any()), k
             assert bool(torch.isnan(v).any()) or k.endswith("layer1.normlayer.ln.bias"), k
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_batch_norm_chain_passes_bad_points_on(dev, bad, ckpt8):
+    """With batch statistics one point that is not finite makes every centre NaN, and the gradients that show it op by op
+    show it here."""
+    mod, xyz, f = _level(dev, "batch")
+    f[0, 4, 17] = bad
+    want, plain = _pass(mod, xyz, f, False)
+    got, grads = _pass(mod, xyz, f, True, ckpt8)
+    assert bool(torch.isnan(want).any()) and torch.equal(torch.isnan(got), torch.isnan(want))
+    for k, v in grads.items():
+        assert bool(torch.isnan(v).any()) == bool(torch.isnan(plain[k]).any()), k
