@@ -326,11 +326,12 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
         s[PTS + i] = fmaf(u, xh[i], s[PTS + i]);
       }
     };
-    // dx = rstd (u - s1 / C - xh s2 / C), from x: rstd u - (x - mean) rstd^2 s2 / C - rstd s1 / C
+    // dx = rstd (u - s1 / C - xh s2 / C), from x: xh s2 = (x - mean) (rstd s2) -- rstd^2 would leave fp32's range long before
+    // any of these factors does
     auto out = [&](size_t at_c, float g, const float (&v)[PTS], const float (&dz)[PTS]) {
       float e[PTS];
 #pragma unroll
-      for (int i = 0; i < PTS; ++i) e[i] = fmaf(rs[i], dz[i] * g, fmaf(v[i] - mu[i], s[PTS + i], s[i]));
+      for (int i = 0; i < PTS; ++i) e[i] = rs[i] * fmaf(v[i] - mu[i], s[PTS + i], fmaf(dz[i], g, s[i]));
       if (at.live) rv::put<STREAM>(rv::at32(po_ + at_c, o), shut<T>(e).r);
     };
     float v[PTS], d[PTS];
@@ -369,8 +370,8 @@ __global__ __launch_bounds__(MAX_THREADS) void ln_chan_grad_kernel(int tiles, in
     slot_sum<2 * PTS, PX>(s, buf[turn]);
 #pragma unroll
     for (int i = 0; i < PTS; ++i) {
-      s[i] *= -rc * rs[i];
-      s[PTS + i] *= -rc * rs[i] * rs[i];
+      s[i] *= -rc;
+      s[PTS + i] *= -rc * rs[i];
     }
     if (KC > 0) {
 #pragma unroll
