@@ -63,6 +63,14 @@ def _like(m):
     return torch.empty_like(m) if m.is_contiguous() else m.new_empty(m.shape)
 
 
+def _no_view(t):
+    """t's memory as a tensor that is no view: an output of an autograd function that is one cannot be changed in place, as a
+    ReLU(inplace=True) behind the layer does."""
+    if not t._is_view():
+        return t
+    return torch.empty(0, dtype=t.dtype, device=t.device).set_(t.untyped_storage(), t.storage_offset(), t.size(), t.stride())
+
+
 def _align16(n):
     return (n + 15) & ~15
 
@@ -258,7 +266,7 @@ class _Linear8(torch.autograd.Function):
                 ctx.kept, buf = (act.rows, C, act.shape), act._buf
         ctx.save_for_backward(weight, buf)        # (the buffer is given up behind this layer's backward pass)
         ctx.lead = x.shape[:-1]
-        return y.view(x.shape[:-1] + (N,)) if x.dim() != 2 else y
+        return _no_view(y.view(x.shape[:-1] + (N,)) if x.dim() != 2 else y)
 
     @staticmethod
     @once_differentiable

@@ -19,7 +19,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .._lib import lib, check, on_device
-from .act8 import Act8, _dtype, _like, _need, _rows, _stream
+from .act8 import Act8, _dtype, _like, _need, _no_view, _rows, _stream
 
 MAX_CHANNELS = 8192
 _CHANNELS = "layer norm takes 1 to %d channels" % MAX_CHANNELS
@@ -241,10 +241,10 @@ class _LayerNorm(torch.autograd.Function):
                 y, saved = layer_norm_forward8(v, weight, bias, eps, relu)
                 ctx.kept = (saved.act.rows, saved.act.channels, saved.act.shape, saved.dtype, saved.relu)
                 ctx.save_for_backward(weight, saved._buf)
-            return y.movedim(-1, 1) if ctx.moved else y
+            return _no_view(_second(y, x) if ctx.moved else y)
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps, channel_dim, relu)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
-        return y
+        return _no_view(y)
 
     @staticmethod
     @once_differentiable
