@@ -73,17 +73,22 @@ def _strides3(t):
 def _ln_of(norm):
     """The LayerNorm of a SharedMLP layer's norm (channels second, fp32 parameters, ReLU left to the layer), or None."""
     ln = getattr(norm, "ln", None) if norm is not None else None
-    ok = (isinstance(ln, LayerNorm) and ln.channel_dim == 1 and not ln.relu and ln.weight.dtype == torch.float32
-          and ln.bias.dtype == torch.float32)
-    return ln if ok else None
+    return ln if isinstance(ln, LayerNorm) and ln.channel_dim == 1 and not ln.relu else None
 
 
-def shared_mlp_layers(mlp):
+def _readable(p, n, device):
+    """Whether the kernels may read p by its address: n contiguous fp32 values, on `device` if one is given."""
+    return (p.dtype == torch.float32 and p.numel() == n and p.is_contiguous()
+            and (device is None or p.device == device))
+
+
+def shared_mlp_layers(mlp, device=None):
     """SharedMLP -> [(conv, bn)] when every layer is exactly [1x1 Conv2d without bias] -> BatchNorm2d -> ReLU
     (the only form PVN3D builds) with the BatchNorm in training mode (a frozen / eval BatchNorm inside a module that
     is in training mode normalises with its running statistics and must not update them: that composition is left
-    to torch), or [(conv, ln)] when the norm of every layer is a LayerNorm; None otherwise."""
-    out = []
+    to torch), or [(conv, ln)] when the norm of every layer is a LayerNorm; None otherwise.  Parameters of another type, size or
+    device than the kernels read are left to torch too, which converts or refuses them."""
+    out, width = [], None
     for layer in mlp.children():
         names = [n for n, _ in layer.named_children()]
         conv = getattr(layer, "conv", None)
@@ -94,14 +99,18 @@ def shared_mlp_layers(mlp):
                 or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1 or conv.bias is not None
                 or not isinstance(act, nn.ReLU)):
             return None
-        ln = _ln_of(norm)
-        if ln is not None:
-            out.append((conv, ln))
-            continue
-        if (not isinstance(bn, nn.BatchNorm2d) or not bn.affine or not bn.track_running_stats
-                or bn.momentum is None or not bn.training):
+        if (not _readable(conv.weight, conv.out_channels * conv.in_channels, device)
+                or width not in (None, conv.in_channels)):
             return None
-        out.append((conv, bn))
+        width = conv.out_channels
+        ln = _ln_of(norm)
+        if ln is None and (not isinstance(bn, nn.BatchNorm2d) or not bn.affine or not bn.track_running_stats
+                           or bn.momentum is None or not bn.training):
+            return None
+        read = (ln.weight, ln.bias) if ln is not None else (bn.weight, bn.bias, bn.running_mean, bn.running_var)
+        if not all(_readable(p, width, device) for p in read):
+            return None
+        out.append((conv, ln if ln is not None else bn))
     if len({isinstance(n, LayerNorm) for _, n in out}) > 1:
         return None
     return out or None
@@ -588,7 +597,7 @@ def sa_level_train(module, xyz, new_xyz, features, idxs):
     spec, layer_lists = [], []
     c_feat = features.size(1) if features is not None else 0
     for grouper, mlp, idx in zip(module.groupers, module.mlps, idxs):
-        layers = shared_mlp_layers(mlp)
+        layers = shared_mlp_layers(mlp, xyz.device)
         if layers is None or not isinstance(grouper, pointnet2_utils.QueryAndGroup) or idx is None:
             return None
         if (idx.size(2) > (MAX_NSAMPLE_LN if _is_ln(layers) else MAX_NSAMPLE)
@@ -597,6 +606,8 @@ def sa_level_train(module, xyz, new_xyz, features, idxs):
         if features is None and not grouper.use_xyz:
             return None
         use_xyz = grouper.use_xyz or features is None
+        if layers[0][0].in_channels != c_feat + (3 if use_xyz else 0):
+            return None                                   # (torch says so)
         spec.append((idx, use_xyz, layers))
         layer_lists.append(layers)
     out = SALevelTrain.apply(xyz, new_xyz, features, spec, *_flat_params(layer_lists)).transpose(1, 2)
@@ -607,11 +618,11 @@ def sa_level_train(module, xyz, new_xyz, features, idxs):
 
 def fp_train(module, unknow_feats, known_feats, idx, weight):
     """PointnetFPModule.forward in training mode -> (B, C_out, n) (transposed view), or None."""
-    layers = shared_mlp_layers(module.mlp)
+    layers = shared_mlp_layers(module.mlp, known_feats.device)
     if layers is None:
         return None
     c_in = known_feats.size(1) + (unknow_feats.size(1) if unknow_feats is not None else 0)
-    if max([c_in] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16:
+    if layers[0][0].in_channels != c_in or max([c_in] + [conv.out_channels for conv, _ in layers]) > MAX_LD - 16:
         return None
     channel_major = not getattr(module, "_point_major_out", False)
     out = FPTrain.apply(unknow_feats, known_feats, idx.contiguous(), weight.contiguous(), layers, channel_major,
