@@ -10,8 +10,6 @@ reference option: its statistics do not depend on the batch, which a rank that t
 """
 import torch.nn as nn
 
-from ..layer_norm import LayerNorm
-
 
 class _Norm2d(nn.Sequential):
     def __init__(self, channels):
@@ -30,6 +28,7 @@ class LayerNorm2d(nn.Sequential):
 
     def __init__(self, channels):
         super(LayerNorm2d, self).__init__()
+        from ..layer_norm import LayerNorm        # (needs the kernels' library, which this module does not)
         self.add_module("ln", LayerNorm(channels, channel_dim=1))
 
 
