@@ -49,7 +49,7 @@ def _by_rows(x, channel_dim):
     if d == n - 1:
         rows, C = True, x.size(-1)
     else:
-        _need(d == 1, "channel_dim must be 1 or the last dimension")
+        _need(d == 1 and n > 1, "channel_dim must be 1 or the last dimension")
         C = x.size(1)
         # a point-major view in place; fewer points than a chunk of the channel-major kernel, or more than it addresses:
         # as rows of a copy

@@ -1,5 +1,9 @@
 """Argument checks that need no GPU, beside those of test_norm_act8_refusals.py."""
+import pytest
+import torch
+
 from pvn3d_amd._lib import lib
+from pvn3d_amd.lib import layer_norm as ln
 
 P = 4096            # a non-null pointer that no refused call may touch
 
@@ -25,3 +29,11 @@ def test_exact_columns_refuse():
     assert call(M=0) == 0 and call(K=0) == 0
     assert lib.pvn3d_act8_columns_workspace_bytes(0, 8, 3) == 0 and lib.pvn3d_act8_columns_workspace_bytes(4, 8, 9) == 0
     assert lib.pvn3d_act8_columns_workspace_bytes(1 << 20, 8, 3) % (8 * 3 * 4) == 0
+
+
+@pytest.mark.parametrize("shape,channel_dim", [((8,), 1), ((8,), 2), ((4, 8), 0), ((4, 8), 3), ((4, 8, 3), -4), ((4, 8, 3, 2), 2),
+                                               ((), -1)])
+def test_channel_dimensions_that_are_none(shape, channel_dim):
+    """A channel_dim that x has not, or that is neither 1 nor the last one, is an error of the call."""
+    with pytest.raises(RuntimeError):
+        ln._by_rows(torch.zeros(shape), channel_dim)
