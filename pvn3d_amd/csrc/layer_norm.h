@@ -55,11 +55,11 @@ struct lane_cols {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
         float f[4] = {missing, missing, missing, missing};
-        if (p && TPR > 1) {
-          traits<float>::unpack(*reinterpret_cast<const rv::u4_any*>(p + at[k] + i), f);
-        } else if (p) {
+        if (TPR == 1) {                                // nothing behind C: a ReLU's bits there are off
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[j] = i + j < C ? p[i + j] : 0.f;
+          for (int j = 0; j < 4; ++j) f[j] = i + j < C ? p ? p[i + j] : missing : 0.f;
+        } else if (p) {
+          traits<float>::unpack(*reinterpret_cast<const rv::u4_any*>(p + at[k] + i), f);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[k][i + j] = f[j];
