@@ -108,10 +108,6 @@ __device__ __forceinline__ void get(const void* p, u2_any& r) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[traits<T>::VEC]) {
-  traits<T>::unpack(*reinterpret_cast<const u4_any*>(p), v);
-}
 template <typename T, bool STREAM>
 __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[traits<T>::VEC]) {
   put<STREAM>(p, traits<T>::pack(v));
