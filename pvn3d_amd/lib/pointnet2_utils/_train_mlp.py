@@ -108,7 +108,7 @@ def shared_mlp_layers(mlp, device=None):
                            or bn.momentum is None or not bn.training):
             return None
         read = (ln.weight, ln.bias) if ln is not None else (bn.weight, bn.bias, bn.running_mean, bn.running_var)
-        if not all(_readable(p, width, device) for p in read):
+        if not all(p is None or _readable(p, width, device) for p in read):
             return None
         out.append((conv, ln if ln is not None else bn))
     if len({isinstance(n, LayerNorm) for _, n in out}) > 1:

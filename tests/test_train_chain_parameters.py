@@ -39,6 +39,14 @@ def test_parameters_the_kernels_cannot_read(norm):
     assert _train_mlp.shared_mlp_layers(mlp) is None
 
 
+def test_no_running_statistics_to_update():
+    """A BatchNorm whose buffers were taken away trains on the chain like one that has them."""
+    mlp = _mlp("batch")
+    for layer in mlp:
+        layer.normlayer.bn.running_mean = layer.normlayer.bn.running_var = None
+    assert len(_train_mlp.shared_mlp_layers(mlp)) == 2
+
+
 @pytest.mark.parametrize("norm", ["batch", "layer"])
 def test_inputs_of_other_channels(norm):
     """Features that a level was not built for are left to the composition (which refuses them)."""
