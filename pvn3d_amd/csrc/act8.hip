@@ -148,8 +148,8 @@ __device__ __forceinline__ bf16x8 tr_frag(const unsigned short* base, int stride
 
 // What bounds it: HBM for narrow layers (1572864 rows, 64 x 32: 45 us with the sum of 512 partial tiles, 5.6 TB/s).
 // For wide ones how much the two waves of a SIMD overlap: a step of 64 rows of the 256 x 128 tile keeps the matrix pipes busy
-// for 45 % of its cycles, LDS (176 KB) for 45 %, the vector units for 22 %.  12288 rows, 512 x 1536 take 34 us with the sum
-// of the 33 MB of partial tiles, 556 TFLOP/s; 98304 rows, 512 x 512 76 us, 675 TFLOP/s (the library's bf16 product: 81 and
+// for 45 % of its cycles, LDS (176 KB) for 45 %, the vector units for 22 %.  12288 rows, 512 x 1536 take 33.6 us with the sum
+// of the 31.5 MB of partial tiles, 575 TFLOP/s; 98304 rows, 512 x 512 78 us, 661 TFLOP/s (the library's bf16 product: 81 and
 // 311 us; its rate for a large square one: 1257 TFLOP/s).
 constexpr int odd64(int cols) {                                  // row stride in elements: 32 times an odd number
   return ((cols / 32) & 1) ? cols : cols + 32;
@@ -390,8 +390,8 @@ __global__ __launch_bounds__(WM * WN > 1 ? 64 * WM * WN : 256) void act8_wgrad_k
 }
 
 // Tile, rows of a step and number of row splits of a call.  Every split leaves a partial tile that is written and read
-// again, so there are no more workgroups than keep the chip busy: one of eight waves per CU for the 256 x 128 tile (33 MB of
-// partial sums at most; 98304 x 512 x 512: 81 us, 93 us with two per CU), two of four waves for the others (786432 x 96 x 64:
+// again, so there are no more workgroups than keep the chip busy: one of eight waves per CU for the 256 x 128 tile (33.5 MB of
+// partial sums at most; 98304 x 512 x 512: 78 us, 87 us with two per CU), two of four waves for the others (786432 x 96 x 64:
 // 43 us, 55 with one, 54 with three; 1572864 x 32 x 16: 27, 37, 28).  The 256 x 128 tile converts each code for twice the
 // output; up to 128 output channels half of it would be empty (393216 x 128 x 128: 128 x 128).
 struct wg_plan { int kind, tm, tn, S; };

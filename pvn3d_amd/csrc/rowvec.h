@@ -74,8 +74,12 @@ template <> struct traits<fp16> {
 // Tensors that no cache holds until their next use are read and written past the caches (non-temporal): from STREAM_BYTES
 // on, as instances of their own (a choice at run time cost more than it gave).  bf16: forward 1572864 x 64 73.7 us, so 68.4;
 // backward 786432 x 128 117.5, 106; forward and backward with 8 bits kept, 393216 x 196 186, 165.5; pack and unpack
-// 786432 x 96 77.7, 71.  The next kernel counts too: forward of 524288 x 128 (134 MB) and an addition to its result 88 us
-// either way, a product, its backward and an addition 170, 160; of 131072 x 128 24.4 us, 27.4, and 44.4, 46.7.
+// 786432 x 96 77.7, 71.  The next kernel counts too.  With the chain's consumers (rows of 128 bf16 channels; cached, past the caches, us):
+//                                       33 MB   67 MB         100 MB        134 MB        201 MB        402 MB
+//   forward, then the next product      35, 38  58.3, 61.8    78.4, 84.9    106.7, 109.6  163.8, 161.1  317.9, 315.1
+//   forward, product, packing           44, 48  73.8, 76.5    104.3, 107.6  140.9, 143.6  215.9, 216.0  426.0, 426.6
+//   product, backward, product          68, 69  105.8, 110.0  148.1, 151.7  202.8, 193.8  306.0, 285.8  582.5, 557.5
+// The forward alone would change over a little later, the two passes together do so here.
 constexpr long long STREAM_BYTES = 1ll << 27;
 typedef unsigned v4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned v2_any __attribute__((ext_vector_type(2), aligned(2)));

@@ -8,7 +8,8 @@ point's own, so a rank that trains on one frame computes what one that trains on
 x is float32, bfloat16 or float16; statistics, sums and gradients of the parameters are float32 in a fixed order (the same
 bits on every call).  ``channel_dim`` -1: channels last, (..., C), rows of any stride; ``channel_dim`` 1: (B, C, ...), a
 contiguous tensor or a transposed view of a point-major one (read in place).  1 <= C <= 8192.  var + eps has to be a normal
-fp32 number, 1.2e-38 or more: a point of equal values with eps = 0 is not finite.
+fp32 number, 1.2e-38 or more: a point of equal values with eps = 0 is not finite.  A point that holds an infinity or a NaN
+is NaN throughout and its statistics are not finite; the other points are not touched by it.
 
 ``layer_norm`` is the differentiable call and ``LayerNorm`` the module; ``layer_norm_forward`` / ``layer_norm_backward`` are
 the two launches for callers with a backward pass of their own, ``layer_norm_forward8`` / ``layer_norm_backward8`` the same
