@@ -251,7 +251,7 @@ def _product(m, C, weight, transpose):
                                        1 if transpose else 0, wb.data_ptr(), N, ldw, st), "mt_pack_weight")
         check(lib.pvn3d_mt_gemm_nt(m.size(0), N, ldw, a.data_ptr(), lda, wb.data_ptr(), ldw, out.data_ptr(), _ld(N),
                                    None, None, 0, st), "mt_gemm_nt")
-    return out[:, :N]
+    return out if out.size(1) == N else out[:, :N]
 
 
 class _Linear8(torch.autograd.Function):
