@@ -40,6 +40,45 @@ def test_gradient_of_exact_columns_of_nothing_and_refusals(dev):
             act8._columns_weight_grad(a, b)
 
 
+def test_gradient_of_exact_columns_beyond_32_bits(dev):
+    """Row offsets beyond 2^31 elements: a gradient that is one but for a few rows, columns that are zero but for them."""
+    rows, M, K = (1 << 21) + 35, 1032, 3
+    dy = torch.ones((rows, M), dtype=torch.bfloat16, device=dev)
+    x = torch.zeros((rows, K), dtype=torch.bfloat16, device=dev)
+    pick = [0, 1, rows // 2, rows - 33, rows - 2, rows - 1]
+    g = torch.Generator().manual_seed(15)
+    x[pick] = torch.randn(len(pick), K, generator=g).to(torch.bfloat16).to(dev)
+    dy[pick] = torch.randn(len(pick), M, generator=g).to(torch.bfloat16).to(dev)
+    dw = act8._columns_weight_grad(dy, x).double()
+    a, b = dy[pick].double(), x[pick].double()
+    assert bool(((dw - a.t() @ b).abs() <= 8 * 2.0 ** -24 * (a.abs().t() @ b.abs())).all())
+
+
+def test_gradient_of_exact_columns_captured_and_on_two_streams(dev):
+    g = torch.Generator().manual_seed(12)
+    sets = [(torch.randn(r, M, generator=g).to(torch.bfloat16).to(dev), torch.randn(r, K, generator=g).to(torch.bfloat16).to(dev))
+            for r, M, K in ((60000, 64, 3), (50001, 33, 6))]
+    want = [act8._columns_weight_grad(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(act8._columns_weight_grad(*sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want[i]) for i in range(2) for r in got[i])
+    dy, x = sets[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = act8._columns_weight_grad(dy, x)
+    for i in range(4):
+        dy.copy_(torch.randn(dy.shape, generator=g))
+        x.copy_(torch.randn(x.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, act8._columns_weight_grad(dy, x))
+
+
 def _rel(a, b):
     a, b = a.double().flatten(), b.double().flatten()
     return float((a - b).norm() / b.norm())
