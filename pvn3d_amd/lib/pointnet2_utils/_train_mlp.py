@@ -70,16 +70,22 @@ def _strides3(t):
     return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
 
 
-def _ln_of(norm):
-    """The LayerNorm of a SharedMLP layer's norm (channels second, fp32 parameters, ReLU left to the layer), or None."""
-    ln = getattr(norm, "ln", None) if norm is not None else None
-    return ln if isinstance(ln, LayerNorm) and ln.channel_dim == 1 and not ln.relu else None
+def _is_plain_ln(ln):
+    """Whether it is the LayerNorm of a SharedMLP layer: channels second, ReLU left to the layer."""
+    return isinstance(ln, LayerNorm) and ln.channel_dim == 1 and not ln.relu
 
 
-def _readable(p, n, device):
-    """Whether the kernels may read p by its address: n contiguous fp32 values, on `device` if one is given."""
-    return (p.dtype == torch.float32 and p.numel() == n and p.is_contiguous()
-            and (device is None or p.device == device))
+def _value(m, name):
+    """A parameter or buffer of m; an attribute where something (a weight norm) has put one in its place."""
+    if name in m._parameters:
+        return m._parameters[name]
+    return m._buffers[name] if name in m._buffers else getattr(m, name, None)
+
+
+def _readable(p, n, index):
+    """Whether the kernels may read p by its address: n contiguous fp32 values, on device `index` if one is given."""
+    return (p.dtype is torch.float32 and p.numel() == n and p.is_contiguous()
+            and (index is None or p.get_device() == index))
 
 
 def shared_mlp_layers(mlp, device=None):
@@ -87,32 +93,40 @@ def shared_mlp_layers(mlp, device=None):
     (the only form PVN3D builds) with the BatchNorm in training mode (a frozen / eval BatchNorm inside a module that
     is in training mode normalises with its running statistics and must not update them: that composition is left
     to torch), or [(conv, ln)] when the norm of every layer is a LayerNorm; None otherwise.  Parameters of another type, size or
-    device than the kernels read are left to torch too, which converts or refuses them."""
-    out, width = [], None
-    for layer in mlp.children():
-        names = [n for n, _ in layer.named_children()]
-        conv = getattr(layer, "conv", None)
-        norm = getattr(layer, "normlayer", None)
-        bn = getattr(norm, "bn", None) if norm is not None else None
-        act = getattr(layer, "activation", None)
-        if (names[:1] != ["conv"] or not isinstance(conv, nn.Conv2d) or conv.kernel_size != (1, 1)
-                or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1 or conv.bias is not None
-                or not isinstance(act, nn.ReLU)):
-            return None
-        if (not _readable(conv.weight, conv.out_channels * conv.in_channels, device)
-                or width not in (None, conv.in_channels)):
+    device than the kernels read are left to torch too, which converts or refuses them.
+    (Modules and parameters are taken from their dictionaries: an attribute of an nn.Module costs three times that, and a step
+    of one frame waits for the host.)"""
+    out, width, kind = [], None, None
+    index = (device.index if device.type == "cuda" else -1) if device is not None else None
+    for layer in mlp._modules.values():
+        if layer is None:
+            continue
+        parts = layer._modules
+        conv, norm, act = parts.get("conv"), parts.get("normlayer"), parts.get("activation")
+        if (next(iter(parts), None) != "conv" or not isinstance(conv, nn.Conv2d) or conv.kernel_size != (1, 1)
+                or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1
+                or _value(conv, "bias") is not None or not isinstance(act, nn.ReLU) or norm is None
+                or width not in (None, conv.in_channels)
+                or not _readable(_value(conv, "weight"), conv.out_channels * conv.in_channels, index)):
             return None
         width = conv.out_channels
-        ln = _ln_of(norm)
-        if ln is None and (not isinstance(bn, nn.BatchNorm2d) or not bn.affine or not bn.track_running_stats
-                           or bn.momentum is None or not bn.training):
+        n = norm._modules.get("ln")
+        if _is_plain_ln(n):
+            if kind not in (None, "ln"):
+                return None
+            kind = "ln"
+        else:
+            n = norm._modules.get("bn")
+            if (kind not in (None, "bn") or not isinstance(n, nn.BatchNorm2d) or not n.affine or not n.track_running_stats
+                    or n.momentum is None or not n.training):
+                return None
+            kind = "bn"
+            for p in (_value(n, "running_mean"), _value(n, "running_var")):
+                if p is not None and not _readable(p, width, index):
+                    return None
+        if not (_readable(_value(n, "weight"), width, index) and _readable(_value(n, "bias"), width, index)):
             return None
-        read = (ln.weight, ln.bias) if ln is not None else (bn.weight, bn.bias, bn.running_mean, bn.running_var)
-        if not all(p is None or _readable(p, width, device) for p in read):
-            return None
-        out.append((conv, ln if ln is not None else bn))
-    if len({isinstance(n, LayerNorm) for _, n in out}) > 1:
-        return None
+        out.append((conv, n))
     return out or None
 
 

@@ -39,6 +39,16 @@ def test_parameters_the_kernels_cannot_read(norm):
     assert _train_mlp.shared_mlp_layers(mlp) is None
 
 
+@pytest.mark.filterwarnings("ignore")
+def test_weights_that_something_else_holds():
+    """A weight norm replaces the parameter by an attribute of the same name: still the kernels' form."""
+    mlp = _mlp("batch")
+    nn.utils.weight_norm(mlp[0].conv)
+    nn.utils.parametrizations.spectral_norm(mlp[1].conv)
+    layers = _train_mlp.shared_mlp_layers(mlp)
+    assert len(layers) == 2 and layers[0][0].weight.shape == (8, 6, 1, 1)
+
+
 def test_no_running_statistics_to_update():
     """A BatchNorm whose buffers were taken away trains on the chain like one that has them."""
     mlp = _mlp("batch")
