@@ -95,17 +95,22 @@ def _pass(mod, xyz, f, fused, ckpt8=False):
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_layer_norm_chain_passes_bad_points_on(dev, bad, ckpt8):
     """One point that is not finite, and a whole cloud of them: the centres that have it as a neighbour are NaN and no
-    others, and the parameters' gradients show it."""
+    others, and the parameters' gradients show it.  Which centres is taken from the neighbour lists: torch's convolution in
+    the composition may spread a NaN to other points (it depends on the solver that it picks; 608 NaN where 224 belong)."""
     mod, xyz, f = _level(dev, "layer")
+    _, lists = mod.sample_and_query(xyz)
     for where in ("point", "cloud"):
         g = f.clone()
         if where == "point":
             g[0, 4, 17] = bad
         else:
             g[1] = bad
-        want, plain = _pass(mod, xyz, g, False)
+        _, plain = _pass(mod, xyz, g, False)
         got, grads = _pass(mod, xyz, g, True, ckpt8)
-        assert bool(torch.isnan(want).any()) and torch.equal(torch.isnan(got), torch.isnan(want))
+        points = ~torch.isfinite(g).all(1)                                    # (B, N)
+        want = torch.cat([torch.gather(points[:, None].expand(-1, 128, -1), 2, idx.long()).any(2)[:, None].expand(-1, width, -1)
+                          for idx, width in zip(lists, (32, 64))], 1)
+        assert bool(want.any()) and not bool(want.all()) and torch.equal(torch.isnan(got), want)
         assert bool(torch.isfinite(got[~torch.isnan(got)]).all())
         # (the last layer's dbias is a sum of the output's gradients alone: finite)
         for k, v in grads.items():
